@@ -197,6 +197,143 @@ int kllm_tt_gemm_tc(const float *x, int rows, const float *codebook, int n_codes
 int kllm_tt_gemv_noalloc(const float *x, const float *codebook, int n_codes,
                          const uint16_t *idx, int K, int N, float *y, void *stream);
 
+/* ------------------------------------------------ batch serving operators --
+ * What a batch that answers one prompt many times needs next to the greedy
+ * decode above: key/value caches in 8 bits, attention that reads a prefix
+ * which all sequences share once, and tokens drawn from the logits.  None has
+ * a counterpart in the reference (its caches are fp32, its attention one
+ * sequence's, its pick the first maximum: _tape_runner.c:1602-1763).
+ *
+ * All pointers inside these structs are device memory of the calling
+ * thread's current device unless marked "host"; the structs themselves are
+ * host memory and may go away after the call.  Every call launches on
+ * `stream` (a cudaStream_t, NULL = default stream), allocates nothing, never
+ * waits, and may be captured into a CUDA graph.  Returns 0, or non-zero
+ * with kllm_last_error() set and nothing launched. */
+enum {
+    KLLM_KV_F32 = 0,    /* fp32 as it is, no scales */
+    KLLM_KV_I8 = 1,     /* 8-bit integers -127..127 and one scale per row */
+    KLLM_KV_E4M3 = 2    /* 8-bit floats (4 exponent, 3 fraction bits) and one
+                           scale per row */
+};
+
+/* A cache of keys and values: n_seq sequences of up to max_pos positions, a
+ * row of head_dim values per (sequence, kv head, position).
+ * k, v: [n_seq][n_kv][max_pos][head_dim] floats or codes, sequences
+ * seq_stride elements apart; k_scale, v_scale: [n_seq][n_kv][max_pos] floats,
+ * sequences scale_stride apart (unused for KLLM_KV_F32).
+ * A row x is stored as code_i = rn(fl(x_i * fl(Q / a))) and scale = fl(a / Q),
+ * a = max(max |x_i|, 2^-100), Q = 127 (I8) or 448 (E4M3), ties to even (the
+ * scale at most the largest with Q * scale finite), and stands for the values
+ * fl(code_i * scale).  A row that holds an infinity or
+ * a NaN is stored as zeros with a NaN scale: it reads back as NaN.
+ * head_dim is 32, 64 or 128; k and v start on 16 bytes and seq_stride is a
+ * multiple of 16 elements (4 for KLLM_KV_F32). */
+typedef struct {
+    int format;              /* KLLM_KV_* */
+    int n_seq, n_kv, head_dim, max_pos;
+    void *k, *v;
+    float *k_scale, *v_scale;
+    long long seq_stride, scale_stride;
+} kllm_kv_cache;
+
+/* New rows for a cache.  Row r goes to position pos[r] of sequence seq[r]
+ * (seq NULL: of sequence r); with pos NULL the rows are consecutive
+ * positions pos0 + r of sequence 0 (a prompt).  A row whose position or
+ * sequence lies outside the cache (a negative one among them: padding) is
+ * skipped whole.  Two rows must not name the same place.
+ * Head h of row r of q, k and v starts row_stride * r + head_stride * h
+ * floats after q, k and v; k and v are required, n_heads = 0 leaves q out.
+ * With rope_cos and rope_sin
+ * ([rope_rows][head_dim]) q and k are turned as the tape does it
+ * (rotate-half, fp32) by the angles of row position + rope_offset; a row
+ * whose angles lie outside the tables is skipped. */
+typedef struct {
+    int rows;
+    int n_heads;             /* query heads, 0: no q */
+    int pos0;
+    int rope_rows, rope_offset;
+    const int *seq, *pos;
+    const float *q, *k, *v;
+    long long row_stride, head_stride;
+    float *q_out;            /* [rows][n_heads][head_dim] */
+    const float *rope_cos, *rope_sin;   /* both or neither */
+} kllm_kv_rows;
+
+/* Turn q and k, quantise k and v and write them into the cache: one kernel. */
+int kllm_kv_append(const kllm_kv_cache *cache, const kllm_kv_rows *rows, void *stream);
+
+/* Read rows of a cache back as fp32: row r (placed by seq, pos, pos0 as for
+ * kllm_kv_rows) to k and v, head h of it at row_stride * r + head_stride * h.
+ * Rows that lie outside the cache are left as they were. */
+int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int *pos, int pos0,
+                 float *k, float *v, long long row_stride, long long head_stride, void *stream);
+
+/* Attention of one query token per sequence (a decode step) over a prefix
+ * that all sequences share and each sequence's own positions:
+ *   out[i][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - max s),
+ *   s_j = scale * q[i][h] . k_j
+ * for j over the prefix's first prefix_len positions, then the first
+ * own_len[i] positions of sequence i.  Query head h uses kv head
+ * h / (n_heads / n_kv).  The prefix (sequence 0 of `prefix`) is read once
+ * for all sequences.  prefix may be NULL (prefix_len 0), own may be NULL
+ * (every own length 0); where both are given their formats, n_kv and
+ * head_dim agree.  Results are fp32 with fp32 sums in an order of their own.
+ *   own_len[i] < 0      a padding row: out[i] is left as it was
+ *   own_len[i] > own->max_pos or max_len: the smaller of those is taken
+ *   no position at all  out[i] is zeros
+ * max_len is an upper bound of the own lengths (it sizes the launch, so a
+ * captured graph serves every length up to it).  Positions past the lengths
+ * are not read.  workspace: kllm_batch_attention_workspace(a) bytes on 16
+ * bytes; calls that overlap on the GPU need one each. */
+typedef struct {
+    int n_seq, n_heads;
+    int prefix_len, max_len;
+    float scale;
+    const float *q;          /* [n_seq], rows of n_heads * head_dim, q_stride floats apart */
+    long long q_stride;
+    const kllm_kv_cache *prefix, *own;   /* host */
+    const int *own_len;      /* [n_seq] */
+    float *out;              /* as q */
+    long long out_stride;
+    void *workspace;
+    size_t workspace_bytes;
+} kllm_batch_attn;
+
+/* Bytes of workspace the call needs (workspace and its size unread), or 0
+ * for a call that kllm_batch_attention would refuse. */
+size_t kllm_batch_attention_workspace(const kllm_batch_attn *a);
+int kllm_batch_attention(const kllm_batch_attn *a, void *stream);
+
+/* One token per row of logits, drawn with a given uniform number:
+ *   w_i  = exp((x_i - max x) / temperature), NaN logits as -infinity
+ *   kept = the first top_k of the order (x descending, index ascending);
+ *          of those, each whose mass of w before it is < top_p times theirs;
+ *          of those, each with w_i >= min_p (the first of the order always)
+ *   token = the first index whose running sum of kept w, in index order,
+ *           exceeds u times their whole sum
+ * top_k <= 0, top_p >= 1 and min_p <= 0 turn a rule off; temperature <= 0
+ * picks the first maximum, by the rule of the greedy decode (a NaN at index
+ * 0 picks 0).  Where no logit is above -infinity the token is 0; where some
+ * are +infinity those share the mass alone.  u is taken into [0, 1); NaN
+ * settings are refused nowhere and turn their rule off (u: 0).
+ * Weights are 2^-40 fixed point, their sums exact integers: a row's token
+ * does not depend on the launch or on the other rows.  vocab is at most
+ * 2^22.  Settings are one per row; a NULL array turns the rule off
+ * (temperature: 1, u: required). */
+typedef struct {
+    int rows, vocab;
+    const float *logits;     /* rows of vocab floats, row_stride apart */
+    long long row_stride;
+    const float *temperature;
+    const int *top_k;
+    const float *top_p, *min_p;
+    const float *u;
+    int *tokens;             /* [rows] */
+} kllm_sample_rows;
+
+int kllm_sample(const kllm_sample_rows *rows, void *stream);
+
 /* ------------------------------------------------------------- chips -----
  * Chip directory loader: the same files, read the same way, as the
  * reference CLI's static chip_load (csrc/kllm.c:152-388): processor.json,

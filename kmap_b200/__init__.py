@@ -66,6 +66,12 @@ _SIGS = {
                                     C.c_int, _fp(C.c_int), _fp(C.c_int)]),
     "kllm_chip_decode": (C.c_int, [C.c_void_p, _fp(C.c_int32), C.c_int, C.c_int, C.c_int,
                                     C.c_char_p]),
+    "kllm_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kllm_kv_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                               C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p]),
+    "kllm_batch_attention_workspace": (C.c_size_t, [C.c_void_p]),
+    "kllm_batch_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "kllm_sample": (C.c_int, [C.c_void_p, C.c_void_p]),
     "kllm_plan_match": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                   C.c_int, _fp(C.c_int), _fp(C.c_int), C.c_int, C.c_int,
                                   C.c_int, C.c_char_p, C.c_int]),
@@ -160,6 +166,43 @@ class InferStats(C.Structure):
 
 
 MODE_AUTO, MODE_GENERIC, MODE_FUSED = 0, 1, 2
+
+# ------------------------------------------- batch serving operators ------
+# Structures of kllm_kv_append / kllm_kv_read, kllm_batch_attention and
+# kllm_sample: device addresses (a torch tensor's data_ptr()), fields in the
+# header's order and with its meaning.
+
+KV_F32, KV_I8, KV_E4M3 = 0, 1, 2
+
+
+class KvCache(C.Structure):
+    _fields_ = [("format", C.c_int), ("n_seq", C.c_int), ("n_kv", C.c_int),
+                ("head_dim", C.c_int), ("max_pos", C.c_int), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("seq_stride", C.c_longlong), ("scale_stride", C.c_longlong)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("rows", C.c_int), ("n_heads", C.c_int), ("pos0", C.c_int),
+                ("rope_rows", C.c_int), ("rope_offset", C.c_int), ("seq", C.c_void_p),
+                ("pos", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("row_stride", C.c_longlong), ("head_stride", C.c_longlong),
+                ("q_out", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p)]
+
+
+class BatchAttn(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_heads", C.c_int), ("prefix_len", C.c_int),
+                ("max_len", C.c_int), ("scale", C.c_float), ("q", C.c_void_p),
+                ("q_stride", C.c_longlong), ("prefix", C.c_void_p), ("own", C.c_void_p),
+                ("own_len", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_longlong),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class SampleRows(C.Structure):
+    _fields_ = [("rows", C.c_int), ("vocab", C.c_int), ("logits", C.c_void_p),
+                ("row_stride", C.c_longlong), ("temperature", C.c_void_p),
+                ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("u", C.c_void_p), ("tokens", C.c_void_p)]
 
 
 def exchange_blocks(block: bytes, group=None) -> list:
