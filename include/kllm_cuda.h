@@ -93,7 +93,9 @@ typedef struct {
     int stream_values;       /* persistent step: what the weight streams hold,
                                 0 = codebook table slots, 1 = bf16 values,
                                 2 = fp16 values (exact codebooks only) */
-    int reserved[6];
+    int shared_prefix;       /* kllm_infer_batch_ex: prompt positions that were
+                                computed and held once for all sequences */
+    int reserved[5];
 } kllm_infer_stats;
 
 void kllm_default_infer_opts(kllm_infer_opts *o);
@@ -237,8 +239,8 @@ typedef struct {
     long long seq_stride, scale_stride;
 } kllm_kv_cache;
 
-/* New rows for a cache.  Row r goes to position pos[r] of sequence seq[r]
- * (seq NULL: of sequence r); with pos NULL the rows are consecutive
+/* New rows for a cache.  Row r goes to position pos0 + pos[r] of sequence
+ * seq[r] (seq NULL: of sequence r); with pos NULL the rows are consecutive
  * positions pos0 + r of sequence 0 (a prompt).  A row whose position or
  * sequence lies outside the cache (a negative one among them: padding) is
  * skipped whole.  Two rows must not name the same place.
@@ -378,6 +380,33 @@ int kllm_infer_batch(TapeCtx *ctx, const int *prompts, const int *prompt_lens, i
 /* The same on a loaded chip (prepares its fused plan first). */
 int kllm_chip_infer_batch(kllm_chip *chip, const int *prompts, const int *prompt_lens, int nseq,
                           int max_new, int eos, int *out, int *out_lens);
+
+/* Options of kllm_infer_batch_ex (zeros: what kllm_infer_batch does).  All
+ * pointers are host memory. */
+typedef struct {
+    int kv_format;           /* KLLM_KV_* of the sequences' caches and the prefix */
+    int share_prefix;        /* 1: the prompts' longest common prefix is computed
+                                and held once (every prompt keeps its last
+                                token) */
+    const float *temperature;   /* [nseq] each, as kllm_sample; NULL: off */
+    const int *top_k;
+    const float *top_p, *min_p;
+    const float *u;          /* [nseq][max_new] uniform numbers in [0, 1), one
+                                per generated token; NULL: greedy */
+    int reserved[8];
+} kllm_batch_opts;
+
+/* kllm_infer_batch with a prefix that the sequences share, caches in 8 bits
+ * and drawn tokens (kllm_kv_append, kllm_batch_attention and kllm_sample in
+ * the captured step).  With 8-bit caches every decoded position attends to
+ * the stored values; a prompt's own positions see fp32 values among
+ * themselves and the stored ones of the prefix.  The prompt passes use the
+ * context's single-sequence cache.  Head dims 32, 64 and 128. */
+int kllm_infer_batch_ex(TapeCtx *ctx, const int *prompts, const int *prompt_lens, int nseq,
+                        int max_new, int eos, const kllm_batch_opts *opts, int *out, int *out_lens);
+int kllm_chip_infer_batch_ex(kllm_chip *chip, const int *prompts, const int *prompt_lens, int nseq,
+                             int max_new, int eos, const kllm_batch_opts *opts, int *out,
+                             int *out_lens);
 
 /* kllm_plan_prepare with the chip's tables, for its max_seq_len. */
 int kllm_chip_plan_prepare(kllm_chip *chip);

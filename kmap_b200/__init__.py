@@ -64,6 +64,11 @@ _SIGS = {
                                          C.c_int, _fp(C.c_int), _fp(C.c_int)]),
     "kllm_infer_batch": (C.c_int, [C.c_void_p, _fp(C.c_int), _fp(C.c_int), C.c_int, C.c_int,
                                     C.c_int, _fp(C.c_int), _fp(C.c_int)]),
+    "kllm_infer_batch_ex": (C.c_int, [C.c_void_p, _fp(C.c_int), _fp(C.c_int), C.c_int, C.c_int,
+                                       C.c_int, C.c_void_p, _fp(C.c_int), _fp(C.c_int)]),
+    "kllm_chip_infer_batch_ex": (C.c_int, [C.c_void_p, _fp(C.c_int), _fp(C.c_int), C.c_int,
+                                            C.c_int, C.c_int, C.c_void_p, _fp(C.c_int),
+                                            _fp(C.c_int)]),
     "kllm_chip_decode": (C.c_int, [C.c_void_p, _fp(C.c_int32), C.c_int, C.c_int, C.c_int,
                                     C.c_char_p]),
     "kllm_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -162,7 +167,8 @@ class InferStats(C.Structure):
     _fields_ = [("fused", C.c_int), ("steps", C.c_int), ("prefill_ms", C.c_double),
                 ("decode_ms", C.c_double), ("total_ms", C.c_double),
                 ("launches", C.c_longlong), ("step_kernel", C.c_int),
-                ("stream_values", C.c_int), ("reserved", C.c_int * 6)]
+                ("stream_values", C.c_int), ("shared_prefix", C.c_int),
+                ("reserved", C.c_int * 5)]
 
 
 MODE_AUTO, MODE_GENERIC, MODE_FUSED = 0, 1, 2
@@ -196,6 +202,12 @@ class BatchAttn(C.Structure):
                 ("q_stride", C.c_longlong), ("prefix", C.c_void_p), ("own", C.c_void_p),
                 ("own_len", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_longlong),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class BatchOpts(C.Structure):
+    _fields_ = [("kv_format", C.c_int), ("share_prefix", C.c_int), ("temperature", C.c_void_p),
+                ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("u", C.c_void_p), ("reserved", C.c_int * 8)]
 
 
 class SampleRows(C.Structure):
@@ -366,19 +378,39 @@ class Chip:
         toks = out[:n.value].copy()
         return (toks, lg) if logits else toks
 
-    def infer_batch(self, prompts, max_new: int, eos: int = -1, use_graphs: bool = True):
-        """Greedy generation for several sequences at once
-        (kllm_chip_infer_batch): returns one token array per sequence, each
-        cut before its first `eos`."""
+    def infer_batch(self, prompts, max_new: int, eos: int = -1, use_graphs: bool = True,
+                    kv_format: int = KV_F32, share_prefix: bool = False, u=None, temperature=None,
+                    top_k=None, top_p=None, min_p=None):
+        """Generation for several sequences at once (kllm_chip_infer_batch_ex):
+        returns one token array per sequence, each cut before its first `eos`.
+        Greedy, or drawn from `u` ([sequences][max_new] uniform numbers) under
+        temperature, top_k, top_p and min_p (one for all sequences, or one per
+        sequence); `share_prefix` computes and holds the prompts' common prefix
+        once, `kv_format` is the caches' (KV_F32, KV_I8, KV_E4M3)."""
+        n_seq = len(prompts)
         lens = np.array([len(p) for p in prompts], np.int32)
         flat = np.ascontiguousarray(np.concatenate([np.asarray(p, np.int32) for p in prompts]),
                                     np.int32)
-        out = np.zeros((len(prompts), max_new), np.int32)
-        n = np.zeros(len(prompts), np.int32)
+        out = np.zeros((n_seq, max_new), np.int32)
+        n = np.zeros(n_seq, np.int32)
+        keep = {}
+        for name, x, kind in (("u", u, np.float32), ("temperature", temperature, np.float32),
+                              ("top_k", top_k, np.int32), ("top_p", top_p, np.float32),
+                              ("min_p", min_p, np.float32)):
+            if x is not None:
+                shape = (n_seq, max_new) if name == "u" else (n_seq,)
+                x = np.asarray(x, kind)
+                if name == "u" and x.shape != shape:
+                    raise KllmError("infer_batch: u of shape %s for %s" % (x.shape, shape))
+                keep[name] = np.ascontiguousarray(np.broadcast_to(x, shape))
+        o = BatchOpts(kv_format, 1 if share_prefix else 0,
+                      *(keep[f].ctypes.data if f in keep else None
+                        for f in ("temperature", "top_k", "top_p", "min_p", "u")))
         self.set_opts(use_graphs=use_graphs)
-        check(lib().kllm_chip_infer_batch(self.h, _iptr(flat), _iptr(lens), len(prompts), max_new,
-                                          eos, _iptr(out), _iptr(n)), "kllm_chip_infer_batch")
-        return [out[i, :n[i]].copy() for i in range(len(prompts))]
+        check(lib().kllm_chip_infer_batch_ex(self.h, _iptr(flat), _iptr(lens), n_seq, max_new, eos,
+                                             C.byref(o), _iptr(out), _iptr(n)),
+              "kllm_chip_infer_batch_ex")
+        return [out[i, :n[i]].copy() for i in range(n_seq)]
 
     def infer_bytes(self, text: bytes, max_new: int, max_seq: int = 0, stop_after: int = -1):
         """Bytes in, streamed bytes out (processor_infer_bytes)."""

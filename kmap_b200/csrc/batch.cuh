@@ -362,4 +362,19 @@ __global__ void k_bd_argmax_pick(const float *__restrict__ part, int nz, int V, 
     pos[r] = pos[r] + 1;
 }
 
+// After a drawn token of each row (kllm_sample's kernel): kept as generated
+// token pos[r] - start[r], the next step's number put in place, the row's
+// position advances.
+__global__ void k_bd_drawn(int nseq, const int *__restrict__ start, int max_new,
+                           const int *__restrict__ tok, const float *__restrict__ u,
+                           float *__restrict__ unow, int *__restrict__ pos,
+                           int *__restrict__ gen) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= nseq) return;
+    const int step = pos[r] - start[r];
+    if (step >= 0 && step < max_new) gen[(size_t)r * max_new + step] = tok[r];
+    if (step + 1 < max_new) unow[r] = u[(size_t)r * max_new + step + 1];
+    pos[r] = pos[r] + 1;
+}
+
 }  // namespace kllm

@@ -236,8 +236,8 @@ k_ba_part(const BaArgs a) {
                     ba_mma_tf32(c, qa[2 * u + 1], h[2], h[3]);
                     ba_mma_tf32(cl, qa[2 * u + 1], l[2], l[3]);
                 }
-                s[t][0] = (c[0] + (c[2] + cl[0])) * rowfac;
-                s[t][1] = (c[1] + (c[3] + cl[1])) * rowfac;
+                s[t][0] = (c[0] + ((c[2] + cl[0]) + cl[2])) * rowfac;
+                s[t][1] = (c[1] + ((c[3] + cl[1]) + cl[3])) * rowfac;
             } else {
                 uint32_t kw[HD / 16];
                 ba_ld<HD / 4>(kw, kb + (long long)jk * HD + i * (HD / 4), in);

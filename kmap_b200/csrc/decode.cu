@@ -227,10 +227,19 @@ struct ByteSink : TokenSink {
 };
 }  // namespace
 
-extern "C" int kllm_infer_batch(TapeCtx *ctx, const int *prompts, const int *prompt_lens,
-                                int nseq, int max_new, int eos, int *out, int *out_lens) {
+static int infer_batch(const char *who, TapeCtx *ctx, const int *prompts, const int *prompt_lens,
+                       int nseq, int max_new, int eos, const kllm_batch_opts *bo, int *out,
+                       int *out_lens) {
     if (!ctx || !prompts || !prompt_lens || !out || !out_lens || nseq < 1 || max_new < 1) {
-        set_error("kllm_infer_batch: bad argument");
+        set_error("%s: bad argument", who);
+        return -1;
+    }
+    if (bo && (bo->kv_format < KLLM_KV_F32 || bo->kv_format > KLLM_KV_E4M3)) {
+        set_error("%s: unknown cache format %d", who, bo->kv_format);
+        return -1;
+    }
+    if (bo && !bo->u && (bo->temperature || bo->top_k || bo->top_p || bo->min_p)) {
+        set_error("%s: settings of the draw without its uniform numbers", who);
         return -1;
     }
     CtxImpl *c = impl(ctx);
@@ -239,16 +248,31 @@ extern "C" int kllm_infer_batch(TapeCtx *ctx, const int *prompts, const int *pro
     memset(&c->stats, 0, sizeof c->stats);
     const long long l0 = g_launches;
     double pre = 0, dec = 0;
-    const bool ok = plan_infer_batch(c, prompts, prompt_lens, nseq, max_new, eos, out, out_lens,
-                                     &pre, &dec);
+    int shared = 0;
+    const bool ok = plan_infer_batch(c, prompts, prompt_lens, nseq, max_new, eos, bo, out, out_lens,
+                                     &pre, &dec, &shared);
     c->stats.fused = 1;
     c->stats.steps = max_new;
     c->stats.prefill_ms = pre;
     c->stats.decode_ms = dec;
     c->stats.launches = g_launches - l0;
+    c->stats.shared_prefix = shared;
     c->stats.total_ms =
         std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
     return ok ? 0 : -1;
+}
+
+extern "C" int kllm_infer_batch(TapeCtx *ctx, const int *prompts, const int *prompt_lens,
+                                int nseq, int max_new, int eos, int *out, int *out_lens) {
+    return infer_batch("kllm_infer_batch", ctx, prompts, prompt_lens, nseq, max_new, eos, nullptr,
+                       out, out_lens);
+}
+
+extern "C" int kllm_infer_batch_ex(TapeCtx *ctx, const int *prompts, const int *prompt_lens,
+                                   int nseq, int max_new, int eos, const kllm_batch_opts *opts,
+                                   int *out, int *out_lens) {
+    return infer_batch("kllm_infer_batch_ex", ctx, prompts, prompt_lens, nseq, max_new, eos, opts,
+                       out, out_lens);
 }
 
 extern "C" int kllm_plan_prepare(TapeCtx *ctx, const float *embed_table, int vocab_size,

@@ -46,7 +46,7 @@ __device__ __forceinline__ float4 kv_source(const float *p, bool vec, int nz, lo
 __device__ __forceinline__ bool kv_place(const kllm_kv_cache &c, const int *seq, const int *pos,
                                          int pos0, int r, int *s, long long *p) {
     *s = seq ? seq[r] : pos ? r : 0;
-    *p = pos ? (long long)pos[r] : (long long)pos0 + r;
+    *p = (long long)pos0 + (pos ? pos[r] : r);
     return *s >= 0 && *s < c.n_seq && *p >= 0 && *p < c.max_pos;
 }
 

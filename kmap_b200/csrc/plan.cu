@@ -42,6 +42,7 @@
 #include "persist.cuh"
 #include "batch.cuh"
 #include "prefill.cuh"
+#include "serve.cuh"
 
 namespace kllm {
 
@@ -1318,24 +1319,25 @@ static bool plan_layer_wt(CtxImpl *c, DecodePlan *p, cudaStream_t s) {
     return true;
 }
 
-// Batched prompt pass (KLLM infer option `prefill`): positions 0..R-1 of
-// the prompt through every layer at once -- projections as TT-GEMMs (rows
+// Batched prompt pass (KLLM infer option `prefill`): positions off..off + R - 1
+// of the prompt (off = 0 but where a batch's shared prefix, positions
+// 0..off - 1, is in the cache already) through every layer at once -- projections as TT-GEMMs (rows
 // bit-identical to the TT-GEMV), norms, RoPE, causal attention, residuals
 // and SwiGLU as row kernels -- leaving the KV cache of those positions as
 // the per-token steps would.  The last layer needs only its k and v.  The
 // prompt's last position then runs as a regular decode step, which picks
 // the first token.  Its activations live in one arena of the plan, grown
 // (once) to the longest prompt seen and freed with the plan.
-static bool plan_prefill(CtxImpl *c, DecodePlan *p, int R, const int *prompt_dev, float *kc_base,
-                         float *vc_base, cudaStream_t s) {
+static bool plan_prefill(CtxImpl *c, DecodePlan *p, int R, int off, const int *prompt_dev,
+                         float *kc_base, float *vc_base, cudaStream_t s) {
     const TemplateInfo &t = p->ti;
     const TapeCtx *ctx = &c->base;
     const int H = t.H, hd = t.hd, nh = t.nh, nkv = t.nkv, F = t.F, L = t.L;
     const int qd = nh * hd, kvd = nkv * hd, nq = qd + 2 * kvd, mp = p->max_pos;
     if (R <= 0) return true;
     if (!((hd == 64 || hd == 128) && env_on("KLLM_PREFILL_FLASH", true)) &&
-        (size_t)(R + 1) * 4 > 200 * 1024) {
-        set_error("prefill: %d positions exceed the attention kernel's score buffer", R);
+        (size_t)(off + R + 1) * 4 > 200 * 1024) {
+        set_error("prefill: %d positions exceed the attention kernel's score buffer", off + R);
         return false;
     }
     // Tensor-core projections (pfgemm.cu) when every codebook is bf16 (the
@@ -1390,7 +1392,7 @@ static bool plan_prefill(CtxImpl *c, DecodePlan *p, int R, const int *prompt_dev
     // the row kernel, one block per position and head)
     const bool flash = (hd == 64 || hd == 128) && env_on("KLLM_PREFILL_FLASH", true);
     const size_t att_smem = flash ? (hd == 64 ? pf_flash_smem<64>() : pf_flash_smem<128>())
-                                  : (size_t)(R + 1) * 4;
+                                  : (size_t)(off + R + 1) * 4;
     if (ok && att_smem > 48 * 1024) {
         const void *fn = !flash ? (const void *)k_pf_attention
                          : hd == 64 ? (const void *)k_pf_flash<64> : (const void *)k_pf_flash<128>;
@@ -1408,18 +1410,19 @@ static bool plan_prefill(CtxImpl *c, DecodePlan *p, int R, const int *prompt_dev
         k_pf_rmsnorm<<<R, PF_THREADS, 0, s>>>(hA, p->dev_norm[2 * l], p->eps[2 * l], H, xn);
         ok = gemm(ls.qkv, xn, big);
         if (!ok) break;
-        k_pf_rope_kv<<<R, PF_THREADS, 0, s>>>(big, nq, nh, nkv, hd, p->rcos, p->rsin, mp, qr, kc, vc);
+        k_pf_rope_kv<<<R, PF_THREADS, 0, s>>>(big, nq, nh, nkv, hd, p->rcos, p->rsin, mp, off, qr,
+                                           kc, vc);
         g_launches += 2;
         if (l + 1 == L) break;   // later positions need only this layer's k and v
         if (!flash)
             k_pf_attention<<<dim3(R, nh), PF_THREADS, att_smem, s>>>(
-                qr, kc, vc, nh, t.groups, hd, mp, p->scale, cx);
+                qr, kc, vc, nh, t.groups, hd, mp, off, p->scale, cx);
         else if (hd == 64)
             k_pf_flash<64><<<dim3((R + PFA_BQ - 1) / PFA_BQ, nh), 256, att_smem, s>>>(
-                qr, kc, vc, R, nh, t.groups, mp, p->scale, cx);
+                qr, kc, vc, R, nh, t.groups, mp, off, p->scale, cx);
         else
             k_pf_flash<128><<<dim3((R + PFA_BQ - 1) / PFA_BQ, nh), 256, att_smem, s>>>(
-                qr, kc, vc, R, nh, t.groups, mp, p->scale, cx);
+                qr, kc, vc, R, nh, t.groups, mp, off, p->scale, cx);
         ok = gemm(ls.o, cx, big);
         if (!ok) break;
         k_pf_add<<<ew_blocks, 256, 0, s>>>(hA, big, (long long)R * H, hB);
@@ -1451,8 +1454,16 @@ static bool plan_prefill(CtxImpl *c, DecodePlan *p, int R, const int *prompt_dev
 // captured as a CUDA graph and replayed.  Sequences run the full max_new
 // steps; out_lens cut each at its first EOS (the reference stops there and
 // emits nothing after it).
+//
+// With options (bo): the prompts' longest common prefix is computed once and
+// kept in one cache that every sequence attends to, the sequences' own
+// caches then hold the positions behind it; caches in 8 bits; tokens drawn
+// from given numbers.  The prompt passes run in the plan's single-sequence
+// fp32 cache (prefix first, then each sequence's rest over it) and their rows
+// are stored from there.
 bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq, int max_new,
-                      int eos, int *out, int *out_lens, double *prefill_ms, double *decode_ms) {
+                      int eos, const kllm_batch_opts *bo, int *out, int *out_lens,
+                      double *prefill_ms, double *decode_ms, int *shared) {
     DecodePlan *p = c->plan;
     if (!p || !p->persist) {
         set_error("batched decode: no fused decode plan");
@@ -1485,6 +1496,27 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
             }
         total += lens[i];
     }
+    const int fmt = bo ? bo->kv_format : KLLM_KV_F32;
+    int P = 0;   // positions of the shared prefix: each sequence keeps one prompt token at least
+    if (bo && bo->share_prefix) {
+        P = *std::min_element(lens, lens + nseq) - 1;
+        size_t off = 0;
+        for (int i = 0; i < nseq; i++) {
+            int n = 0;
+            while (n < P && prompts[n] == prompts[off + n]) n++;
+            P = n;
+            off += lens[i];
+        }
+    }
+    if (shared) *shared = P;
+    // the caches of the batch serving operators where they are asked for;
+    // the fp32 caches and attention of the plain greedy batch otherwise
+    const bool serve = fmt != KLLM_KV_F32 || P > 0, drawn = bo && bo->u;
+    const int cap = serve ? *std::max_element(lens, lens + nseq) - P + max_new : mp;
+    if (serve && hd != 32 && hd != 64 && hd != 128) {
+        set_error("batched decode: head dim %d for a shared prefix or 8-bit caches (32, 64, 128)", hd);
+        return false;
+    }
     cudaStream_t s = c->stream;
     // tensor-core projections by default when the codebooks are bf16 numbers
     // (KLLM_BATCH_TC=0: the exact FP32 TT-GEMM, each row bit-identical to
@@ -1506,7 +1538,7 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
         }
     }
     const size_t att_smem = bd_att_smem(t.groups, hd, mp);
-    if (att_smem > 227 * 1024) {
+    if (!serve && att_smem > 227 * 1024) {
         set_error("batched decode: %d positions of %d query heads exceed the attention block's "
                   "shared memory", mp, t.groups);
         return false;
@@ -1518,14 +1550,49 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     // maxima; ints: prompts, tokens, positions, first positions, generated
     // tokens, the slice maxima's indices
     auto up4 = [](size_t n) { return (n + 3) & ~(size_t)3; };
-    const size_t seq_stride = (size_t)L * nkv * mp * hd;
-    const size_t kv = up4((size_t)nseq * seq_stride);
+    const size_t seq_stride = (size_t)L * nkv * cap * hd, scale_stride = (size_t)L * nkv * cap;
+    const size_t es = fmt == KLLM_KV_F32 ? 4 : 1;   // bytes of a cached value
+    const size_t kv = up4(((size_t)nseq * seq_stride * es + 3) / 4);
+    // the serving caches beside the codes: scales, and the prefix
+    const size_t rsc = es == 4 ? 0 : up4((size_t)nseq * scale_stride);
+    const size_t pkv = up4(((size_t)L * nkv * P * hd * es + 3) / 4);
+    const size_t psc = es == 4 ? 0 : up4((size_t)L * nkv * P);
+    // layer l of the sequences' caches, and of the prefix
+    kllm_kv_cache own = {fmt, nseq, nkv, hd, cap, nullptr, nullptr, nullptr, nullptr,
+                         (long long)seq_stride, (long long)scale_stride};
+    kllm_kv_cache pfx = own;
+    pfx.n_seq = 1;
+    pfx.max_pos = std::max(P, 1);
+    kllm_batch_attn at = {};
+    at.n_seq = nseq;
+    at.n_heads = nh;
+    at.prefix_len = P;
+    at.max_len = cap;
+    at.scale = p->scale;
+    at.q_stride = qd;
+    size_t att_ws = 0;
+    if (serve) {
+        // any addresses on 16 bytes: only the sizes count here
+        kllm_kv_cache o = own, q = pfx;
+        o.k = o.v = q.k = q.v = p->kc;
+        o.k_scale = o.v_scale = q.k_scale = q.v_scale = p->kc;
+        kllm_batch_attn t = at;
+        t.q = p->kc;
+        t.own = &o;
+        t.prefix = P ? &q : nullptr;
+        t.own_len = p->prompt;
+        att_ws = kllm_batch_attention_workspace(&t);
+        if (!att_ws) return false;
+    }
+    const size_t rws = up4((att_ws + 3) / 4), ru = drawn ? up4((size_t)nseq * (max_new + 1)) : 0;
+    const size_t rset = drawn ? up4((size_t)4 * nseq) : 0;
     const size_t rh = up4((size_t)nseq * H), rq = up4((size_t)nseq * qd);
     const size_t wide = up4((size_t)nseq * std::max({(size_t)nq, (size_t)2 * F, (size_t)H, (size_t)V}));
     const size_t rxs = up4(((size_t)3 * nseq * std::max({(size_t)H, (size_t)F, (size_t)qd}) + 1) / 2);
     const size_t rpart = up4(part_n), rcand = up4((size_t)nseq * BD_AC);
     const size_t ints = up4(total + 3 * (size_t)nseq + (size_t)nseq * max_new) + rcand;
-    const size_t need = 2 * kv + 2 * rh + wide + rq + rxs + rpart + rcand + ints;
+    const size_t need = 2 * kv + 2 * rsc + 2 * pkv + 2 * psc + rws + ru + rset + 2 * rh + wide + rq +
+                        rxs + rpart + rcand + ints;
     if (p->bd_cap < need) {
         if (!KLLM_CUDA(cudaStreamSynchronize(s))) return false;
         if (p->bd_arena) cudaFree(p->bd_arena);
@@ -1536,7 +1603,10 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     }
     float *kcs = p->bd_arena, *vcs = kcs + kv, *h = vcs + kv, *hB = h + rh, *big = hB + rh,
           *qr = big + wide, *xs = qr + rq, *part = xs + rxs, *cand_v = part + rpart;
-    int *d_cand_i = reinterpret_cast<int *>(cand_v + rcand), *d_prompts = d_cand_i + rcand,
+    float *ksc = cand_v + rcand, *vsc = ksc + rsc, *kpre = vsc + rsc, *vpre = kpre + pkv,
+          *kpsc = vpre + pkv, *vpsc = kpsc + psc, *d_u = vpsc + psc, *d_unow = d_u + (size_t)nseq * max_new,
+          *d_set = d_u + ru, *d_ws = d_set + rset;
+    int *d_cand_i = reinterpret_cast<int *>(d_ws + rws), *d_prompts = d_cand_i + rcand,
         *d_tok = d_prompts + total, *d_pos = d_tok + nseq, *d_start = d_pos + nseq,
         *d_gen = d_start + nseq;
     std::vector<int> tok0(nseq), pos0(nseq);
@@ -1544,7 +1614,9 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
         size_t off = 0;
         for (int i = 0; i < nseq; i++) {
             tok0[i] = prompts[off + lens[i] - 1];
-            pos0[i] = lens[i] - 1;
+            // the position of the token to feed; with serving caches the
+            // sequence's own positions once it is appended
+            pos0[i] = serve ? lens[i] - P : lens[i] - 1;
             off += lens[i];
         }
     }
@@ -1554,6 +1626,60 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
         !KLLM_CUDA(cudaMemcpyAsync(d_start, pos0.data(), nseq * 4, cudaMemcpyHostToDevice, s)) ||
         !KLLM_CUDA(cudaMemsetAsync(p->status, 0, 4, s)))
         return false;
+    // settings of the draw: temperature, top-p, min-p, top-k, a row of each
+    // (a rule left out: its value for off), and the numbers of every step
+    std::vector<float> set((size_t)4 * nseq), u0(nseq);
+    if (drawn) {
+        for (int i = 0; i < nseq; i++) {
+            set[i] = bo->temperature ? bo->temperature[i] : 1.f;
+            set[nseq + i] = bo->top_p ? bo->top_p[i] : 1.f;
+            set[2 * nseq + i] = bo->min_p ? bo->min_p[i] : 0.f;
+            const int k = bo->top_k ? bo->top_k[i] : 0;
+            memcpy(&set[3 * (size_t)nseq + i], &k, 4);
+            u0[i] = bo->u[(size_t)i * max_new];
+        }
+        if (!KLLM_CUDA(cudaMemcpyAsync(d_set, set.data(), set.size() * 4, cudaMemcpyHostToDevice, s)) ||
+            !KLLM_CUDA(cudaMemcpyAsync(d_u, bo->u, (size_t)nseq * max_new * 4, cudaMemcpyHostToDevice, s)) ||
+            !KLLM_CUDA(cudaMemcpyAsync(d_unow, u0.data(), (size_t)nseq * 4, cudaMemcpyHostToDevice, s)))
+            return false;
+    }
+    auto own_layer = [&](int l) {
+        kllm_kv_cache x = own;
+        const size_t at = (size_t)l * nkv * cap;
+        x.k = reinterpret_cast<char *>(kcs) + at * hd * es;
+        x.v = reinterpret_cast<char *>(vcs) + at * hd * es;
+        x.k_scale = ksc + (rsc ? at : 0);
+        x.v_scale = vsc + (rsc ? at : 0);
+        return x;
+    };
+    auto pre_layer = [&](int l) {
+        kllm_kv_cache x = pfx;
+        const size_t at = (size_t)l * nkv * P;
+        x.k = reinterpret_cast<char *>(kpre) + at * hd * es;
+        x.v = reinterpret_cast<char *>(vpre) + at * hd * es;
+        x.k_scale = kpsc + (psc ? at : 0);
+        x.v_scale = vpsc + (psc ? at : 0);
+        return x;
+    };
+    // rows [from, from + n) of the plan's fp32 cache into positions 0.. of
+    // sequence `seq` of a layer's cache
+    auto store = [&](kllm_kv_cache x, int l, int seq, int from, int n) {
+        const size_t base = (size_t)l * nkv * mp * hd + (size_t)from * hd;
+        x.k = static_cast<char *>(x.k) + (size_t)seq * x.seq_stride * es;
+        x.v = static_cast<char *>(x.v) + (size_t)seq * x.seq_stride * es;
+        x.k_scale += (size_t)seq * (rsc ? x.scale_stride : 0);
+        x.v_scale += (size_t)seq * (rsc ? x.scale_stride : 0);
+        x.n_seq = 1;
+        KvAppend a;
+        a.c = x;
+        a.r = {};
+        a.r.rows = n;
+        a.r.k = p->kc + base;
+        a.r.v = p->vc + base;
+        a.r.row_stride = hd;
+        a.r.head_stride = (long long)mp * hd;
+        return n < 1 || kv_append(s, a);
+    };
     // the lm_head as bf16 Wt for the tensor-core form (built once)
     if (lm_tc && !p->bd_lm_wt) {
         if (!KLLM_CUDA(cudaMalloc(&p->bd_lm_wt, (size_t)lms.tt_K * lms.tt_N * 2)) ||
@@ -1562,13 +1688,27 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     }
     if (!KLLM_CUDA(cudaEventRecord(p->ev0, s))) return false;
     // prompt passes, one sequence after another, into the sequences' caches
+    if (serve && P > 0) {
+        if (!plan_prefill(c, p, P, 0, d_prompts, p->kc, p->vc, s)) return false;
+        for (int l = 0; l < L; l++) {
+            const kllm_kv_cache x = pre_layer(l);
+            const size_t base = (size_t)l * nkv * mp * hd;
+            if (!store(x, l, 0, 0, P)) return false;
+            // what comes after attends to the values that the cache holds
+            if (fmt != KLLM_KV_F32 && !kv_read(s, x, P, nullptr, nullptr, 0, p->kc + base,
+                                               p->vc + base, hd, (long long)mp * hd))
+                return false;
+        }
+    }
     {
         size_t off = 0;
         for (int i = 0; i < nseq; i++) {
-            if (lens[i] >= 2 && !plan_prefill(c, p, lens[i] - 1, d_prompts + off,
-                                              kcs + (size_t)i * seq_stride,
-                                              vcs + (size_t)i * seq_stride, s))
-                return false;
+            const int n = lens[i] - 1 - P;
+            float *kd = serve ? p->kc : kcs + (size_t)i * seq_stride;
+            float *vd = serve ? p->vc : vcs + (size_t)i * seq_stride;
+            if (n > 0 && !plan_prefill(c, p, n, P, d_prompts + off + P, kd, vd, s)) return false;
+            for (int l = 0; serve && l < L; l++)
+                if (!store(own_layer(l), l, i, P, n)) return false;
             off += lens[i];
         }
     }
@@ -1607,7 +1747,7 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     auto att = hd == 32 ? att_for(std::integral_constant<int, 32>(), t.groups)
              : hd == 64 ? att_for(std::integral_constant<int, 64>(), t.groups)
                         : att_for(std::integral_constant<int, 128>(), t.groups);
-    if (att_smem > 48 * 1024 &&
+    if (!serve && att_smem > 48 * 1024 &&
         !KLLM_CUDA(cudaFuncSetAttribute(att, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)att_smem)))
         return false;
@@ -1626,10 +1766,30 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
             const LayerSlots &ls = t.layers[l];
             float *kc = kcs + (size_t)l * nkv * mp * hd, *vc = vcs + (size_t)l * nkv * mp * hd;
             if (!gemm(ls.qkv, l, 0, &y, &nz)) return false;
-            k_bd_rope_kv<<<dim3(nseq, 8), PF_THREADS, 0, s>>>(y, nz, d_pos, nq, nh, nkv, hd, p->rcos,
-                                                     p->rsin, mp, seq_stride, qr, kc, vc);
-            att<<<dim3(nseq, nkv), BD_ATT_THREADS, att_smem, s>>>(
-                qr, kc, vc, d_pos, nh, t.groups, mp, seq_stride, p->scale, lt, xs);
+            if (serve) {
+                // d_pos counts the own positions, this token's among them
+                KvAppend a;
+                a.c = own_layer(l);
+                a.r = {nseq, nh, -1, mp, P, nullptr, d_pos, y, y + qd, y + qd + kvd, nq, hd, qr,
+                       p->rcos, p->rsin};
+                a.nz = nz;
+                a.plane = (long long)nseq * nq;
+                const kllm_kv_cache x = pre_layer(l);
+                at.q = qr;
+                at.own = &a.c;
+                at.prefix = P ? &x : nullptr;
+                at.own_len = d_pos;
+                at.workspace = d_ws;
+                at.workspace_bytes = rws * 4;
+                if (!kv_append(s, a) || !batch_attention(s, at, lt, xs)) return false;
+            } else {
+                k_bd_rope_kv<<<dim3(nseq, 8), PF_THREADS, 0, s>>>(y, nz, d_pos, nq, nh, nkv, hd,
+                                                                  p->rcos, p->rsin, mp, seq_stride,
+                                                                  qr, kc, vc);
+                att<<<dim3(nseq, nkv), BD_ATT_THREADS, att_smem, s>>>(
+                    qr, kc, vc, d_pos, nh, t.groups, mp, seq_stride, p->scale, lt, xs);
+                g_launches += 2;
+            }
             if (!gemm(ls.o, l, 1, &y, &nz)) return false;
             k_bd_add_norm<<<nseq * BD_CL, PF_THREADS, 0, s>>>(h, nullptr, nullptr, y, nz,
                                                       p->dev_norm[2 * l + 1], p->eps[2 * l + 1],
@@ -1641,9 +1801,19 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
             k_bd_add_norm<<<nseq * BD_CL, PF_THREADS, 0, s>>>(
                 hB, nullptr, nullptr, y, nz, last ? p->dev_norm.back() : p->dev_norm[2 * l + 2],
                 last ? p->f_eps : p->eps[2 * l + 2], H, h, last ? lmt : lt, xs);
-            g_launches += 5;
+            g_launches += 3;
         }
         if (!gemm(t.lm, 0, 4, &y, &nz)) return false;
+        if (drawn) {
+            const kllm_sample_rows r = {nseq, V, y, V, d_set,
+                                        reinterpret_cast<const int *>(d_set + 3 * (size_t)nseq),
+                                        d_set + nseq, d_set + 2 * (size_t)nseq, d_unow, d_tok};
+            if (!sample_rows(s, r, nz, (long long)nseq * V)) return false;
+            k_bd_drawn<<<(nseq + 31) / 32, 32, 0, s>>>(nseq, d_start, max_new, d_tok, d_u, d_unow,
+                                                       d_pos, d_gen);
+            g_launches++;
+            return KLLM_CUDA(cudaGetLastError());
+        }
         k_bd_argmax_part<<<dim3(nseq, BD_AC), PF_THREADS, 0, s>>>(y, nz, V, cand_v, d_cand_i);
         k_bd_argmax_pick<<<(nseq + 31) / 32, 32, 0, s>>>(y, nz, V, nseq, cand_v, d_cand_i, d_start,
                                                         max_new, d_tok, d_pos, d_gen);
@@ -1765,7 +1935,7 @@ bool plan_infer(CtxImpl *c, const int *prompt, int prompt_len, int max_new, int 
     if (c->opts.prefill && p->persist && want_rows == 0 && prompt_len >= 2) {
         const int R = prompt_len - 1;
         StepState st1 = {R, prompt_len, 0, 0};
-        if (!plan_prefill(c, p, R, p->prompt, p->kc, p->vc, s) ||
+        if (!plan_prefill(c, p, R, 0, p->prompt, p->kc, p->vc, s) ||
             !KLLM_CUDA(cudaMemcpyAsync(p->st, &st1, sizeof st1, cudaMemcpyHostToDevice, s)))
             return false;
         launched = R;

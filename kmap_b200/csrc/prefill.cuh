@@ -60,49 +60,49 @@ __global__ void k_pf_rmsnorm(const float *__restrict__ x, const float *__restric
         out[(size_t)r * H + i] = __fmul_rn(__fmul_rn(xr[i], rsq), w[i]);
 }
 
-// Rotate-half RoPE of row r (position r) of the fused QKV output, q to
-// q_out[r][qd], rotated k and plain v into the layer's cache rows r:
+// Rotate-half RoPE of row r (position off + r) of the fused QKV output, q to
+// q_out[r][qd], rotated k and plain v into the layer's cache rows off + r:
 // v' = y * cos[dim] + rot * sin[dim], rot = -y[dim + hd/2] in the first
 // half of a head and +y[dim - hd/2] in the second.  (grid: R blocks)
 __global__ void k_pf_rope_kv(const float *__restrict__ qkv, int nq, int nh, int nkv, int hd,
                              const float *__restrict__ rcos, const float *__restrict__ rsin,
-                             int max_pos, float *__restrict__ q_out, float *__restrict__ kc,
-                             float *__restrict__ vc) {
-    const int r = blockIdx.x;
+                             int max_pos, int off, float *__restrict__ q_out,
+                             float *__restrict__ kc, float *__restrict__ vc) {
+    const int r = blockIdx.x, at = off + r;
     const int qd = nh * hd, kvd = nkv * hd;
     const float *y = qkv + (size_t)r * nq;
     for (int n = threadIdx.x; n < qd + 2 * kvd; n += blockDim.x) {
         if (n < qd + kvd) {
             const int head = n / hd, dim = n % hd, half = hd / 2;
             const float pk = dim < half ? -y[n + half] : y[n - half];
-            const float v = __fadd_rn(__fmul_rn(y[n], rcos[(size_t)r * hd + dim]),
-                                      __fmul_rn(pk, rsin[(size_t)r * hd + dim]));
+            const float v = __fadd_rn(__fmul_rn(y[n], rcos[(size_t)at * hd + dim]),
+                                      __fmul_rn(pk, rsin[(size_t)at * hd + dim]));
             if (head < nh)
                 q_out[(size_t)r * qd + n] = v;
             else
-                kc[((size_t)(head - nh) * max_pos + r) * hd + dim] = v;
+                kc[((size_t)(head - nh) * max_pos + at) * hd + dim] = v;
         } else {
             const int vi = n - qd - kvd;
-            vc[((size_t)(vi / hd) * max_pos + r) * hd + vi % hd] = y[n];
+            vc[((size_t)(vi / hd) * max_pos + at) * hd + vi % hd] = y[n];
         }
     }
 }
 
-// Causal attention of row r (position r), head h: scores over positions
-// 0..r of the head's kv group, softmax (exp in double), P.V.
-// (grid: R x nh blocks, dynamic shared memory: (R + 1) floats)
+// Causal attention of row r (position off + r), head h: scores over positions
+// 0..off + r of the head's kv group, softmax (exp in double), P.V.
+// (grid: R x nh blocks, dynamic shared memory: (off + R + 1) floats)
 __global__ void k_pf_attention(const float *__restrict__ q, const float *__restrict__ kc,
                                const float *__restrict__ vc, int nh, int groups, int hd,
-                               int max_pos, float scale, float *__restrict__ ctx) {
+                               int max_pos, int off, float scale, float *__restrict__ ctx) {
     extern __shared__ float sc[];
     __shared__ float red[PF_THREADS / 32];
-    const int r = blockIdx.x, h = blockIdx.y, g = h / groups;
+    const int r = blockIdx.x, h = blockIdx.y, g = h / groups, last = off + r;
     const int qd = nh * hd;
     const float *qr = q + (size_t)r * qd + h * hd;
     const float *kg = kc + (size_t)g * max_pos * hd;
     const float *vg = vc + (size_t)g * max_pos * hd;
     float m = -INFINITY;
-    for (int j = threadIdx.x; j <= r; j += PF_THREADS) {
+    for (int j = threadIdx.x; j <= last; j += PF_THREADS) {
         float dot = 0.f;
         for (int d = 0; d < hd; d++) dot = __fadd_rn(dot, __fmul_rn(qr[d], kg[(size_t)j * hd + d]));
         const float s = __fmul_rn(dot, scale);
@@ -111,23 +111,23 @@ __global__ void k_pf_attention(const float *__restrict__ q, const float *__restr
     }
     const float mx = pf_block_max(m, red);
     float sum = 0.f;
-    for (int j = threadIdx.x; j <= r; j += PF_THREADS) {
+    for (int j = threadIdx.x; j <= last; j += PF_THREADS) {
         const float e = (float)exp((double)__fsub_rn(sc[j], mx));
         sc[j] = e;
         sum = __fadd_rn(sum, e);
     }
     const float tot = pf_block_sum(sum, red);
-    for (int j = threadIdx.x; j <= r; j += PF_THREADS) sc[j] = __fdiv_rn(sc[j], tot);
+    for (int j = threadIdx.x; j <= last; j += PF_THREADS) sc[j] = __fdiv_rn(sc[j], tot);
     __syncthreads();
     for (int d = threadIdx.x; d < hd; d += PF_THREADS) {
         float acc = 0.f;
-        for (int j = 0; j <= r; j++) acc = __fadd_rn(acc, __fmul_rn(sc[j], vg[(size_t)j * hd + d]));
+        for (int j = 0; j <= last; j++) acc = __fadd_rn(acc, __fmul_rn(sc[j], vg[(size_t)j * hd + d]));
         ctx[(size_t)r * qd + h * hd + d] = acc;
     }
 }
 
-// Causal attention of R prompt positions, tiled (flash-style): block =
-// (64 queries, head h); key/value tiles of 64 positions of the head's kv
+// Causal attention of R prompt positions off..off + R - 1 over positions 0 up
+// to their own, tiled (flash-style): block = (64 queries, head h); key/value tiles of 64 positions of the head's kv
 // group go through shared memory, scores with fused multiply-adds, an
 // online softmax per query row (running max and sum, exp in float) and the
 // P.V tile product.  A tolerance result like the row kernel above (whose
@@ -144,7 +144,8 @@ __host__ __device__ constexpr size_t pf_flash_smem() {
 template <int HD>
 __global__ void __launch_bounds__(256)
 k_pf_flash(const float *__restrict__ q, const float *__restrict__ kc, const float *__restrict__ vc,
-           int R, int nh, int groups, int max_pos, float scale, float *__restrict__ ctx) {
+           int R, int nh, int groups, int max_pos, int off, float scale,
+           float *__restrict__ ctx) {
     constexpr int DQ = HD / 16;                 // output dims per thread (4 or 8)
     extern __shared__ float sm[];
     float *Qs = sm;                             // [BQ][HD + 1]
@@ -168,7 +169,7 @@ k_pf_flash(const float *__restrict__ q, const float *__restrict__ kc, const floa
 #pragma unroll
         for (int d = 0; d < DQ; d++) o[i][d] = 0.f;
     }
-    const int last_q = min(q0 + PFA_BQ, R) - 1;
+    const int last_q = off + min(q0 + PFA_BQ, R) - 1;
     for (int k0 = 0; k0 <= last_q; k0 += PFA_BK) {
         __syncthreads();   // the previous tile's Ks, Vs, Ps are free
         for (int i = tid; i < PFA_BK * HD; i += 256) {
@@ -198,7 +199,7 @@ k_pf_flash(const float *__restrict__ q, const float *__restrict__ kc, const floa
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int qi = q0 + ty * 4 + i;
+            const int qi = off + q0 + ty * 4 + i;
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; j++) {

@@ -86,9 +86,7 @@ struct SaRow {
 
     __device__ __forceinline__ float at(int i) const {
         if (cached || nz == 1) return src[i];
-        float a = g[i];
-        for (int z = 1; z < nz; z++) a = __fadd_rn(a, g[(long long)z * plane + i]);
-        return a;
+        return bd_sum(g, nz, plane, i);
     }
     // weight of a logit, 2^-40 fixed point
     __device__ __forceinline__ u64 weight(float x) const {
@@ -329,13 +327,8 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int cached)
     const bool greedy = T <= 0.f;
     if (greedy || row.m == -INFINITY) {
         if (c == 0 && tid == 0) {
-            const float x0 = a.logits[(long long)r * a.row_stride];
-            bool nan0 = x0 != x0;
-            for (int z = 1; z < nz; z++) {
-                const float v = a.logits[(long long)r * a.row_stride + z * plane];
-                nan0 = nan0 || v != v;
-            }
-            a.tokens[r] = nan0 || row.m == -INFINITY ? 0 : first_max;
+            const float x0 = bd_sum(a.logits + (long long)r * a.row_stride, nz, plane, 0);
+            a.tokens[r] = x0 != x0 || row.m == -INFINITY ? 0 : first_max;
         }
         cl.sync();
         return;

@@ -128,3 +128,17 @@ def test_bad_sample(built_lib, kw, word):
     d.update(kw)
     a = K.SampleRows(**d)
     _refused(built_lib.kllm_sample(C.byref(a), None), word)
+
+
+def test_infer_batch_ex_refuses(built_lib):
+    """Before the context is looked at: a format that is none, settings without numbers."""
+    import kmap_b200 as K
+    one = (C.c_int * 4)(1, 1, 1, 1)
+    ctx = built_lib.tape_ctx_create(1, 1)
+    for f in (built_lib.kllm_infer_batch_ex, built_lib.kllm_chip_infer_batch_ex):
+        _refused(f(None, one, one, 1, 1, -1, None, one, one), "bad argument")
+    o = K.BatchOpts(3)
+    _refused(built_lib.kllm_infer_batch_ex(ctx, one, one, 1, 1, -1, C.byref(o), one, one), "format")
+    o = K.BatchOpts(0, 0, C.addressof(one))
+    _refused(built_lib.kllm_infer_batch_ex(ctx, one, one, 1, 1, -1, C.byref(o), one, one), "uniform")
+    built_lib.tape_ctx_destroy(ctx)
