@@ -13,24 +13,25 @@
 //   2. a histogram of the row over 1024 ranges of the distance to the
 //      maximum (each 3 % of weight wide): a count and, in the low bits, where
 //      in the range its tokens lie, so that a range's mass is known to 0.2 %;
-//      for top-p alone the exact whole mass beside it;
 //   3. from it the range in which top-k, or top-p, ends;
 //   4a. few tokens up to there (512): they go to one block, whose threads
 //      take one each, and count the tokens and the mass before theirs, then
 //      the kept mass up to theirs in index order: top-k, top-p, min-p and the
 //      draw in two loops over the list;
 //   4b. many: the prefix's last logit tau, and how many of the tokens that
-//      equal it are kept, from histograms over the keys (order-preserving
-//      integers) of the ranges that the boundary can lie in, until one key is
-//      left; then the kept mass of every warp's part, and the draw by the
-//      warp that holds it.  Each lane keeps a mask of its tokens up to the
-//      boundary's range, so that these passes touch no others.
+//      equal it are kept.  One pass collects the tokens of the ranges that
+//      the boundary can lie in and sums the weights before them; histograms
+//      over the collected tokens' keys (order-preserving integers) close in
+//      on one key; then the kept mass of every warp's part, and the draw by
+//      the warp that holds it.  Passes take four tokens a lane at a time, for
+//      the weights' chains to overlap, and skip what no lane wants.
 // Histograms are summed over the cluster by every block for itself
 // (distributed shared memory): one cluster barrier a step.
 //
-// Bound: a row's 4 vocab bytes are read once; past that the weights take 15
-// double-precision operations a token where all are needed (top-p alone, plain
-// temperature), and few rows wait for the chain of dependent steps.
+// Bound: a row's 4 vocab bytes are read once; past that, instructions: some
+// 30 a weight, and a weight a token where all are needed (top-p alone, plain
+// temperature), another for the kept ones; few rows wait for the chain of
+// dependent steps.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -48,6 +49,7 @@ typedef unsigned long long u64;
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_CL = 8;
 constexpr int SA_BINS = 1024, SA_FINE = 512;       // ranges of step 2; keys of step 4b
 constexpr int SA_LIST = SA_THREADS;                // most tokens of step 4a
+constexpr int SA_NEAR = 2048;                      // most collected tokens of a block in step 4b
 constexpr float SA_OCTAVES = 41.5f;                // weights below 2^-41 of the largest are zero
 constexpr int SA_VOCAB = 1 << 22;                  // sums stay below 2^62
 constexpr size_t SA_CACHE = 180 * 1024;            // slice bytes that are kept on chip
@@ -62,17 +64,30 @@ __device__ __forceinline__ float sa_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// 2^-(j / 32) as fractions of 2^32
+__constant__ uint32_t sa_tab[32] = {
+    0xffffffffu, 0xfa83b2dbu, 0xf5257d15u, 0xefe4b99cu, 0xeac0c6e8u, 0xe5b906e7u, 0xe0ccdeecu,
+    0xdbfbb798u, 0xd744fccbu, 0xd2a81d92u, 0xce248c15u, 0xc9b9bd86u, 0xc5672a11u, 0xc12c4ccau,
+    0xbd08a39fu, 0xb8fbaf47u, 0xb504f334u, 0xb123f582u, 0xad583eeau, 0xa9a15ab5u, 0xa5fed6aau,
+    0xa2704303u, 0x9ef53261u, 0x9b8d39bau, 0x9837f052u, 0x94f4efa9u, 0x91c3d374u, 0x8ea4398bu,
+    0x8b95c1e4u, 0x88980e81u, 0x85aac368u, 0x82cd8699u};
+
 struct SaShared {
     alignas(16) uint32_t coarse[SA_BINS];          // counts, and below them positions
     alignas(16) u64 fine[2][SA_FINE + 2];          // + the exact mass before the ranges
-    alignas(16) ulonglong2 list[SA_LIST];          // (key, ~index) and weight
-    u64 best[SA_CL], mass[SA_CL], total[SA_CL];    // written by the blocks of the cluster
+    union {
+        alignas(16) ulonglong2 list[SA_LIST];      // 4a: (key, ~index) and weight
+        int near[SA_NEAR];                         // 4b: places of the collected tokens
+    };
+    uint32_t tab[32];                              // 2^-(j / 32), 32-bit fractions
+    float top[SA_CL];
+    u64 mass[SA_CL], total[SA_CL];                 // written by the blocks of the cluster
     int ties[SA_CL];
     u64 wsum[SA_WARPS], wabove[SA_WARPS];
-    double wlo[SA_WARPS], whi[SA_WARPS];
+    double wlo[SA_WARPS], whi[SA_WARPS], goal_lo, goal_hi;
     int wtie[SA_WARPS];
     u64 sel_before, sel_amount;
-    int sel_bin, sel_upto, lo_bin, hi_bin, icut, n_list;
+    int sel_bin, sel_upto, lo_bin, hi_bin, icut, n_list, n_near;
 };
 
 __device__ __forceinline__ u64 sa_warp_sum(u64 v) {
@@ -138,40 +153,31 @@ struct SaKept {
 struct SaScale {
     float m, binf;
     double md, lt;
+    const uint32_t *tab;    // sa_tab in shared memory
 
-    // Range of the distance to the maximum, as a number (no NaN unless x is
-    // -infinity under T = infinity).
+    // Range of the distance to the maximum, as a number.
     __device__ __forceinline__ float range(float x) const { return x == m ? 0.f : (m - x) * binf; }
 
-    // Weight of a logit, 2^-40 fixed point.  2^-t = 2^-n 2^f, n the integer next to t, with 2^f
-    // on [-1/2, 1/2] as the polynomial of degree 9 that meets it at the Chebyshev nodes (relative
-    // error 2^-45.6); both roundings to integers are additions of a power of two, since
-    // conversions from and to 64 bits run at a quarter of the additions' rate.  No branch: several
-    // tokens' chains overlap.
+    // Weight of a logit, 2^-40 fixed point: t = (m - x) log2(e) / T in double precision, its whole
+    // part n and a fraction of 32 bits by one addition (conversions from and to 64 bits are slow);
+    // 2^-fraction as a table's 2^-(j / 32), one word a bank, times 1 - z (c1 - z (c2 - z c3)), the
+    // polynomial that meets 2^-z at the Chebyshev nodes of [0, 1/32), all as 32-bit fractions
+    // (relative error below 2^-29); the sum of t and 1.5 * 2^20 has n in its upper word and the
+    // fraction in its lower.  No branch: several tokens' chains overlap.
     __device__ __forceinline__ u64 weight(float x) const {
-        // a normal float's bits as a double's; the others are converted
+        // the float's bits as a double's (what is below 2^-126 becomes some number below it,
+        // -infinity becomes -2^128)
         const uint32_t b = __float_as_uint(x);
-        double xd = __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
-                                     (int)(b << 29));
-        if ((b & 0x7f800000u) == 0) xd = (double)x;
-        const double t = (md - xd) * lt;
-        const double magic = 0x1.8p52;
-        const double y = t + magic;
-        const double f = (y - magic) - t;
-        double p = 1.0205905413765595794e-7;
-        p = fma(p, f, 1.325964524488711024e-6);
-        p = fma(p, f, 0.000015252672924850736404);
-        p = fma(p, f, 0.00015403433751251008921);
-        p = fma(p, f, 0.0013333558200794592645);
-        p = fma(p, f, 0.0096181291939343133551);
-        p = fma(p, f, 0.055504108664651672007);
-        p = fma(p, f, 0.2402265069564033974);
-        p = fma(p, f, 0.69314718055994615897);
-        p = fma(p, f, 1.0000000000000134868);
-        const int n = __double2loint(y);
-        const double r = __hiloint2double(__double2hiint(p) + ((40 - n) << 20), __double2loint(p)) + 0x1p52;
-        const u64 w = (u64)__double_as_longlong(r) & 0xfffffffffffffull;
-        return x == m ? 1ull << 40 : t < (double)SA_OCTAVES && x != -INFINITY ? w : 0ull;
+        const double xd = __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
+                                           (int)(b << 29));
+        const double y = fma(md - xd, lt, 0x1.8p20);
+        const uint32_t n = (uint32_t)__double2hiint(y) - 0x41380000u, lo = (uint32_t)__double2loint(y);
+        const uint32_t z = lo & 0x07ffffffu, t = tab[lo >> 27];
+        uint32_t q = 0x3d7f23e8u - __umulhi(z, 0x0e181d25u);
+        q = 0xb17217d1u - __umulhi(z, q);
+        const uint32_t f = t - __umulhi(t, __umulhi(z, q));
+        const u64 w = ((((u64)f << 9) >> (n & 63u)) + 1) >> 1;
+        return x == m ? 1ull << 40 : n <= 41u ? w : 0ull;
     }
 };
 
@@ -183,8 +189,7 @@ struct SaSlice {
     int nz;
     long long plane;
     int first;              // index of its first token
-    int i0, i1, steps;      // this warp's part, and its 32-token steps
-    int per_bit;            // steps a bit of a lane's mask stands for
+    int wper, i0, i1, steps;    // tokens per warp, this warp's part, and its 32-token steps
 
     // a logit of the slice, NaN as -infinity
     __device__ __forceinline__ float at(int i) const {
@@ -192,30 +197,99 @@ struct SaSlice {
         const float x = bd_sum(g, nz, plane, i);
         return x != x ? -INFINITY : x;
     }
-    // f(x, i) for this lane's tokens in the steps of the mask
-    template <class F>
-    __device__ __forceinline__ void each(uint32_t mask, F &&f) const {
+    // Steps four at a time: f(x, i, in) with four of this lane's tokens, their places in the slice
+    // and whether each is `wanted` (never -infinity), where any of the warp's is.
+    template <class P, class F>
+    __device__ __forceinline__ void each4(P &&wanted, F &&f) const {
         const int lane = threadIdx.x & 31;
-        while (mask) {
-            const int b = __ffs(mask) - 1;
-            mask &= mask - 1;
-            for (int j = b * per_bit; j < (b + 1) * per_bit; j++) {
-                const int i = i0 + 32 * j + lane;
-                if (i < i1) f(at(i), i);
+#pragma unroll 1
+        for (int j0 = 0; j0 < steps; j0 += 4) {
+            float x[4];
+            int i[4];
+            bool in[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                i[e] = i0 + 32 * (j0 + e) + lane;
+                x[e] = i[e] < i1 ? at(i[e]) : -INFINITY;
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) in[e] = wanted(x[e], i[e]);
+            if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) f(x, i, in);
         }
+    }
+    // the sum of this lane's wanted tokens' weights
+    template <class P>
+    __device__ __forceinline__ u64 mass(const SaScale &sc, P &&wanted) const {
+        u64 sum = 0;
+        each4(wanted, [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
+            u64 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = sc.weight(x[e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += in[e] ? w[e] : 0ull;
+        });
+        return sum;
     }
 };
 
-// Narrows the keys of ranges [lo_bin, hi_bin] until the boundary's key is
-// found, among the tokens that `in` keeps (limited): with MASS the last token
-// whose mass before is < goal, else the one with `count` - 1 before it.
-// `above` is the amount before the ranges (MASS: found by the first pass, and
-// left per warp in sh.wabove).
+// Places of the flagged ones of a warp's four tokens a lane in a block's list:
+// one addition to its length for all of them.  Called by the whole warp.
+__device__ __forceinline__ void sa_append(int *length, const bool (&in)[4], int (&at)[4]) {
+    const int lane = threadIdx.x & 31;
+    const unsigned below = (1u << lane) - 1u;
+    unsigned b[4];
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        b[e] = __ballot_sync(0xffffffffu, in[e]);
+        at[e] = n + __popc(b[e] & below);
+        n += __popc(b[e]);
+    }
+    int first = 0;
+    if (n) {
+        if (lane == 0) first = atomicAdd(length, n);
+        first = __shfl_sync(0xffffffffu, first, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) at[e] += first;
+}
+
+// What a pass over the collected tokens does: f(x, i) for each, or, where a
+// block had more of them than it can hold, for every token of its slice that
+// the ranges [flo, fhi) hold.
+template <bool CACHED, class F>
+__device__ __forceinline__ void sa_near(const SaShared &sh, const SaScale &sc, const SaSlice<CACHED> &sl,
+                                        float flo, float fhi, F &&f) {
+    const int n = sh.n_near;
+    if (n <= SA_NEAR) {
+        for (int q = threadIdx.x; q < n; q += SA_THREADS) {
+            const int i = sh.near[q];
+            f(sl.at(i), i);
+        }
+    } else {
+        sl.each4(
+            [&](float x, int) {
+                const float t = sc.range(x);
+                return t < fhi && t >= flo;
+            },
+            [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (in[e]) f(x[e], i[e]);
+            });
+    }
+}
+
+// The boundary's key, among the tokens that `in` keeps (limited): with MASS
+// that of the last token whose mass before is < frac times their whole mass,
+// else of the one with `count` - 1 before it; it lies in ranges
+// [lo_bin, hi_bin], the tokens themselves in those up to `last`.  `above` is
+// the amount before the boundary's ranges (MASS: summed here, and left per
+// warp in sh.wabove).
 template <bool MASS, bool CACHED>
 __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &sc,
-                            const SaSlice<CACHED> &sl, uint32_t mask, const SaKept &in, bool limited,
-                            int lo_bin, int hi_bin, u64 above, u64 count, double goal, int &buf) {
+                            const SaSlice<CACHED> &sl, const SaKept &in, bool limited, int lo_bin,
+                            int hi_bin, int last, u64 above, u64 count, double frac, int &buf) {
     const int C = (int)cl.num_blocks(), c = (int)cl.block_rank(), tid = threadIdx.x;
     const int lane = tid & 31, warp = tid >> 5;
     // the ranges' keys, a little to the safe side
@@ -226,6 +300,40 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
     uint32_t klo = sa_key(__double2float_rd(xl));
     const float flo = (float)lo_bin, fhi = (float)(hi_bin + 1);
     const float tau = limited ? in.tau : -INFINITY;
+    // collect (tau's own ties are added once, below)
+    if (tid == 0) sh.n_near = 0;
+    __syncthreads();
+    u64 a = 0, all_mass = 0;
+    const float fend = MASS ? (float)(last + 1) : fhi;
+    sl.each4(
+        [&](float x, int) {
+            const float t = sc.range(x);
+            return t < fend && (MASS || t >= flo) && x > tau;
+        },
+        [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+            bool near[4];
+            int at[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float t = sc.range(x[e]);
+                near[e] = in[e] && t >= flo && t < fhi;
+                if (MASS) {
+                    const u64 w = in[e] ? sc.weight(x[e]) : 0ull;
+                    all_mass += w;
+                    a += t < flo ? w : 0ull;
+                }
+            }
+            sa_append(&sh.n_near, near, at);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (near[e] && at[e] < SA_NEAR) sh.near[at[e]] = i[e];
+        });
+    if (MASS) {
+        a = sa_warp_sum(a);
+        all_mass = sa_warp_sum(all_mass);
+        if (lane == 0) sh.wabove[warp] = a, sh.wsum[warp] = all_mass;
+    }
+    double goal = 0;
     SaKept out;
     for (int level = 0; level < 6; level++) {
         int shift = 0;
@@ -233,31 +341,21 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
         u64 *hist = sh.fine[buf];
         hist[tid] = 0;
         __syncthreads();
-        u64 a = 0;
-        sl.each(mask, [&](float x, int) {
-            const float t = sc.range(x);
-            // tau's own ties are added once, below
-            if (!(t < fhi) || (limited && !(x > tau))) return;
-            if (t < flo) {
-                if (MASS && level == 0) a += sc.weight(x);
-                return;
-            }
+        sa_near(sh, sc, sl, flo, fhi, [&](float x, int) {
             const uint32_t k = sa_key(x);
-            if (k < klo || k > khi) return;
+            if (!(x > tau) || k < klo || k > khi) return;
             const u64 w = MASS ? sc.weight(x) : 1ull;
             if (w) atomicAdd(&hist[(khi - k) >> shift], w);
         });
-        if (MASS && level == 0) {
-            a = sa_warp_sum(a);
-            if (lane == 0) sh.wabove[warp] = a;
-        }
         __syncthreads();
         if (tid == 0) {
             if (MASS && level == 0) {
-                u64 t = 0;
+                u64 t = 0, t2 = 0;
 #pragma unroll
-                for (int w = 0; w < SA_WARPS; w++) t += sh.wabove[w];
+                for (int w = 0; w < SA_WARPS; w++) t += sh.wabove[w], t2 += sh.wsum[w];
+                if (c == 0 && limited) t2 += sc.weight(in.tau) * in.ties;
                 hist[SA_FINE] = t;
+                hist[SA_FINE + 1] = t2;
             }
             // the kept ties at tau, once for the cluster
             if (c == 0 && limited) {
@@ -267,13 +365,19 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
             }
         }
         cl.sync();
-        u64 mine = 0, amass = 0;
+        u64 mine = 0;
 #pragma unroll
         for (int k = 0; k < SA_CL; k++)
             if (k < C) mine += cl.map_shared_rank(&sh, k)->fine[buf][tid];
         if (MASS && level == 0) {
-            if (lane < C) amass = cl.map_shared_rank(&sh, lane)->fine[buf][SA_FINE];
-            above = sa_warp_sum(amass);
+            u64 t = 0, t2 = 0;
+            if (lane < C) {
+                const u64 *h = cl.map_shared_rank(&sh, lane)->fine[buf];
+                t = h[SA_FINE];
+                t2 = h[SA_FINE + 1];
+            }
+            above = sa_warp_sum(t);
+            goal = frac * (double)sa_warp_sum(t2);
         }
         buf ^= 1;
         u64 all;
@@ -383,11 +487,10 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     sl.g = a.logits + (long long)r * a.row_stride + sl.first;
     sl.nz = nz;
     sl.plane = plane;
-    const int wper = ((n_slice + SA_WARPS - 1) / SA_WARPS + 31) / 32 * 32;
-    sl.i0 = min(warp * wper, n_slice);
-    sl.i1 = min(sl.i0 + wper, n_slice);
+    sl.wper = ((n_slice + SA_WARPS - 1) / SA_WARPS + 31) / 32 * 32;
+    sl.i0 = min(warp * sl.wper, n_slice);
+    sl.i1 = min(sl.i0 + sl.wper, n_slice);
     sl.steps = (sl.i1 - sl.i0 + 31) / 32;
-    sl.per_bit = (wper / 32 + 31) / 32;
     const float T = a.temperature ? a.temperature[r] : 1.f;
     const int topk = a.top_k ? a.top_k[r] : 0;
     const float topp = a.top_p ? a.top_p[r] : 1.f;
@@ -395,9 +498,10 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     float u = a.u[r];
     u = u > 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
 
-    // 1. load the slice; its largest (key, first index)
-    u64 best = 0;
+    // 1. load the slice; its largest
+    float top = -INFINITY;
     if (tid == 0) sh.n_list = 0;
+    if (tid < 32) sh.tab[tid] = sa_tab[tid];
     for (int b = tid; b < SA_BINS; b += SA_THREADS) sh.coarse[b] = 0;
 #pragma unroll 1
     for (int j0 = 0; j0 < sl.steps; j0 += 8) {
@@ -411,82 +515,82 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int i = sl.i0 + 32 * (j0 + e) + lane;
-            if (i >= sl.i1) continue;
-            if (x[e] != x[e]) x[e] = -INFINITY;
-            if (CACHED) cache[i] = x[e];
-            best = max(best, (u64)sa_key(x[e]) << 32 | (0xffffffffu - (uint32_t)(sl.first + i)));
+            x[e] = fmaxf(x[e], -INFINITY);      // a NaN becomes -infinity
+            if (CACHED && i < sl.i1) cache[i] = x[e];
+            top = fmaxf(top, x[e]);
         }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) sh.wsum[warp] = best;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) sh.wlo[warp] = (double)top;
     __syncthreads();
     if (tid < C) {
-        u64 b = 0;
+        double b = sh.wlo[0];
 #pragma unroll
-        for (int w = 0; w < SA_WARPS; w++) b = max(b, sh.wsum[w]);
-        cl.map_shared_rank(&sh, tid)->best[c] = b;
+        for (int w = 1; w < SA_WARPS; w++) b = fmax(b, sh.wlo[w]);
+        cl.map_shared_rank(&sh, tid)->top[c] = (float)b;
     }
     cl.sync();
-    best = 0;
 #pragma unroll
     for (int k = 0; k < SA_CL; k++)
-        if (k < C) best = max(best, sh.best[k]);
+        if (k < C) top = fmaxf(top, sh.top[k]);
     SaScale sc;
-    sc.m = sa_value((uint32_t)(best >> 32));
+    sc.m = top;
+    sc.tab = sh.tab;
     if (T <= 0.f || sc.m == -INFINITY) {
+        // the first maximum
+        int at = 0x7fffffff;
+        sl.each4([&](float x, int) { return x == top; },
+                 [&](const float (&)[4], const int (&i)[4], const bool (&in)[4]) {
+#pragma unroll
+                     for (int e = 0; e < 4; e++)
+                         if (in[e]) at = min(at, sl.first + i[e]);
+                 });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) sh.wtie[warp] = at;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 0; w < SA_WARPS; w++) at = min(at, sh.wtie[w]);
+            cl.map_shared_rank(&sh, 0)->ties[c] = at;
+        }
+        cl.sync();
         if (c == 0 && tid == 0) {
+            for (int k = 0; k < C; k++) at = min(at, sh.ties[k]);
             const float x0 = bd_sum(a.logits + (long long)r * a.row_stride, nz, plane, 0);
-            a.tokens[r] = x0 != x0 || sc.m == -INFINITY ? 0 : (int)(0xffffffffu - (uint32_t)best);
+            a.tokens[r] = x0 != x0 || top == -INFINITY ? 0 : at;
         }
         return;     // the last barrier is behind every remote access
     }
     sc.md = (double)sc.m;
-    sc.lt = 1.4426950408889634 / (double)(T == T ? T : 1.f);
+    sc.lt = 1.4426950408889634 / (double)(T == T ? fminf(fmaxf(T, 1e-30f), 1e30f) : 1.f);
     sc.binf = (float)(sc.lt * ((double)SA_BINS / SA_OCTAVES));
     // min-p: a bound on the weight
     u64 wmin = 1;
     if (minp > 0.f) wmin = max(1ull, (u64)ceil((double)fminf(minp, 1.f) * 0x1p40));
     const bool use_k = topk > 0 && topk < a.vocab, use_p = topp < 1.f;
     SaKept kept = {-INFINITY, 0, 0, false};
-    uint32_t mask = sl.steps ? 0xffffffffu >> (32 - (sl.steps + sl.per_bit - 1) / sl.per_bit) : 0u;
-    bool above_known = false;
-    int buf = 0, p_lo = 0;
+    bool above_known = false, limited = false;      // limited: top-k cuts
+    float tau_k = -INFINITY;
+    int buf = 0, p_lo = 0, p_hi = 0;
     if (use_k || use_p) {
         // 2. counts, and positions in units that cannot carry into them
         int bits = 32;
         while (bits > 1 && (1u << (bits - 1)) > (uint32_t)per) bits--;     // 2^bits > per
         const int pos_bits = 32 - bits;
-        const uint32_t pos_mask = (1u << pos_bits) - 1u, Q = max(pos_mask / (uint32_t)per, 1u);
-        const bool mass = use_p && !use_k;
-        u64 sum = 0;
-#pragma unroll 1
-        for (int j0 = 0; j0 < sl.steps; j0 += 4) {
-            float x[4], t[4];
-            bool any = false;
+        const uint32_t pos_mask = (1u << pos_bits) - 1u;
+        const int q_bits = max(31 - __clz((int)max(pos_mask / (uint32_t)per, 1u)), 0);
+        const float Q = (float)(1 << q_bits);
+        sl.each4([&](float x, int) { return sc.range(x) < (float)SA_BINS; },
+                 [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = sl.i0 + 32 * (j0 + e) + lane;
-                x[e] = i < sl.i1 ? sl.at(i) : -INFINITY;
-                t[e] = sc.range(x[e]);
-                any = any || t[e] < (float)SA_BINS;
-                if (x[e] > -INFINITY && t[e] < (float)SA_BINS) {
-                    const int b = (int)t[e];
-                    atomicAdd(&sh.coarse[b],
-                              (1u << pos_bits) + (uint32_t)((t[e] - (float)b) * (float)Q));
-                }
-            }
-            if (mass && __any_sync(0xffffffffu, any))
-                sum += (sc.weight(x[0]) + sc.weight(x[1])) + (sc.weight(x[2]) + sc.weight(x[3]));
-        }
-        u64 total = 0;
-        if (mass) {
-            sum = sa_warp_sum(sum);
-            if (lane == 0) sh.wabove[warp] = sum;
-            total = sa_cluster_sum(cl, sh, &SaShared::total, sh.wabove, 0);
-        } else {
-            cl.sync();
-        }
+                     for (int e = 0; e < 4; e++) {
+                         const uint32_t t = (uint32_t)(int)(sc.range(x[e]) * Q);
+                         if (in[e])
+                             atomicAdd(&sh.coarse[t >> q_bits],
+                                       (1u << pos_bits) + (t & ((1u << q_bits) - 1u)));
+                     }
+                 });
+        cl.sync();
         uint32_t cnt[2] = {}, pos[2] = {};
 #pragma unroll
         for (int k = 0; k < SA_CL; k++)
@@ -501,7 +605,8 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
         const uint32_t first = sa_scan<uint32_t>(cnt[0] + cnt[1], reinterpret_cast<uint32_t *>(sh.wsum), &all);
         const uint32_t from[3] = {first, first + cnt[0], first + cnt[0] + cnt[1]};
         int last = SA_BINS - 1, upto = (int)all;
-        const bool limited = use_k && all > (uint32_t)topk;
+        u64 k_before = 0;
+        limited = use_k && all > (uint32_t)topk;
         if (limited) {
 #pragma unroll
             for (int j = 0; j < 2; j++)
@@ -513,103 +618,109 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
             __syncthreads();
             last = sh.sel_bin;
             upto = sh.sel_upto;
+            k_before = sh.sel_before;
         }
-        // bounds of the mass before each range: a range's tokens weigh
-        // e^(-d f) of its upper edge, f in [0, 1) their place in it and d its
-        // width, 1 - d f <= e^(-d f) <= 1 - d f + d^2 / 2
-        int p_hi = last;
-        double goal = 0;
-        auto bracket = [&]() {
-            goal = (double)topp * (double)total;
+        p_hi = last;
+        if (use_p) {
+            // Bounds of the mass up to each range: a range's tokens weigh
+            // e^(-d f) of its upper edge, f in [0, 1) their place in it and d its
+            // width, 1 - d f <= e^(-d f) <= 1 - d f + d^2 / 2.
             constexpr double d = (double)SA_OCTAVES / SA_BINS * 0.6931471805599453;
-            double lo[2], hi[2], slo = 0, shi = 0;
+            double lo[3], hi[3];
+            lo[0] = hi[0] = 0;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const double edge = 0x1p40 * (double)exp2f(-(float)(2 * tid + j) * (SA_OCTAVES / SA_BINS));
                 const double n = cnt[j], s = (double)pos[j] / Q;
-                lo[j] = slo, hi[j] = shi;        // before range j, within the thread
-                slo += edge * (1 - 1e-5) * (n * (1 - d / Q) - s * d) - n;
-                shi += edge * (1 + 1e-5) * (n * (1 + d * d / 2) - s * d) + n;
+                lo[j + 1] = lo[j] + edge * (1 - 1e-5) * (n * (1 - d / Q) - s * d) - n;
+                hi[j + 1] = hi[j] + edge * (1 + 1e-5) * (n * (1 + d * d / 2) - s * d) + n;
             }
             double sum;
-            const double blo = sa_scan<double>(slo, sh.wlo, &sum), bhi = sa_scan<double>(shi, sh.whi, &sum);
+            const double blo = sa_scan<double>(lo[2], sh.wlo, &sum), bhi = sa_scan<double>(hi[2], sh.whi, &sum);
+#pragma unroll
+            for (int j = 0; j < 3; j++) lo[j] += blo, hi[j] += bhi;
             if (tid == 0) sh.lo_bin = 0, sh.hi_bin = last;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (2 * tid + j == last) {
+                    // what top-k leaves of the last range is anything from nothing to all
+                    sh.goal_lo = (double)topp * (limited ? lo[j] : lo[j + 1]) * (1 - 1e-9);
+                    sh.goal_hi = (double)topp * hi[j + 1] * (1 + 1e-9);
+                }
             __syncthreads();
+            const double goal_lo = topp > 0.f ? sh.goal_lo : 0.0, goal_hi = topp > 0.f ? sh.goal_hi : 0.0;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int b = 2 * tid + j;
                 // the boundary lies in or behind the last range that surely starts before
                 // the goal, and before the first that surely starts behind it
-                if (b <= last && cnt[j] && bhi + hi[j] < goal * (1 - 1e-9)) atomicMax(&sh.lo_bin, b);
-                if (b <= last && b > 0 && blo + lo[j] > goal * (1 + 1e-9)) atomicMin(&sh.hi_bin, b - 1);
+                if (b <= last && cnt[j] && hi[j] < goal_lo) atomicMax(&sh.lo_bin, b);
+                if (b <= last && b > 0 && lo[j] > goal_hi) atomicMin(&sh.hi_bin, b - 1);
             }
             __syncthreads();
             p_lo = sh.lo_bin;
             p_hi = max(sh.hi_bin, p_lo);
-            if (2 * tid == p_hi) sh.sel_upto = (int)from[1];
-            if (2 * tid + 1 == p_hi) sh.sel_upto = (int)from[2];
-            __syncthreads();
-            upto = min(upto, sh.sel_upto);
-        };
-        // top-p alone: nothing behind its own ranges is looked at again (top-p
-        // after top-k: its whole mass has still to be summed)
-        if (mass) bracket();
-        // the lanes' tokens up to the last range
-        {
-            const float fhi = (float)((mass ? p_hi : last) + 1);
-            uint32_t mk = 0;
-#pragma unroll 4
-            for (int j = 0; j < sl.steps; j++) {
-                const int i = sl.i0 + 32 * j + lane;
-                const float x = i < sl.i1 ? sl.at(i) : -INFINITY;
-                if (x > -INFINITY && sc.range(x) < fhi) mk |= 1u << (sl.per_bit == 1 ? j : j / sl.per_bit);
+            if (!limited) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    if (2 * tid + j == p_hi) sh.sel_upto = (int)from[j + 1];
+                __syncthreads();
+                upto = sh.sel_upto;
             }
-            mask = mk;
-            if (upto <= SA_LIST) {
-                // 4a. to block 0, whatever the order
-                sl.each(mask, [&](float x, int i) {
-                    if (x > -INFINITY && sc.range(x) < fhi)
-                        sh.list[atomicAdd(&sh.n_list, 1)].x =
-                            (u64)sa_key(x) << 32 | (0xffffffffu - (uint32_t)(sl.first + i));
-                });
-                cl.sync();
-                int n = 0, have = 0;
-                if (c == 0) {
-                    have = sh.n_list;
-                    n = have;
-                    for (int k = 1; k < C; k++) {
-                        const SaShared *o = cl.map_shared_rank(&sh, k);
-                        const int m = o->n_list;
-                        for (int i = tid; i < m; i += SA_THREADS) sh.list[n + i].x = o->list[i].x;
-                        n += m;
-                    }
+        }
+        // (top-p after top-k: its whole mass is that of all that top-k leaves)
+        if (upto <= SA_LIST) {
+            // 4a. the tokens up to the last range to block 0, whatever the order;
+            // where top-k cuts nothing the whole mass beside them
+            const bool mass = use_p && !limited;
+            const float fhi = (float)((mass ? p_hi : last) + 1), fend = mass ? (float)SA_BINS : fhi;
+            u64 sum = 0;
+            sl.each4([&](float x, int) { return sc.range(x) < fend; },
+                     [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+                         bool near[4];
+                         int at[4];
+#pragma unroll
+                         for (int e = 0; e < 4; e++) {
+                             near[e] = in[e] && sc.range(x[e]) < fhi;
+                             if (mass) sum += in[e] ? sc.weight(x[e]) : 0ull;
+                         }
+                         sa_append(&sh.n_list, near, at);
+#pragma unroll
+                         for (int e = 0; e < 4; e++)
+                             if (near[e])
+                                 sh.list[at[e]].x =
+                                     (u64)sa_key(x[e]) << 32 | (0xffffffffu - (uint32_t)(sl.first + i[e]));
+                     });
+            u64 total = 0;
+            if (mass) {
+                sum = sa_warp_sum(sum);
+                if (lane == 0) sh.wabove[warp] = sum;
+                total = sa_cluster_sum(cl, sh, &SaShared::total, sh.wabove, 0);
+            }
+            if (!mass) cl.sync();
+            int n = 0;
+            if (c == 0) {
+                n = sh.n_list;
+                for (int k = 1; k < C; k++) {
+                    const SaShared *o = cl.map_shared_rank(&sh, k);
+                    const int m = o->n_list;
+                    for (int i = tid; i < m; i += SA_THREADS) sh.list[n + i].x = o->list[i].x;
+                    n += m;
                 }
-                cl.sync();      // the other blocks may leave
-                if (c == 0)
-                    sa_list(sh, sc, n, limited ? topk : 0, use_p ? topp : 1.f, total, wmin, u,
-                            &a.tokens[r]);
-                return;
             }
+            cl.sync();      // the other blocks may leave
+            if (c == 0)
+                sa_list(sh, sc, n, limited ? topk : 0, use_p ? topp : 1.f, total, wmin, u, &a.tokens[r]);
+            return;
         }
         // 4b. the boundary's key
         if (limited) {
-            kept = sa_narrow<false>(cl, sh, sc, sl, mask, kept, false, last, last, sh.sel_before,
-                                    (u64)topk, 0.0, buf);
+            kept = sa_narrow<false>(cl, sh, sc, sl, kept, false, last, last, last, k_before, (u64)topk,
+                                    0.0, buf);
+            tau_k = kept.tau;
         }
         if (use_p) {
-            if (!mass) {
-                // the exact mass of what top-k leaves
-                u64 t = 0;
-                sl.each(mask, [&](float x, int) {
-                    if (x > kept.tau) t += sc.weight(x);
-                });
-                t = sa_warp_sum(t);
-                if (lane == 0) sh.wabove[warp] = t;
-                const u64 extra = c == 0 && limited ? sc.weight(kept.tau) * kept.ties : 0ull;
-                total = sa_cluster_sum(cl, sh, &SaShared::total, sh.wabove, extra);
-                bracket();
-            }
-            kept = sa_narrow<true>(cl, sh, sc, sl, mask, kept, limited, p_lo, p_hi, 0, 0, goal, buf);
+            kept = sa_narrow<true>(cl, sh, sc, sl, kept, limited, p_lo, p_hi, last, 0, 0, (double)topp, buf);
             above_known = wmin <= 1;
         }
     }
@@ -617,7 +728,10 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     int icut = 0x7fffffff;
     if (kept.cut) {
         int n = 0;
-        sl.each(mask, [&](float x, int) { n += x == kept.tau; });
+        sl.each4([&](float x, int) { return x == kept.tau; },
+                 [&](const float (&)[4], const int (&)[4], const bool (&in)[4]) {
+                     n += in[0] + in[1] + in[2] + in[3];
+                 });
         const int nw = __reduce_add_sync(0xffffffffu, n);
         if (lane == 0) sh.wtie[warp] = nw;
         __syncthreads();
@@ -657,36 +771,33 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
         const u64 w = sc.weight(x);
         return w >= wmin && keeps(x, i) ? w : 0;
     };
-    u64 sum = 0;
-    if (above_known) {      // the mass before step 4b's ranges is there
-        const float flo = (float)p_lo;
-        sl.each(mask, [&](float x, int i) {
-            if (keeps(x, i) && !(sc.range(x) < flo)) sum += sc.weight(x);
+    u64 sum;
+    if (above_known) {
+        // step 4b left the mass before its ranges; the collected tokens', and
+        // those of top-k's own last logit where top-p stopped there
+        __syncthreads();
+        if (lane == 0) sh.wsum[warp] = sh.wabove[warp];
+        __syncthreads();
+        sa_near(sh, sc, sl, (float)p_lo, (float)(p_hi + 1), [&](float x, int i) {
+            if (x > tau_k && keeps(x, i)) atomicAdd(&sh.wsum[i / sl.wper], sc.weight(x));
         });
-        sum = sa_warp_sum(sum) + sh.wabove[warp];
-    } else if (use_k || use_p) {
-        sl.each(mask, [&](float x, int i) {
-            if (keeps(x, i)) sum += mass_of(x, i);
-        });
-        sum = sa_warp_sum(sum);
+        if (limited && kept.tau <= tau_k)
+            sl.each4([&](float x, int i) { return x == tau_k && keeps(x, i); },
+                     [&](const float (&)[4], const int (&)[4], const bool (&in)[4]) {
+                         atomicAdd(&sh.wsum[warp], (u64)(in[0] + in[1] + in[2] + in[3]) * sc.weight(tau_k));
+                     });
+        __syncthreads();
+        sum = sh.wsum[warp];
     } else {
-#pragma unroll 1
-        for (int j0 = 0; j0 < sl.steps; j0 += 4) {
-            float x[4];
-            bool any = false;
+        sum = 0;
+        sl.each4([&](float x, int i) { return keeps(x, i) && sc.range(x) < (float)SA_BINS; },
+                 [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
+                     u64 w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = sl.i0 + 32 * (j0 + e) + lane;
-                x[e] = i < sl.i1 ? sl.at(i) : -INFINITY;
-                any = any || sc.range(x[e]) < (float)SA_BINS;
-            }
-            if (__any_sync(0xffffffffu, any))
+                     for (int e = 0; e < 4; e++) w[e] = sc.weight(x[e]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const u64 w = sc.weight(x[e]);
-                    sum += w >= wmin ? w : 0;
-                }
-        }
+                     for (int e = 0; e < 4; e++) sum += in[e] && w[e] >= wmin ? w[e] : 0ull;
+                 });
         sum = sa_warp_sum(sum);
     }
     __syncthreads();
