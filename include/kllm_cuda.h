@@ -316,8 +316,9 @@ int kllm_batch_attention(const kllm_batch_attn *a, void *stream);
  *           exceeds u times their whole sum
  * top_k <= 0, top_p >= 1 and min_p <= 0 turn a rule off; temperature <= 0
  * picks the first maximum, by the rule of the greedy decode (a NaN at index
- * 0 picks 0).  Where no logit is above -infinity the token is 0; where some
- * are +infinity those share the mass alone.  u is taken into [0, 1); NaN
+ * 0 picks 0).  Where no logit is above -infinity the token is 0; +infinity
+ * counts as the largest number; temperatures are taken into [1e-30, 1e30], u
+ * into [0, 1); NaN
  * settings are refused nowhere and turn their rule off (u: 0).
  * Weights are 2^-40 fixed point, their sums exact integers: a row's token
  * does not depend on the launch or on the other rows.  vocab is at most

@@ -33,6 +33,7 @@
 // temperature), another for the kept ones; few rows wait for the chain of
 // dependent steps.
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include <algorithm>
 #include <mutex>
@@ -48,12 +49,14 @@ typedef unsigned long long u64;
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_CL = 8;
 constexpr int SA_BINS = 1024, SA_FINE = 512;       // ranges of step 2; keys of step 4b
-constexpr int SA_LIST = SA_THREADS;                // most tokens of step 4a
+constexpr int SA_RPT = SA_BINS / SA_THREADS, SA_FPT = SA_FINE / SA_THREADS;   // of each per thread
+constexpr int SA_LIST = 512;                       // most tokens of step 4a
+constexpr int SA_LPT = SA_LIST / SA_THREADS;
 constexpr int SA_NEAR = 2048;                      // most collected tokens of a block in step 4b
 constexpr float SA_OCTAVES = 41.5f;                // weights below 2^-41 of the largest are zero
 constexpr int SA_VOCAB = 1 << 22;                  // sums stay below 2^62
 constexpr size_t SA_CACHE = 180 * 1024;            // slice bytes that are kept on chip
-static_assert(SA_BINS == 2 * SA_THREADS && SA_FINE == SA_THREADS, "one thread per two ranges, per key");
+static_assert(SA_RPT == 2 && SA_FPT == 1, "loads of 8 bytes per thread");
 
 // Order-preserving integer of a logit (no NaN); one for both zeros.
 __device__ __forceinline__ uint32_t sa_key(float x) {
@@ -149,21 +152,25 @@ struct SaKept {
     bool cut;
 };
 
-// The row's weights: its maximum, log2(e) / T, ranges per logit.
+// The row's weights: its maximum, log2(e) / T, units per logit (2^q_bits to a
+// range of step 2).
 struct SaScale {
-    float m, binf;
+    float m, unit;
+    int q_bits;
     double md, lt;
     const uint32_t *tab;    // sa_tab in shared memory
 
-    // Range of the distance to the maximum, as a number.
-    __device__ __forceinline__ float range(float x) const { return x == m ? 0.f : (m - x) * binf; }
+    // Distance to the maximum in units.
+    __device__ __forceinline__ float dist(float x) const { return (m - x) * unit; }
+    __device__ __forceinline__ float units(int range) const { return (float)(range << q_bits); }
 
     // Weight of a logit, 2^-40 fixed point: t = (m - x) log2(e) / T in double precision, its whole
-    // part n and a fraction of 32 bits by one addition (conversions from and to 64 bits are slow);
-    // 2^-fraction as a table's 2^-(j / 32), one word a bank, times 1 - z (c1 - z (c2 - z c3)), the
+    // part n and a fraction of 32 bits by one addition (conversions from and to 64 bits are slow):
+    // the sum of t and 1.5 * 2^20 has n in its upper word and the fraction in its lower.
+    // 2^-fraction is a table's 2^-(j / 32), one word a bank, times 1 - z (c1 - z (c2 - z c3)), the
     // polynomial that meets 2^-z at the Chebyshev nodes of [0, 1/32), all as 32-bit fractions
-    // (relative error below 2^-29); the sum of t and 1.5 * 2^20 has n in its upper word and the
-    // fraction in its lower.  No branch: several tokens' chains overlap.
+    // (relative error below 2^-29); the shift by n and the rounding are one addition of 2^52.
+    // No branch: several tokens' chains overlap.
     __device__ __forceinline__ u64 weight(float x) const {
         // the float's bits as a double's (what is below 2^-126 becomes some number below it,
         // -infinity becomes -2^128)
@@ -171,64 +178,65 @@ struct SaScale {
         const double xd = __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
                                            (int)(b << 29));
         const double y = fma(md - xd, lt, 0x1.8p20);
-        const uint32_t n = (uint32_t)__double2hiint(y) - 0x41380000u, lo = (uint32_t)__double2loint(y);
-        const uint32_t z = lo & 0x07ffffffu, t = tab[lo >> 27];
+        const uint32_t n = min((uint32_t)__double2hiint(y) - 0x41380000u, 63u);
+        const uint32_t lo = (uint32_t)__double2loint(y), z = lo & 0x07ffffffu, t = tab[lo >> 27];
         uint32_t q = 0x3d7f23e8u - __umulhi(z, 0x0e181d25u);
         q = 0xb17217d1u - __umulhi(z, q);
         const uint32_t f = t - __umulhi(t, __umulhi(z, q));
-        const u64 w = ((((u64)f << 9) >> (n & 63u)) + 1) >> 1;
-        return x == m ? 1ull << 40 : n <= 41u ? w : 0ull;
+        const double v = __hiloint2double(0x43300000, (int)f) - 0x1p52;        // f as a double
+        const double r = fma(v, __hiloint2double((int)((1031u - n) << 20), 0), 0x1p52);   // f 2^(8 - n)
+        return (u64)(__double2hiint(r) & 0xfffff) << 32 | (uint32_t)__double2loint(r);
     }
 };
 
 // A block's slice of the row.
 template <bool CACHED>
 struct SaSlice {
-    float *cache;           // the slice in shared memory (CACHED)
+    float *cache;           // the slice in shared memory (CACHED), -infinity behind its end
     const float *g;         // in global memory
     int nz;
     long long plane;
-    int first;              // index of its first token
-    int wper, i0, i1, steps;    // tokens per warp, this warp's part, and its 32-token steps
+    int first, n;           // index of its first token, tokens
+    int wper, i0;           // tokens per warp (a multiple of 128), this warp's first
 
-    // a logit of the slice, NaN as -infinity
+    // a logit, NaN as -infinity, +infinity as the largest number
+    static __device__ __forceinline__ float tame(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
     __device__ __forceinline__ float at(int i) const {
         if constexpr (CACHED) return cache[i];
-        const float x = bd_sum(g, nz, plane, i);
-        return x != x ? -INFINITY : x;
+        return i < n ? tame(bd_sum(g, nz, plane, i)) : -INFINITY;
     }
-    // Steps four at a time: f(x, i, in) with four of this lane's tokens, their places in the slice
-    // and whether each is `wanted` (never -infinity), where any of the warp's is.
+    __device__ __forceinline__ float4 at4(int i) const {
+        if constexpr (CACHED) return *reinterpret_cast<const float4 *>(cache + i);
+        return make_float4(at(i), at(i + 1), at(i + 2), at(i + 3));
+    }
+    // f(x, i, in) with four tokens in a row of this lane, the first one's place in the slice and
+    // whether each is `wanted` (never -infinity), where any of the warp's is.
     template <class P, class F>
     __device__ __forceinline__ void each4(P &&wanted, F &&f) const {
-        const int lane = threadIdx.x & 31;
+        int i = i0 + 4 * (threadIdx.x & 31);
+        const int end = min(i0 + wper, n);      // (the warp's: the same for its lanes)
 #pragma unroll 1
-        for (int j0 = 0; j0 < steps; j0 += 4) {
-            float x[4];
-            int i[4];
+        for (int j = i0; j < end; j += 128, i += 128) {
+            const float4 v = at4(i);
+            const float x[4] = {v.x, v.y, v.z, v.w};
             bool in[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                i[e] = i0 + 32 * (j0 + e) + lane;
-                x[e] = i[e] < i1 ? at(i[e]) : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) in[e] = wanted(x[e], i[e]);
-            if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) f(x, i, in);
+            for (int e = 0; e < 4; e++) in[e] = wanted(x[e], i + e);
+            if (__any_sync(0xffffffffu, (in[0] || in[1]) || (in[2] || in[3]))) f(x, i, in);
         }
     }
-    // the sum of this lane's wanted tokens' weights
-    template <class P>
-    __device__ __forceinline__ u64 mass(const SaScale &sc, P &&wanted) const {
-        u64 sum = 0;
-        each4(wanted, [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
-            u64 w[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = sc.weight(x[e]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += in[e] ? w[e] : 0ull;
-        });
-        return sum;
+    // f(x, i) for the tokens of a lane's share of the warp's part, when each lane takes a run of
+    // them (lanes start at different places of theirs: few bank conflicts)
+    template <class F>
+    __device__ __forceinline__ void run4(F &&f) const {
+        const int lane = threadIdx.x & 31, len = wper / 128, base = i0 + lane * 4 * len;
+        int q = lane % len;
+#pragma unroll 2
+        for (int e = 0; e < len; e++) {
+            const float4 v = at4(base + 4 * q);
+            f(v.x, base + 4 * q), f(v.y, base + 4 * q + 1), f(v.z, base + 4 * q + 2), f(v.w, base + 4 * q + 3);
+            q = q + 1 < len ? q + 1 : 0;
+        }
     }
 };
 
@@ -246,10 +254,8 @@ __device__ __forceinline__ void sa_append(int *length, const bool (&in)[4], int 
         n += __popc(b[e]);
     }
     int first = 0;
-    if (n) {
-        if (lane == 0) first = atomicAdd(length, n);
-        first = __shfl_sync(0xffffffffu, first, 0);
-    }
+    if (lane == 0) first = atomicAdd(length, n);
+    first = __shfl_sync(0xffffffffu, first, 0);
 #pragma unroll
     for (int e = 0; e < 4; e++) at[e] += first;
 }
@@ -269,13 +275,13 @@ __device__ __forceinline__ void sa_near(const SaShared &sh, const SaScale &sc, c
     } else {
         sl.each4(
             [&](float x, int) {
-                const float t = sc.range(x);
+                const float t = sc.dist(x);
                 return t < fhi && t >= flo;
             },
-            [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+            [&](const float (&x)[4], int i, const bool (&in)[4]) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (in[e]) f(x[e], i[e]);
+                    if (in[e]) f(x[e], i + e);
             });
     }
 }
@@ -293,40 +299,42 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
     const int C = (int)cl.num_blocks(), c = (int)cl.block_rank(), tid = threadIdx.x;
     const int lane = tid & 31, warp = tid >> 5;
     // the ranges' keys, a little to the safe side
-    const double step = 1.0 / (double)sc.binf;
+    const double step = (double)(1 << sc.q_bits) / (double)sc.unit;
     const double xh = lo_bin ? sc.md - (double)lo_bin * step * (1 - 1e-6) : sc.md;
     const double xl = sc.md - (double)(hi_bin + 1) * step * (1 + 1e-6);
     uint32_t khi = sa_key(lo_bin ? fminf(__double2float_ru(xh), sc.m) : sc.m);
     uint32_t klo = sa_key(__double2float_rd(xl));
-    const float flo = (float)lo_bin, fhi = (float)(hi_bin + 1);
+    const float flo = sc.units(lo_bin), fhi = sc.units(hi_bin + 1);
     const float tau = limited ? in.tau : -INFINITY;
     // collect (tau's own ties are added once, below)
     if (tid == 0) sh.n_near = 0;
     __syncthreads();
     u64 a = 0, all_mass = 0;
-    const float fend = MASS ? (float)(last + 1) : fhi;
+    const float fend = MASS ? sc.units(last + 1) : fhi;
     sl.each4(
         [&](float x, int) {
-            const float t = sc.range(x);
+            const float t = sc.dist(x);
             return t < fend && (MASS || t >= flo) && x > tau;
         },
-        [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+        [&](const float (&x)[4], int i, const bool (&in)[4]) {
             bool near[4];
             int at[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float t = sc.range(x[e]);
+                const float t = sc.dist(x[e]);
                 near[e] = in[e] && t >= flo && t < fhi;
                 if (MASS) {
-                    const u64 w = in[e] ? sc.weight(x[e]) : 0ull;
+                    u64 w = sc.weight(x[e]);
+                    if (limited && !in[e]) w = 0;
                     all_mass += w;
-                    a += t < flo ? w : 0ull;
+                    if (t < flo) a += w;
                 }
             }
+            if (!__any_sync(0xffffffffu, (near[0] || near[1]) || (near[2] || near[3]))) return;
             sa_append(&sh.n_near, near, at);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (near[e] && at[e] < SA_NEAR) sh.near[at[e]] = i[e];
+                if (near[e] && at[e] < SA_NEAR) sh.near[at[e]] = i + e;
         });
     if (MASS) {
         a = sa_warp_sum(a);
@@ -339,7 +347,7 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
         int shift = 0;
         while (((khi - klo) >> shift) >= (uint32_t)SA_FINE) shift++;
         u64 *hist = sh.fine[buf];
-        hist[tid] = 0;
+        for (int b = tid; b < SA_FINE; b += SA_THREADS) hist[b] = 0;
         __syncthreads();
         sa_near(sh, sc, sl, flo, fhi, [&](float x, int) {
             const uint32_t k = sa_key(x);
@@ -359,16 +367,18 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
             }
             // the kept ties at tau, once for the cluster
             if (c == 0 && limited) {
-                const float t = sc.range(in.tau);
+                const float t = sc.dist(in.tau);
                 if (t >= flo && t < fhi && in.key >= klo && in.key <= khi)
                     hist[(khi - in.key) >> shift] += MASS ? sc.weight(in.tau) * in.ties : in.ties;
             }
         }
         cl.sync();
-        u64 mine = 0;
+        u64 mine[SA_FPT] = {};
 #pragma unroll
         for (int k = 0; k < SA_CL; k++)
-            if (k < C) mine += cl.map_shared_rank(&sh, k)->fine[buf][tid];
+            if (k < C) {
+                mine[0] += cl.map_shared_rank(&sh, k)->fine[buf][tid];
+            }
         if (MASS && level == 0) {
             u64 t = 0, t2 = 0;
             if (lane < C) {
@@ -381,13 +391,18 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
         }
         buf ^= 1;
         u64 all;
-        const u64 before = above + sa_scan<u64>(mine, sh.wsum, &all), end = above + all;
+        u64 before = above + sa_scan<u64>(mine[0], sh.wsum, &all);
+        const u64 end = above + all;
         auto keep = [&](u64 b) { return MASS ? (double)b < goal || b == 0 : b < count; };
         // one thread: the last non-empty range that starts before the boundary
-        if (mine && keep(before) && (before + mine == end || !keep(before + mine))) {
-            sh.sel_bin = tid;
-            sh.sel_before = before;
-            sh.sel_amount = mine;
+#pragma unroll
+        for (int e = 0; e < SA_FPT; e++) {
+            if (mine[e] && keep(before) && (before + mine[e] == end || !keep(before + mine[e]))) {
+                sh.sel_bin = SA_FPT * tid + e;
+                sh.sel_before = before;
+                sh.sel_amount = mine[e];
+            }
+            before += mine[e];
         }
         __syncthreads();
         const uint32_t bin = (uint32_t)sh.sel_bin;
@@ -420,28 +435,38 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
     return out;
 }
 
-// Step 4a, in block 0: the n tokens of sh.list, one per thread.  `whole`: the
+// Step 4a, in block 0: the n tokens of sh.list, SA_LPT per thread.  `whole`: the
 // mass that top-p is a part of, 0: that of what top-k leaves of the list.
 __device__ void sa_list(SaShared &sh, const SaScale &sc, int n, int k, float p, u64 whole, u64 wmin,
                         float u, int *token) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    u64 id = 0, w = 0, before = 0;
-    int rank = 0;
-    if (tid < n) {
-        id = sh.list[tid].x;
-        w = sc.weight(sa_value((uint32_t)(id >> 32)));
-        sh.list[tid].y = w;
+    u64 id[SA_LPT], w[SA_LPT], before[SA_LPT];
+    int rank[SA_LPT];
+    bool keep[SA_LPT];
+#pragma unroll
+    for (int e = 0; e < SA_LPT; e++) {
+        const int q = e * SA_THREADS + tid;
+        id[e] = w[e] = before[e] = 0;
+        rank[e] = 0;
+        if (q < n) {
+            id[e] = sh.list[q].x;
+            w[e] = sc.weight(sa_value((uint32_t)(id[e] >> 32)));
+            sh.list[q].y = w[e];
+        }
     }
     __syncthreads();
     if (warp * 32 < n)
 #pragma unroll 4
         for (int j = 0; j < n; j++) {
             const ulonglong2 t = sh.list[j];
-            if (t.x > id) before += t.y, rank++;
+#pragma unroll
+            for (int e = 0; e < SA_LPT; e++)
+                if (t.x > id[e]) before[e] += t.y, rank[e]++;
         }
-    // (an id is 0 only past the list)
-    bool keep = tid < n && (k <= 0 || rank < k);
-    auto sum = [&](u64 v) {
+    auto sum = [&](bool (&in)[SA_LPT]) {
+        u64 v = 0;
+#pragma unroll
+        for (int e = 0; e < SA_LPT; e++) v += in[e] ? w[e] : 0;
         v = sa_warp_sum(v);
         __syncthreads();
         if (lane == 0) sh.wsum[warp] = v;
@@ -451,31 +476,41 @@ __device__ void sa_list(SaShared &sh, const SaScale &sc, int n, int k, float p, 
         for (int i = 0; i < SA_WARPS; i++) t += sh.wsum[i];
         return t;
     };
+#pragma unroll
+    for (int e = 0; e < SA_LPT; e++) keep[e] = e * SA_THREADS + tid < n && (k <= 0 || rank[e] < k);
     if (p < 1.f) {
-        const double goal = (double)p * (double)(whole ? whole : sum(keep ? w : 0));
-        keep = keep && ((double)before < goal || rank == 0);
+        const double goal = (double)p * (double)(whole ? whole : sum(keep));
+#pragma unroll
+        for (int e = 0; e < SA_LPT; e++) keep[e] = keep[e] && ((double)before[e] < goal || rank[e] == 0);
     }
-    keep = keep && (w >= wmin || rank == 0);
-    const double goal = (double)u * (double)sum(keep ? w : 0);
-    if (tid < n) sh.list[tid].y = keep ? w : 0;
+#pragma unroll
+    for (int e = 0; e < SA_LPT; e++) keep[e] = keep[e] && (w[e] >= wmin || rank[e] == 0);
+    const double goal = (double)u * (double)sum(keep);
+#pragma unroll
+    for (int e = 0; e < SA_LPT; e++)
+        if (e * SA_THREADS + tid < n) sh.list[e * SA_THREADS + tid].y = keep[e] ? w[e] : 0;
     __syncthreads();
     if (warp * 32 < n) {
-        u64 to = 0;       // kept mass of indexes up to this one: ~index from ~0 down
-        const uint32_t mine = (uint32_t)id;
+        u64 to[SA_LPT] = {};       // kept mass of indexes up to this one: ~index from ~0 down
 #pragma unroll 4
         for (int j = 0; j < n; j++) {
             const ulonglong2 t = sh.list[j];
-            if ((uint32_t)t.x >= mine) to += t.y;
+#pragma unroll
+            for (int e = 0; e < SA_LPT; e++)
+                if ((uint32_t)t.x >= (uint32_t)id[e]) to[e] += t.y;
         }
-        if (keep && w && (double)to > goal && (double)(to - w) <= goal)
-            *token = (int)(0xffffffffu - mine);
+#pragma unroll
+        for (int e = 0; e < SA_LPT; e++)
+            if (keep[e] && w[e] && (double)to[e] > goal && (double)(to[e] - w[e]) <= goal)
+                *token = (int)(0xffffffffu - (uint32_t)id[e]);
     }
 }
 
 template <bool CACHED>
 __global__ void __launch_bounds__(SA_THREADS, 2)
-k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
-    extern __shared__ float cache[];
+k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, int pos_bits,
+         int q_bits, bool vec) {
+    extern __shared__ __align__(16) float cache[];
     __shared__ SaShared sh;
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
@@ -483,14 +518,12 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     SaSlice<CACHED> sl;
     sl.cache = cache;
     sl.first = min(c * per, a.vocab);
-    const int n_slice = min(per, a.vocab - sl.first);
+    sl.n = min(per, a.vocab - sl.first);
     sl.g = a.logits + (long long)r * a.row_stride + sl.first;
     sl.nz = nz;
     sl.plane = plane;
-    sl.wper = ((n_slice + SA_WARPS - 1) / SA_WARPS + 31) / 32 * 32;
-    sl.i0 = min(warp * sl.wper, n_slice);
-    sl.i1 = min(sl.i0 + sl.wper, n_slice);
-    sl.steps = (sl.i1 - sl.i0 + 31) / 32;
+    sl.wper = wper;
+    sl.i0 = warp * wper;
     const float T = a.temperature ? a.temperature[r] : 1.f;
     const int topk = a.top_k ? a.top_k[r] : 0;
     const float topp = a.top_p ? a.top_p[r] : 1.f;
@@ -503,22 +536,21 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     if (tid == 0) sh.n_list = 0;
     if (tid < 32) sh.tab[tid] = sa_tab[tid];
     for (int b = tid; b < SA_BINS; b += SA_THREADS) sh.coarse[b] = 0;
-#pragma unroll 1
-    for (int j0 = 0; j0 < sl.steps; j0 += 8) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int i = sl.i0 + 32 * (j0 + e) + lane;
-            x[e] = -INFINITY;
-            if (i < sl.i1) x[e] = nz == 1 ? __ldg(sl.g + i) : bd_sum(sl.g, nz, plane, i);
+#pragma unroll 4
+    for (int j = 0; j < wper; j += 128) {
+        const int i = sl.i0 + j + 4 * lane;
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (vec && i < sl.n) {      // (n is a multiple of four then)
+            v = __ldg(reinterpret_cast<const float4 *>(sl.g + i));
+        } else if (!vec) {
+            if (i < sl.n) v.x = bd_sum(sl.g, nz, plane, i);
+            if (i + 1 < sl.n) v.y = bd_sum(sl.g, nz, plane, i + 1);
+            if (i + 2 < sl.n) v.z = bd_sum(sl.g, nz, plane, i + 2);
+            if (i + 3 < sl.n) v.w = bd_sum(sl.g, nz, plane, i + 3);
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int i = sl.i0 + 32 * (j0 + e) + lane;
-            x[e] = fmaxf(x[e], -INFINITY);      // a NaN becomes -infinity
-            if (CACHED && i < sl.i1) cache[i] = x[e];
-            top = fmaxf(top, x[e]);
-        }
+        v.x = sl.tame(v.x), v.y = sl.tame(v.y), v.z = sl.tame(v.z), v.w = sl.tame(v.w);
+        if (CACHED) *reinterpret_cast<float4 *>(cache + i) = v;
+        top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -540,11 +572,11 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     if (T <= 0.f || sc.m == -INFINITY) {
         // the first maximum
         int at = 0x7fffffff;
-        sl.each4([&](float x, int) { return x == top; },
-                 [&](const float (&)[4], const int (&i)[4], const bool (&in)[4]) {
+        sl.each4([&](float x, int i) { return x == top && i < sl.n; },
+                 [&](const float (&)[4], int i, const bool (&in)[4]) {
 #pragma unroll
                      for (int e = 0; e < 4; e++)
-                         if (in[e]) at = min(at, sl.first + i[e]);
+                         if (in[e]) at = min(at, sl.first + i + e);
                  });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) sh.wtie[warp] = at;
@@ -563,10 +595,13 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     }
     sc.md = (double)sc.m;
     sc.lt = 1.4426950408889634 / (double)(T == T ? fminf(fmaxf(T, 1e-30f), 1e30f) : 1.f);
-    sc.binf = (float)(sc.lt * ((double)SA_BINS / SA_OCTAVES));
-    // min-p: a bound on the weight
+    sc.q_bits = q_bits;
+    sc.unit = (float)(sc.lt * (double)(SA_BINS << q_bits) / (double)SA_OCTAVES);
+    const float f_all = sc.units(SA_BINS);      // weights are zero from here on
+    // min-p: a bound on the weight, which the largest always meets
     u64 wmin = 1;
-    if (minp > 0.f) wmin = max(1ull, (u64)ceil((double)fminf(minp, 1.f) * 0x1p40));
+    if (minp > 0.f)
+        wmin = min(max(1ull, (u64)ceil((double)fminf(minp, 1.f) * 0x1p40)), sc.weight(sc.m));
     const bool use_k = topk > 0 && topk < a.vocab, use_p = topp < 1.f;
     SaKept kept = {-INFINITY, 0, 0, false};
     bool above_known = false, limited = false;      // limited: top-k cuts
@@ -574,44 +609,43 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     int buf = 0, p_lo = 0, p_hi = 0;
     if (use_k || use_p) {
         // 2. counts, and positions in units that cannot carry into them
-        int bits = 32;
-        while (bits > 1 && (1u << (bits - 1)) > (uint32_t)per) bits--;     // 2^bits > per
-        const int pos_bits = 32 - bits;
         const uint32_t pos_mask = (1u << pos_bits) - 1u;
-        const int q_bits = max(31 - __clz((int)max(pos_mask / (uint32_t)per, 1u)), 0);
-        const float Q = (float)(1 << q_bits);
-        sl.each4([&](float x, int) { return sc.range(x) < (float)SA_BINS; },
-                 [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
+        const double Q = (double)(1 << q_bits);
+        sl.each4([&](float x, int) { return sc.dist(x) < f_all; },
+                 [&](const float (&x)[4], int, const bool (&in)[4]) {
 #pragma unroll
                      for (int e = 0; e < 4; e++) {
-                         const uint32_t t = (uint32_t)(int)(sc.range(x[e]) * Q);
+                         const uint32_t t = (uint32_t)(int)sc.dist(x[e]);
                          if (in[e])
                              atomicAdd(&sh.coarse[t >> q_bits],
                                        (1u << pos_bits) + (t & ((1u << q_bits) - 1u)));
                      }
                  });
         cl.sync();
-        uint32_t cnt[2] = {}, pos[2] = {};
+        uint32_t cnt[SA_RPT] = {}, pos[SA_RPT] = {};
 #pragma unroll
         for (int k = 0; k < SA_CL; k++)
             if (k < C) {
                 const uint2 v = reinterpret_cast<const uint2 *>(cl.map_shared_rank(&sh, k)->coarse)[tid];
-                cnt[0] += v.x >> pos_bits, pos[0] += v.x & pos_mask;
-                cnt[1] += v.y >> pos_bits, pos[1] += v.y & pos_mask;
+                const uint32_t w[SA_RPT] = {v.x, v.y};
+#pragma unroll
+                for (int j = 0; j < SA_RPT; j++) cnt[j] += w[j] >> pos_bits, pos[j] += w[j] & pos_mask;
             }
         // 3. the last range that top-k leaves (with fewer tokens that carry
         // weight it cuts nothing)
         uint32_t all;
-        const uint32_t first = sa_scan<uint32_t>(cnt[0] + cnt[1], reinterpret_cast<uint32_t *>(sh.wsum), &all);
-        const uint32_t from[3] = {first, first + cnt[0], first + cnt[0] + cnt[1]};
+        uint32_t from[SA_RPT + 1];
+        from[0] = sa_scan<uint32_t>(cnt[0] + cnt[1], reinterpret_cast<uint32_t *>(sh.wsum), &all);
+#pragma unroll
+        for (int j = 0; j < SA_RPT; j++) from[j + 1] = from[j] + cnt[j];
         int last = SA_BINS - 1, upto = (int)all;
         u64 k_before = 0;
         limited = use_k && all > (uint32_t)topk;
         if (limited) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < SA_RPT; j++)
                 if (from[j] < (uint32_t)topk && from[j + 1] >= (uint32_t)topk) {
-                    sh.sel_bin = 2 * tid + j;
+                    sh.sel_bin = SA_RPT * tid + j;
                     sh.sel_before = from[j];
                     sh.sel_upto = (int)from[j + 1];
                 }
@@ -626,23 +660,23 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
             // e^(-d f) of its upper edge, f in [0, 1) their place in it and d its
             // width, 1 - d f <= e^(-d f) <= 1 - d f + d^2 / 2.
             constexpr double d = (double)SA_OCTAVES / SA_BINS * 0.6931471805599453;
-            double lo[3], hi[3];
+            double lo[SA_RPT + 1], hi[SA_RPT + 1];
             lo[0] = hi[0] = 0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const double edge = 0x1p40 * (double)exp2f(-(float)(2 * tid + j) * (SA_OCTAVES / SA_BINS));
+            for (int j = 0; j < SA_RPT; j++) {
+                const double edge = 0x1p40 * (double)exp2f(-(float)(SA_RPT * tid + j) * (SA_OCTAVES / SA_BINS));
                 const double n = cnt[j], s = (double)pos[j] / Q;
                 lo[j + 1] = lo[j] + edge * (1 - 1e-5) * (n * (1 - d / Q) - s * d) - n;
                 hi[j + 1] = hi[j] + edge * (1 + 1e-5) * (n * (1 + d * d / 2) - s * d) + n;
             }
             double sum;
-            const double blo = sa_scan<double>(lo[2], sh.wlo, &sum), bhi = sa_scan<double>(hi[2], sh.whi, &sum);
+            const double blo = sa_scan<double>(lo[SA_RPT], sh.wlo, &sum), bhi = sa_scan<double>(hi[SA_RPT], sh.whi, &sum);
 #pragma unroll
-            for (int j = 0; j < 3; j++) lo[j] += blo, hi[j] += bhi;
+            for (int j = 0; j <= SA_RPT; j++) lo[j] += blo, hi[j] += bhi;
             if (tid == 0) sh.lo_bin = 0, sh.hi_bin = last;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (2 * tid + j == last) {
+            for (int j = 0; j < SA_RPT; j++)
+                if (SA_RPT * tid + j == last) {
                     // what top-k leaves of the last range is anything from nothing to all
                     sh.goal_lo = (double)topp * (limited ? lo[j] : lo[j + 1]) * (1 - 1e-9);
                     sh.goal_hi = (double)topp * hi[j + 1] * (1 + 1e-9);
@@ -650,8 +684,8 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
             __syncthreads();
             const double goal_lo = topp > 0.f ? sh.goal_lo : 0.0, goal_hi = topp > 0.f ? sh.goal_hi : 0.0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int b = 2 * tid + j;
+            for (int j = 0; j < SA_RPT; j++) {
+                const int b = SA_RPT * tid + j;
                 // the boundary lies in or behind the last range that surely starts before
                 // the goal, and before the first that surely starts behind it
                 if (b <= last && cnt[j] && hi[j] < goal_lo) atomicMax(&sh.lo_bin, b);
@@ -662,8 +696,8 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
             p_hi = max(sh.hi_bin, p_lo);
             if (!limited) {
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    if (2 * tid + j == p_hi) sh.sel_upto = (int)from[j + 1];
+                for (int j = 0; j < SA_RPT; j++)
+                    if (SA_RPT * tid + j == p_hi) sh.sel_upto = (int)from[j + 1];
                 __syncthreads();
                 upto = sh.sel_upto;
             }
@@ -673,23 +707,24 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
             // 4a. the tokens up to the last range to block 0, whatever the order;
             // where top-k cuts nothing the whole mass beside them
             const bool mass = use_p && !limited;
-            const float fhi = (float)((mass ? p_hi : last) + 1), fend = mass ? (float)SA_BINS : fhi;
+            const float fhi = sc.units((mass ? p_hi : last) + 1), fend = mass ? f_all : fhi;
             u64 sum = 0;
-            sl.each4([&](float x, int) { return sc.range(x) < fend; },
-                     [&](const float (&x)[4], const int (&i)[4], const bool (&in)[4]) {
+            sl.each4([&](float x, int) { return sc.dist(x) < fend; },
+                     [&](const float (&x)[4], int i, const bool (&in)[4]) {
                          bool near[4];
                          int at[4];
 #pragma unroll
                          for (int e = 0; e < 4; e++) {
-                             near[e] = in[e] && sc.range(x[e]) < fhi;
-                             if (mass) sum += in[e] ? sc.weight(x[e]) : 0ull;
+                             near[e] = in[e] && sc.dist(x[e]) < fhi;
+                             if (mass) sum += sc.weight(x[e]);
                          }
+                         if (!__any_sync(0xffffffffu, near[0] || near[1] || near[2] || near[3])) return;
                          sa_append(&sh.n_list, near, at);
 #pragma unroll
                          for (int e = 0; e < 4; e++)
                              if (near[e])
                                  sh.list[at[e]].x =
-                                     (u64)sa_key(x[e]) << 32 | (0xffffffffu - (uint32_t)(sl.first + i[e]));
+                                     (u64)sa_key(x[e]) << 32 | (0xffffffffu - (uint32_t)(sl.first + i + e));
                      });
             u64 total = 0;
             if (mass) {
@@ -729,7 +764,7 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     if (kept.cut) {
         int n = 0;
         sl.each4([&](float x, int) { return x == kept.tau; },
-                 [&](const float (&)[4], const int (&)[4], const bool (&in)[4]) {
+                 [&](const float (&)[4], int, const bool (&in)[4]) {
                      n += in[0] + in[1] + in[2] + in[3];
                  });
         const int nw = __reduce_add_sync(0xffffffffu, n);
@@ -747,18 +782,28 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
         for (int w = 0; w < warp; w++) before += sh.wtie[w];
         if (before < kept.ties && before + nw >= kept.ties) {
             // the (kept.ties - before)-th tie of this warp's part
-            int need = (int)(kept.ties - before);
-#pragma unroll 4
-            for (int j = 0; j < sl.steps; j++) {
-                const int i = sl.i0 + 32 * j + lane;
-                unsigned b = __ballot_sync(0xffffffffu, i < sl.i1 && sl.at(i) == kept.tau);
-                const int cnt = __popc(b);
-                if (need > 0 && need <= cnt) {
-                    for (int k = need; k > 1; k--) b &= b - 1;
+            const int need = (int)(kept.ties - before);
+            const int len = sl.wper / 32;
+            int have = 0;
+            sl.run4([&](float x, int) { have += x == kept.tau; });
+            int upto = have;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int who = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+            int left = need - __shfl_sync(0xffffffffu, upto - have, who);
+            for (int e = 0; e < len; e += 32) {
+                const int i = sl.i0 + who * len + e + lane;
+                unsigned b = __ballot_sync(0xffffffffu, e + lane < len && sl.at(i) == kept.tau);
+                if (left <= __popc(b)) {
+                    for (; left > 1; left--) b &= b - 1;
                     if (lane < C)
-                        cl.map_shared_rank(&sh, lane)->icut = sl.first + sl.i0 + 32 * j + __ffs(b) - 1;
+                        cl.map_shared_rank(&sh, lane)->icut = sl.first + sl.i0 + who * len + e + __ffs(b) - 1;
+                    break;
                 }
-                need -= cnt;
+                left -= __popc(b);
             }
         }
         cl.sync();
@@ -778,25 +823,25 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
         __syncthreads();
         if (lane == 0) sh.wsum[warp] = sh.wabove[warp];
         __syncthreads();
-        sa_near(sh, sc, sl, (float)p_lo, (float)(p_hi + 1), [&](float x, int i) {
+        sa_near(sh, sc, sl, sc.units(p_lo), sc.units(p_hi + 1), [&](float x, int i) {
             if (x > tau_k && keeps(x, i)) atomicAdd(&sh.wsum[i / sl.wper], sc.weight(x));
         });
         if (limited && kept.tau <= tau_k)
             sl.each4([&](float x, int i) { return x == tau_k && keeps(x, i); },
-                     [&](const float (&)[4], const int (&)[4], const bool (&in)[4]) {
+                     [&](const float (&)[4], int, const bool (&in)[4]) {
                          atomicAdd(&sh.wsum[warp], (u64)(in[0] + in[1] + in[2] + in[3]) * sc.weight(tau_k));
                      });
         __syncthreads();
         sum = sh.wsum[warp];
     } else {
         sum = 0;
-        sl.each4([&](float x, int i) { return keeps(x, i) && sc.range(x) < (float)SA_BINS; },
-                 [&](const float (&x)[4], const int (&)[4], const bool (&in)[4]) {
-                     u64 w[4];
+        sl.each4([&](float x, int i) { return keeps(x, i) && sc.dist(x) < f_all; },
+                 [&](const float (&x)[4], int, const bool (&in)[4]) {
 #pragma unroll
-                     for (int e = 0; e < 4; e++) w[e] = sc.weight(x[e]);
-#pragma unroll
-                     for (int e = 0; e < 4; e++) sum += in[e] && w[e] >= wmin ? w[e] : 0ull;
+                     for (int e = 0; e < 4; e++) {
+                         const u64 w = sc.weight(x[e]);
+                         if (in[e] && w >= wmin) sum += w;
+                     }
                  });
         sum = sa_warp_sum(sum);
     }
@@ -808,19 +853,13 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
     for (int w = 0; w < warp; w++) before += sh.wsum[w];
     const double goal = (double)u * (double)total;
     if ((double)before <= goal && (double)(before + sum) > goal) {
-        // The token lies in this warp's part: each lane sums `steps` tokens in
-        // a row (read from a place that turns with the lane: no two on one
-        // bank), then the lane that holds it is taken apart.
-        const int len = sl.steps, base = sl.i0 + lane * len;
+        // The token lies in this warp's part: each lane sums a run of tokens, then the run
+        // that holds it is taken apart.
+        const int len = sl.wper / 32;
         u64 part = 0;
-#pragma unroll 4
-        for (int e = 0; e < len; e++) {
-            const int q = e + lane % len, i = base + (q < len ? q : q - len);
-            if (i < sl.i1) {
-                const float x = sl.at(i);
-                if (keeps(x, i)) part += mass_of(x, i);
-            }
-        }
+        sl.run4([&](float x, int i) {
+            if (keeps(x, i)) part += mass_of(x, i);
+        });
         u64 inc = part;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -833,7 +872,7 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per) {
         for (int e0 = 0; e0 < len; e0 += 32) {
             const int i = sl.i0 + who * len + e0 + lane;
             u64 w = 0;
-            if (e0 + lane < len && i < sl.i1) {
+            if (e0 + lane < len) {
                 const float x = sl.at(i);
                 if (keeps(x, i)) w = mass_of(x, i);
             }
@@ -859,7 +898,15 @@ bool sample_rows(cudaStream_t s, const kllm_sample_rows &r, int nz, long long pl
     int C = SA_CL;
     while (C > 1 && r.vocab <= C * 2048) C /= 2;
     const int per = ((r.vocab + C - 1) / C + 3) / 4 * 4;
-    const bool cached = (size_t)per * 4 <= SA_CACHE;
+    const int wper = ((per + SA_WARPS - 1) / SA_WARPS + 127) / 128 * 128;
+    const size_t slice = (size_t)wper * SA_WARPS * 4;
+    const bool cached = slice <= SA_CACHE;
+    // a range's word: a slice's count above the sum of its tokens' positions, q_bits each
+    int pos_bits = 31, q_bits = 0;
+    while ((1ll << (32 - pos_bits)) <= per) pos_bits--;
+    while (((2ll << q_bits) - 1) * per < (1ll << pos_bits) && q_bits < 8) q_bits++;
+    const bool vec = nz == 1 && r.vocab % 4 == 0 && (r.rows == 1 || r.row_stride % 4 == 0) &&
+                     (reinterpret_cast<uintptr_t>(r.logits) & 15) == 0;
     static bool ready[64] = {};
     static std::mutex mu;
     int dev = 0;
@@ -877,7 +924,7 @@ bool sample_rows(cudaStream_t s, const kllm_sample_rows &r, int nz, long long pl
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(r.rows * C));
     cfg.blockDim = dim3(SA_THREADS);
-    cfg.dynamicSmemBytes = cached ? (size_t)per * 4 : 0;
+    cfg.dynamicSmemBytes = cached ? slice : 0;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -885,7 +932,8 @@ bool sample_rows(cudaStream_t s, const kllm_sample_rows &r, int nz, long long pl
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (!KLLM_CUDA(cudaLaunchKernelEx(&cfg, cached ? k_sample<true> : k_sample<false>, r, nz, plane, per))) return false;
+    if (!KLLM_CUDA(cudaLaunchKernelEx(&cfg, cached ? k_sample<true> : k_sample<false>, r, nz, plane, per,
+                                      wper, pos_bits, q_bits, vec))) return false;
     g_launches++;
     return KLLM_CUDA(cudaGetLastError());
 }
