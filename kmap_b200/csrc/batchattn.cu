@@ -15,120 +15,24 @@
 // Scores carry scale * log2(e) * (the key row's scale); a weight carries the
 // value row's scale over the largest scale met so far (a power of two), so
 // p's fp16 terms stay in range whatever the scales are.
-#include <cuda_fp16.h>
-
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
+#include "batchattn.cuh"
+#include "batchattn_tc.cuh"
 #include "rows.cuh"
 #include "serve.cuh"
 
 namespace kllm {
 namespace {
 
-constexpr int BA_THREADS = 128, BA_WARPS = 4, BA_ROWS = 8;
-
-struct BaSide {
-    const void *k, *v;
-    const float *ks, *vs;
-    long long seq_stride, scale_stride;
-    int max_pos;      // rows of a (sequence, head)
-    int parts, chunk; // ranges of `chunk` positions
-};
-
-struct BaArgs {
-    BaSide pre, own;
-    const float *q;
-    long long q_stride;
-    const int *own_len;
-    int n_seq, nh, nkv, groups, prefix_len, own_cap;
-    int tiles_pre, tiles_own;   // 8-row tiles: of n_seq * groups, of groups
-    float qk;                   // scale * log2(e)
-    float *part_ml, *part_o;    // [n_seq * nh][parts][2], [n_seq * nh][parts][HD]
-};
-
-__device__ __forceinline__ int ba_len(const int *own_len, int cap, int i) {
-    return min(own_len ? own_len[i] : 0, cap);
-}
-
-__device__ __forceinline__ uint32_t ba_prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    return __byte_perm(a, b, sel);
-}
-
-__device__ __forceinline__ uint32_t ba_h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// hi and lo fp16 terms of a pair
-__device__ __forceinline__ void ba_split(float a, float b, uint32_t *hi, uint32_t *lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    *hi = *reinterpret_cast<const uint32_t *>(&h);
-    *lo = ba_h2(a - f.x, b - f.y);
-}
-
-// the two codes of each half of a word, (c0, c1) or (c2, c3), as fp16
-template <int FMT, int HALF>
-__device__ __forceinline__ uint32_t ba_codes(uint32_t w) {
-    if constexpr (FMT == KLLM_KV_I8) {
-        // w holds code + 128: the fp16 with bits 0x6400 + u is 1024 + u
-        const uint32_t u = ba_prmt(w, 0x64646464u, HALF ? 0x4342 : 0x4140);
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&u),
-                                  __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        uint32_t d;
-        const uint16_t c = (uint16_t)(HALF ? w >> 16 : w & 0xffffu);
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(c));
-        return d;
-    }
-}
-
-__device__ __forceinline__ void ba_mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                           uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void ba_mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                            uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // tf32 terms: the upper 11 significand bits, and the rest (13 bits, of which
 // the product takes 11)
 __device__ __forceinline__ void ba_split32(float x, uint32_t *hi, uint32_t *lo) {
     *hi = __float_as_uint(x) & 0xffffe000u;
     *lo = __float_as_uint(x - __uint_as_float(*hi));
-}
-
-// the power of two above |x|'s, within the range whose inverse stays normal
-__device__ __forceinline__ float ba_pow2(float x) {
-    const float c = fminf(fmaxf(x, 0x1p-110f), 0x1p110f);
-    return __uint_as_float((__float_as_uint(c) & 0x7f800000u) + 0x00800000u);
-}
-
-template <int BYTES>
-__device__ __forceinline__ void ba_ld(uint32_t *w, const void *p, bool in) {
-    if constexpr (BYTES >= 16) {
-#pragma unroll
-        for (int i = 0; i < BYTES / 16; i++) {
-            uint4 t = make_uint4(0, 0, 0, 0);
-            if (in) t = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-            w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
-        }
-    } else if constexpr (BYTES == 8) {
-        uint2 t = make_uint2(0, 0);
-        if (in) t = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = t.x, w[1] = t.y;
-    } else {
-        w[0] = in ? __ldg(reinterpret_cast<const uint32_t *>(p)) : 0u;
-    }
 }
 
 // One part of eight query rows of one kv head.  grid: the prefix's
@@ -144,7 +48,7 @@ k_ba_part(const BaArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
     // which item
     int b = blockIdx.x, kvh, seq = 0, tile, part, len;
-    const int n_pre = a.nkv * a.tiles_pre * a.pre.parts;
+    const int n_pre = a.wide ? 0 : a.nkv * a.tiles_pre * a.pre.parts;
     const bool pre = b < n_pre;
     if (pre) {
         part = b % a.pre.parts, b /= a.pre.parts;
@@ -440,6 +344,7 @@ k_ba_merge(const float *__restrict__ part_ml, const float *__restrict__ part_o, 
 struct BaCut {
     int tiles_pre = 0, tiles_own = 0, own_cap = 0;
     int parts_pre = 0, chunk_pre = 0, parts_own = 0, chunk_own = 0;
+    bool wide = false;      // the prefix by 128-row tiles
     size_t rows = 0, bytes = 0;
 };
 
@@ -458,8 +363,18 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     x.own_cap = a.own ? std::min(a.max_len, a.own->max_pos) : 0;
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
-        x.tiles_pre = (int)(((long long)a.n_seq * groups + BA_ROWS - 1) / BA_ROWS);
-        ba_split_range((long long)c->n_kv * x.tiles_pre, pre, &x.parts_pre, &x.chunk_pre);
+        const long long rows = (long long)a.n_seq * groups;
+        x.wide = rows >= 32 && pre >= 256;
+        x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : BA_ROWS) - 1) / (x.wide ? BT_ROWS : BA_ROWS));
+        const long long items = (long long)c->n_kv * x.tiles_pre;
+        if (x.wide) {
+            // one block an SM: as many parts as fill them once
+            const int n = (int)std::min<long long>(std::max<long long>(148 / items, 1), (pre + 127) / 128);
+            x.chunk_pre = ((pre + n - 1) / n + 127) / 128 * 128;
+            x.parts_pre = (pre + x.chunk_pre - 1) / x.chunk_pre;
+        } else {
+            ba_split_range(items, pre, &x.parts_pre, &x.chunk_pre);
+        }
     }
     if (x.own_cap > 0) {
         x.tiles_own = (groups + BA_ROWS - 1) / BA_ROWS;
@@ -505,6 +420,20 @@ bool ba_ok(const char *who, const kllm_batch_attn *a) {
     return true;
 }
 
+// A kernel's shared-memory limit, raised once per device.
+bool ba_prepare(const void *kernel, size_t smem) {
+    static std::mutex mu;
+    static std::set<std::pair<int, const void *>> done;
+    int dev = 0;
+    if (!KLLM_CUDA(cudaGetDevice(&dev))) return false;
+    std::lock_guard<std::mutex> lk(mu);
+    if (done.count({dev, kernel})) return true;
+    if (!KLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
+        return false;
+    done.insert({dev, kernel});
+    return true;
+}
+
 template <int HD, int FMT>
 bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int terms, void *terms_out) {
     const kllm_kv_cache *c = a.prefix ? a.prefix : a.own;
@@ -534,11 +463,18 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     const size_t parts = x.parts_pre + x.parts_own;
     k.part_o = reinterpret_cast<float *>(static_cast<char *>(a.workspace) +
                                          (x.rows * parts * 2 * 4 + 15) / 16 * 16);
-    const long long blocks = (long long)k.nkv * x.tiles_pre * x.parts_pre +
+    k.wide = x.wide;
+    const long long pre_blocks = (long long)k.nkv * x.tiles_pre * x.parts_pre;
+    const long long blocks = (x.wide ? 0 : pre_blocks) +
                              (long long)a.n_seq * k.nkv * x.tiles_own * x.parts_own;
-    if (blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
+    if (pre_blocks > 0x7fffffffll || blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
         set_error("kllm_batch_attention: %lld blocks", blocks);
         return false;
+    }
+    if (x.wide) {
+        if (!ba_prepare(reinterpret_cast<const void *>(k_ba_prefix<HD, FMT>), bt_smem<HD, FMT>())) return false;
+        k_ba_prefix<HD, FMT><<<(unsigned)pre_blocks, BT_THREADS, bt_smem<HD, FMT>(), s>>>(k);
+        g_launches++;
     }
     if (blocks) {
         k_ba_part<HD, FMT><<<(unsigned)blocks, BA_THREADS, 0, s>>>(k);

@@ -1,0 +1,115 @@
+// batchattn.cuh -- what the kernels of the shared-prefix attention have in
+// common (batchattn.cu: a few rows at a time; batchattn_tc.cuh: 128).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace kllm {
+namespace {
+
+constexpr int BA_THREADS = 128, BA_WARPS = 4, BA_ROWS = 8;
+
+struct BaSide {
+    const void *k, *v;
+    const float *ks, *vs;
+    long long seq_stride, scale_stride;
+    int max_pos;      // rows of a (sequence, head)
+    int parts, chunk; // ranges of `chunk` positions
+};
+
+struct BaArgs {
+    BaSide pre, own;
+    const float *q;
+    long long q_stride;
+    const int *own_len;
+    int n_seq, nh, nkv, groups, prefix_len, own_cap;
+    int tiles_pre, tiles_own;   // row tiles: of n_seq * groups, of groups
+    bool wide;                  // the prefix runs by itself, in tiles of 128 rows (batchattn_tc.cuh)
+    float qk;                   // scale * log2(e)
+    float *part_ml, *part_o;    // [n_seq * nh][parts][2], [n_seq * nh][parts][HD]
+};
+
+__device__ __forceinline__ int ba_len(const int *own_len, int cap, int i) {
+    return min(own_len ? own_len[i] : 0, cap);
+}
+
+__device__ __forceinline__ uint32_t ba_prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    return __byte_perm(a, b, sel);
+}
+
+__device__ __forceinline__ uint32_t ba_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// hi and lo fp16 terms of a pair
+__device__ __forceinline__ void ba_split(float a, float b, uint32_t *hi, uint32_t *lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    *hi = *reinterpret_cast<const uint32_t *>(&h);
+    *lo = ba_h2(a - f.x, b - f.y);
+}
+
+// the two codes of each half of a word, (c0, c1) or (c2, c3), as fp16
+template <int FMT, int HALF>
+__device__ __forceinline__ uint32_t ba_codes(uint32_t w) {
+    if constexpr (FMT == KLLM_KV_I8) {
+        // w holds code + 128: the fp16 with bits 0x6400 + u is 1024 + u
+        const uint32_t u = ba_prmt(w, 0x64646464u, HALF ? 0x4342 : 0x4140);
+        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&u),
+                                  __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        uint32_t d;
+        const uint16_t c = (uint16_t)(HALF ? w >> 16 : w & 0xffffu);
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(c));
+        return d;
+    }
+}
+
+__device__ __forceinline__ void ba_mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                           uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ba_mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                            uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the power of two above |x|'s, within the range whose inverse stays normal
+__device__ __forceinline__ float ba_pow2(float x) {
+    const float c = fminf(fmaxf(x, 0x1p-110f), 0x1p110f);
+    return __uint_as_float((__float_as_uint(c) & 0x7f800000u) + 0x00800000u);
+}
+
+template <int BYTES>
+__device__ __forceinline__ void ba_ld(uint32_t *w, const void *p, bool in) {
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; i++) {
+            uint4 t = make_uint4(0, 0, 0, 0);
+            if (in) t = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+        }
+    } else if constexpr (BYTES == 8) {
+        uint2 t = make_uint2(0, 0);
+        if (in) t = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = t.x, w[1] = t.y;
+    } else {
+        w[0] = in ? __ldg(reinterpret_cast<const uint32_t *>(p)) : 0u;
+    }
+}
+
+}  // namespace
+}  // namespace kllm
