@@ -473,7 +473,7 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     }
     if (x.wide) {
         if (!ba_prepare(reinterpret_cast<const void *>(k_ba_prefix<HD, FMT>), bt_smem<HD, FMT>())) return false;
-        k_ba_prefix<HD, FMT><<<(unsigned)pre_blocks, BT_THREADS, bt_smem<HD, FMT>(), s>>>(k);
+        k_ba_prefix<HD, FMT><<<(unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, bt_smem<HD, FMT>(), s>>>(k);
         g_launches++;
     }
     if (blocks) {

@@ -93,6 +93,36 @@ __device__ __forceinline__ float ba_pow2(float x) {
     return __uint_as_float((__float_as_uint(c) & 0x7f800000u) + 0x00800000u);
 }
 
+// Loads that stay where they are written (ahead of their use, which the
+// compiler would rather load at), zeros where `in` is false.
+__device__ __forceinline__ void ba_fetch(uint32_t (&w)[4], const void *p, bool in) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %5, 0;\n\t"
+        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
+        : "l"(p), "r"((uint32_t)in));
+}
+__device__ __forceinline__ void ba_fetch(uint32_t (&w)[2], const void *p, bool in) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+        "@p ld.global.nc.v2.u32 {%0, %1}, [%2];\n\t}"
+        : "=&r"(w[0]), "=&r"(w[1])
+        : "l"(p), "r"((uint32_t)in));
+}
+__device__ __forceinline__ void ba_fetch(uint32_t (&w)[1], const void *p, bool in) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "mov.u32 %0, 0;\n\t"
+        "@p ld.global.nc.u32 %0, [%1];\n\t}"
+        : "=&r"(w[0])
+        : "l"(p), "r"((uint32_t)in));
+}
+
 template <int BYTES>
 __device__ __forceinline__ void ba_ld(uint32_t *w, const void *p, bool in) {
     if constexpr (BYTES >= 16) {

@@ -13,13 +13,16 @@
 // registers, which is also where the running maximum's corrections and the
 // tile's value scale come in.
 //
-// 21 warps: 4 softmax (a row per thread), 8 that keep O (a row and half the
-// columns per thread), 8 that bring keys and values from global memory to
-// fp16 operands in shared memory (next tile's loads in flight in registers),
-// one that issues the products.  Keys, values, S/P and O have two buffers
-// each; S of the next tile is issued before P.V of this one, so that the
-// tensor cores work while the softmax does.  Every wait is bounded; one that
-// gives up leaves NaN in the part's sums.
+// Warps: two groups of four that take the tiles' softmax in turn (a row per
+// thread) and each keep half of O's columns; four (fp32: eight) that bring
+// keys and values from global memory to fp16 operands in shared memory (the
+// next tile's loads in flight in registers); one that issues the products.
+// A tile's weights are relative to the tile's own maximum, so that the two
+// groups need nothing of one another; the running maximum is applied where O
+// is added up.  Keys, values, S/P and O have two buffers each; S of the next
+// tile is issued before P.V of this one, so that the tensor cores work while
+// the softmax does.  Every wait is bounded; one that gives up leaves NaN in
+// the part's sums.
 //
 // Bound: products.  With two terms a tile of 128 positions of 8 bits takes
 // 16.8 MFLOP, 1.5 us at the tensor cores' rate, where its bytes take 0.8 us
@@ -33,13 +36,14 @@
 namespace kllm {
 namespace {
 
-constexpr int BT_SOFT = 4, BT_OUT = 8, BT_FEED = 8;              // warps
-constexpr int BT_THREADS = 32 * (BT_SOFT + BT_OUT + BT_FEED + 1);
+constexpr int BT_SOFT = 8;                                       // warps
 constexpr int BT_ROWS = 128, BT_RING = 8;
 
 template <int HD, int FMT>
 struct BtGeom {
     static constexpr bool F32 = FMT == KLLM_KV_F32;
+    static constexpr int FEED = F32 ? 8 : 4;                     // warps
+    static constexpr int THREADS = 32 * (BT_SOFT + FEED + 1);
     static constexpr int BN = F32 ? 64 : 128;                    // positions of a tile
     static constexpr int KT = F32 ? 2 : 1;                       // terms of a key or value
     static constexpr int KB = HD > 64 ? HD / 64 : 1;             // 64-dim blocks of Q and K
@@ -55,13 +59,13 @@ struct BtGeom {
 
 struct BtShared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
-    uint64_t sc_full[BT_RING];
+    uint64_t sc_full[BT_RING], m_full[BT_RING];
     uint32_t tmem;
     int dead;
-    float wmax[2][BT_FEED];
+    float wmax[2][8];
     float vscale[BT_RING];               // what O of the tile is in units of
     float rowfac[BT_ROWS];
-    float corr[BT_RING][BT_ROWS];
+    float mt[BT_RING][BT_ROWS], lt[BT_RING][BT_ROWS];     // a tile's maximum and sum of weights, per row
     alignas(16) float ks[BT_RING][128], pv[BT_RING][128];
 };
 
@@ -90,24 +94,112 @@ __device__ __forceinline__ float bt_ex2(float x) {
     return y;
 }
 
+// Two columns' scores times their keys' scales, and the maximum with them.
+__device__ __forceinline__ float bt_max16(const uint32_t (&x)[16], const float4 *ks, float mx, bool cut,
+                                          int n) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float4 k = ks[e];
+        float2 a = __fmul2_rn(make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])),
+                              make_float2(k.x, k.y));
+        float2 b = __fmul2_rn(make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])),
+                              make_float2(k.z, k.w));
+        if (cut) {
+            if (4 * e >= n) a.x = -INFINITY;
+            if (4 * e + 1 >= n) a.y = -INFINITY;
+            if (4 * e + 2 >= n) b.x = -INFINITY;
+            if (4 * e + 3 >= n) b.y = -INFINITY;
+        }
+        mx = fmaxf(mx, fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y)));
+    }
+    return mx;
+}
+
+// 16 columns' weights p = 2^(score - ref), their sum, and the fp16 terms of
+// p times their values' scales.
+__device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4 *ks, const float4 *pv,
+                                           float fac, float ref, float2 sum, bool cut, int n,
+                                           uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+    const float2 f = make_float2(fac, fac), r = make_float2(-ref, -ref);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float2 k = reinterpret_cast<const float2 *>(ks)[e], v = reinterpret_cast<const float2 *>(pv)[e];
+        const float2 y = __ffma2_rn(
+            __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), k), f, r);
+        float2 p = make_float2(bt_ex2(y.x), bt_ex2(y.y));
+        if (cut) {
+            if (2 * e >= n) p.x = 0.f;
+            if (2 * e + 1 >= n) p.y = 0.f;
+        }
+        sum = __fadd2_rn(sum, p);
+        p = __fmul2_rn(p, v);
+        const __half2 h = __float22half2_rn(p);
+        const float2 g = __half22float2(h);
+        const __half2 l = __float22half2_rn(__fadd2_rn(p, make_float2(-g.x, -g.y)));
+        hi[e] = *reinterpret_cast<const uint32_t *>(&h);
+        lo[e] = *reinterpret_cast<const uint32_t *>(&l);
+    }
+    return sum;
+}
+
+// The softmax of one row of a tile: scores in columns at.., their maximum (in
+// log2, *m) and the weights' sum relative to it; the weights' two terms take
+// the columns of their scores, 8 columns each for 16 positions.  While 16
+// columns are worked on the next 16 are on their way.
+template <int BN, bool CUT>
+__device__ __forceinline__ void bt_soft(uint32_t at, const float4 *ks, const float4 *pv, float fac, int n,
+                                        float *m, float *sum) {
+    uint32_t s0[16], s1[16], hi[8], lo[8];
+    float mx = -INFINITY;
+    tmem_ld16(at, s0);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+        tmem_wait_ld16(s0);
+        tmem_ld16(at + c + 16, s1);
+        mx = bt_max16(s0, ks + c / 4, mx, CUT, n - c);
+        tmem_wait_ld16(s1);
+        tmem_ld16(at + (c + 32) % BN, s0);       // behind the last, the first again
+        mx = bt_max16(s1, ks + c / 4 + 4, mx, CUT, n - c - 16);
+    }
+    const float top = mx * fac, ref = top == -INFINITY ? 0.f : top;
+    float2 t = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+        tmem_wait_ld16(s0);
+        tmem_ld16(at + c + 16, s1);
+        t = bt_exp16(s0, ks + c / 4, pv + c / 4, fac, ref, t, CUT, n - c, hi, lo);
+        tmem_st8(at + c, hi);
+        tmem_st8(at + c + 8, lo);
+        tmem_wait_ld16(s1);
+        if (c + 32 < BN) tmem_ld16(at + c + 32, s0);
+        t = bt_exp16(s1, ks + c / 4 + 4, pv + c / 4 + 4, fac, ref, t, CUT, n - c - 16, hi, lo);
+        tmem_st8(at + c + 16, hi);
+        tmem_st8(at + c + 24, lo);
+    }
+    *m = top;
+    *sum = t.x + t.y;
+}
+
 // 16 bytes at row r, 16-byte chunk c of a 128-byte-swizzled tile
 __device__ __forceinline__ uint8_t *bt_at(uint8_t *tile, int r, int c) {
     return tile + r * 128 + ((c ^ (r & 7)) << 4);
 }
 
 // the largest |x| of the feeding warps' threads (all call it)
+template <int FEED>
 __device__ __forceinline__ float bt_feed_max(float m, float *wmax) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int w = (threadIdx.x >> 5) - BT_SOFT - BT_OUT;
+    const int w = (threadIdx.x >> 5) - BT_SOFT;
     if ((threadIdx.x & 31) == 0) wmax[w] = m;
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * BT_FEED) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * FEED) : "memory");
 #pragma unroll
-    for (int i = 0; i < BT_FEED; i++) m = fmaxf(m, wmax[i]);
+    for (int i = 0; i < FEED; i++) m = fmaxf(m, wmax[i]);
     return m;
 }
 
 // whether all feeding threads say yes: they leave their loop together
+template <int FEED>
 __device__ __forceinline__ bool bt_feed_all(bool yes) {
     uint32_t all;
     asm volatile(
@@ -116,71 +208,67 @@ __device__ __forceinline__ bool bt_feed_all(bool yes) {
         "barrier.cta.red.and.pred p, 2, %2, q;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(all)
-        : "r"((uint32_t)yes), "n"(32 * BT_FEED)
+        : "r"((uint32_t)yes), "n"(32 * FEED)
         : "memory");
     return all != 0;
 }
 
-// What a feeding thread holds of a tile of 8-bit codes: K, 16 codes (16 bytes)
-// of each of BN / rows-a-pass rows; V, DV dims of 8 positions in a row.
+// What a feeding thread (of 128) holds of a tile of 8-bit codes: K, 16 codes
+// (16 bytes) of every RPP-th row; V, DV dims of 8 positions in a row.
 template <int HD>
 struct BtFeed8 {
-    static constexpr int LPR = HD / 16, RPP = 32 * BT_FEED / LPR, NK = (128 + RPP - 1) / RPP;
-    static constexpr int DV = HD / 16 < 4 ? 4 : HD / 16, ITEMS = 16 * (HD / DV);
-    uint4 k[NK];
-    uint32_t v[8][DV / 4];
+    static constexpr int LPR = HD / 16, RPP = 128 / LPR, NK = 128 / RPP, DV = HD / 8;
+    uint32_t k[NK][4], v[8][DV / 4];
     float ks, vs;
 
     __device__ __forceinline__ void load_k(const uint8_t *kb, const float *ksc, const float *vsc, int j0,
                                            int n) {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
 #pragma unroll
         for (int p = 0; p < NK; p++) {
             const int r = p * RPP + t / LPR;
-            k[p] = make_uint4(0, 0, 0, 0);
-            if (r < n) k[p] = __ldg(reinterpret_cast<const uint4 *>(kb + (long long)(j0 + r) * HD) + t % LPR);
+            ba_fetch(k[p], kb + (long long)(j0 + r) * HD + 16 * (t % LPR), r < n);
         }
-        ks = vs = 0.f;
-        if (t < n) ks = __ldg(ksc + j0 + t), vs = __ldg(vsc + j0 + t);
+        uint32_t x[1], y[1];
+        ba_fetch(x, ksc + j0 + t, t < n);
+        ba_fetch(y, vsc + j0 + t, t < n);
+        ks = __uint_as_float(x[0]), vs = __uint_as_float(y[0]);
     }
     __device__ __forceinline__ void load_v(const uint8_t *vb, int j0, int n) {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
-        if (t >= ITEMS) return;
+        const int t = threadIdx.x - 32 * BT_SOFT;
         const int pg = (t & 7) | ((t >> 5) & 1) << 3, dg = ((t >> 3) & 3) | (t >> 6) << 2;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int r = pg * 8 + j;
-            ba_ld<DV>(v[j], vb + (long long)(j0 + r) * HD + dg * DV, r < n);
+            ba_fetch(v[j], vb + (long long)(j0 + r) * HD + dg * DV, r < n);
         }
     }
     template <int FMT>
     __device__ __forceinline__ void store_k(uint8_t *tile) const {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
 #pragma unroll
         for (int p = 0; p < NK; p++) {
             const int r = p * RPP + t / LPR, i = t % LPR, blk = i >> 2, c = 2 * (i & 3);
-            if (RPP * NK > 128 && r >= 128) continue;
-            const uint32_t w[4] = {k[p].x, k[p].y, k[p].z, k[p].w};
-            uint4 o[2];
-            uint32_t *u = reinterpret_cast<uint32_t *>(o);
+            uint32_t u[8];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t x = FMT == KLLM_KV_I8 ? w[e] ^ 0x80808080u : w[e];
+                const uint32_t x = FMT == KLLM_KV_I8 ? k[p][e] ^ 0x80808080u : k[p][e];
                 u[2 * e] = ba_codes<FMT, 0>(x);
                 u[2 * e + 1] = ba_codes<FMT, 1>(x);
             }
             // the lanes of the second block of dims store their odd chunk first: a row's eight
             // lanes then touch eight different banks' worth
             uint8_t *b = tile + blk * (128 * 128);
-            const int s = blk & 1;
-            *reinterpret_cast<uint4 *>(bt_at(b, r, c + s)) = o[s];
-            *reinterpret_cast<uint4 *>(bt_at(b, r, c + 1 - s)) = o[1 - s];
+            const bool s = blk & 1;
+            *reinterpret_cast<uint4 *>(bt_at(b, r, c + s)) =
+                make_uint4(s ? u[4] : u[0], s ? u[5] : u[1], s ? u[6] : u[2], s ? u[7] : u[3]);
+            *reinterpret_cast<uint4 *>(bt_at(b, r, c + 1 - s)) =
+                make_uint4(s ? u[0] : u[4], s ? u[1] : u[5], s ? u[2] : u[6], s ? u[3] : u[7]);
         }
     }
     template <int FMT>
     __device__ __forceinline__ void store_v(uint8_t *tile) const {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
-        if (t >= ITEMS) return;
+        const int t = threadIdx.x - 32 * BT_SOFT;
         const int pg = (t & 7) | ((t >> 5) & 1) << 3, dg = ((t >> 3) & 3) | (t >> 6) << 2;
         uint8_t *b = tile + (pg >> 3) * (HD * 128);
 #pragma unroll
@@ -208,29 +296,31 @@ struct BtFeed8 {
 // dims of 8 positions in a row.
 template <int HD>
 struct BtFeed32 {
-    static constexpr int LPR = HD / 4, RPP = 32 * BT_FEED / LPR, NK = (64 + RPP - 1) / RPP;
+    static constexpr int LPR = HD / 4, RPP = 256 / LPR, NK = (64 + RPP - 1) / RPP;
     static constexpr int ITEMS = 8 * (HD / 4);
     float4 k[NK], v[8];
 
     __device__ __forceinline__ void load_k(const uint8_t *kb, int j0, int n) {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
 #pragma unroll
         for (int p = 0; p < NK; p++) {
             const int r = p * RPP + t / LPR;
-            k[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < n)
-                k[p] = __ldg(reinterpret_cast<const float4 *>(kb + (long long)(j0 + r) * HD * 4) + t % LPR);
+            uint32_t w[4];
+            ba_fetch(w, kb + ((long long)(j0 + r) * HD + 4 * (t % LPR)) * 4, r < n);
+            k[p] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+                               __uint_as_float(w[3]));
         }
     }
     __device__ __forceinline__ void load_v(const uint8_t *vb, int j0, int n) {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
         const int pg = t & 7, dg = t >> 3;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int r = pg * 8 + j;
-            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (t < ITEMS && r < n)
-                v[j] = __ldg(reinterpret_cast<const float4 *>(vb + (long long)(j0 + r) * HD * 4) + dg);
+            uint32_t w[4];
+            ba_fetch(w, vb + ((long long)(j0 + r) * HD + 4 * dg) * 4, t < ITEMS && r < n);
+            v[j] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+                               __uint_as_float(w[3]));
         }
     }
     static __device__ __forceinline__ float most(float4 x) {
@@ -249,7 +339,7 @@ struct BtFeed32 {
         return m;
     }
     __device__ __forceinline__ void store_k(uint8_t *tile, int term, float f) const {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
 #pragma unroll
         for (int p = 0; p < NK; p++) {
             const int r = p * RPP + t / LPR, i = t % LPR, blk = i >> 4;
@@ -263,7 +353,7 @@ struct BtFeed32 {
         }
     }
     __device__ __forceinline__ void store_v(uint8_t *tile, int term, float f) const {
-        const int t = threadIdx.x - 32 * (BT_SOFT + BT_OUT);
+        const int t = threadIdx.x - 32 * BT_SOFT;
         if (t >= ITEMS) return;
         const int pg = t & 7, dg = t >> 3;
 #pragma unroll
@@ -283,7 +373,7 @@ struct BtFeed32 {
 
 // grid: (kv head, tile of 128 rows, part) of the prefix
 template <int HD, int FMT>
-__global__ void __launch_bounds__(BT_THREADS, 1)
+__global__ void __launch_bounds__((BtGeom<HD, FMT>::THREADS), 1)
 k_ba_prefix(const BaArgs a) {
     using G = BtGeom<HD, FMT>;
     constexpr bool F32 = G::F32;
@@ -301,20 +391,23 @@ k_ba_prefix(const BaArgs a) {
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.k_full[i], 32 * BT_FEED);
+            mbar_init(&sh.k_full[i], 32 * G::FEED);
             mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 32 * BT_FEED);
+            mbar_init(&sh.v_full[i], 32 * G::FEED);
             mbar_init(&sh.v_empty[i], 1);
             mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], 32 * BT_SOFT);
+            mbar_init(&sh.p_full[i], 128);
             mbar_init(&sh.o_full[i], 1);
-            mbar_init(&sh.o_empty[i], 32 * BT_OUT);
+            mbar_init(&sh.o_empty[i], 32 * BT_SOFT);
         }
-        for (int i = 0; i < BT_RING; i++) mbar_init(&sh.sc_full[i], 32 * BT_FEED);
+        for (int i = 0; i < BT_RING; i++) {
+            mbar_init(&sh.sc_full[i], 32 * G::FEED);
+            mbar_init(&sh.m_full[i], 128);
+        }
         sh.dead = 0;
         mbar_fence_init();
     }
-    if (warp == BT_SOFT + BT_OUT + BT_FEED) {
+    if (warp == BT_SOFT + G::FEED) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&sh.tmem)), "r"(G::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -322,7 +415,7 @@ k_ba_prefix(const BaArgs a) {
     // The queries: LPR lanes a row, four dims each.  q times scale * log2(e), brought to
     // [2^13, 2^14) by a power of two, in two fp16 terms.
     {
-        constexpr int LPR = HD / 4, RPW = 32 / LPR, WARPS = BT_THREADS / 32;
+        constexpr int LPR = HD / 4, RPW = 32 / LPR, WARPS = G::THREADS / 32;
 #pragma unroll 2
         for (int r0 = warp * RPW; r0 < BT_ROWS; r0 += WARPS * RPW) {
             const int r = r0 + lane / LPR, i = lane % LPR, R = tile * BT_ROWS + r;
@@ -363,115 +456,78 @@ k_ba_prefix(const BaArgs a) {
     };
 
     if (warp < BT_SOFT) {
-        // ------------------------------------------------------- softmax --
-        const int r = 32 * warp + lane;
-        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        // --------------------------------------------- softmax and output --
+        const int group = warp >> 2, r = 32 * (warp & 3) + lane;
+        constexpr int NC = HD / 2;                 // columns of O of this thread
+        const int c0 = group * NC;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const float fac = sh.rowfac[r];
-        float m_run = -INFINITY, l_run = 0.f;
-        bool ok = true;
-        for (int t = 0; t < nt; t++) {
-            const int ring = t & (BT_RING - 1), n = min(G::BN, p1 - p0 - t * G::BN);
-            ok = __all_sync(0xffffffffu, bt_wait(&sh.sc_full[ring], (t / BT_RING) & 1, &sh.dead) &&
-                                             bt_wait(&sh.s_full[t & 1], (t / 2) & 1, &sh.dead));
-            if (!ok) break;
-            tc_fence_after();
-            const float4 *ks = reinterpret_cast<const float4 *>(sh.ks[ring]);
-            const float4 *pv = reinterpret_cast<const float4 *>(sh.pv[ring]);
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < G::BN / 32; c++) {
-                float s[32];
-                tmem_ld32(s_cols(t) + lanes + 32 * c, s);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float4 k = ks[8 * c + e];
-                    s[4 * e] *= k.x, s[4 * e + 1] *= k.y, s[4 * e + 2] *= k.z, s[4 * e + 3] *= k.w;
-                }
-                if (32 * c + 32 > n) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (32 * c + e >= n) s[e] = -INFINITY;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e++) mx = fmaxf(mx, s[e]);
-            }
-            const float m_new = fmaxf(m_run, mx * fac);
-            const float corr = m_run == -INFINITY ? 0.f : bt_ex2(m_run - m_new);
-            const float ref = m_new == -INFINITY ? 0.f : m_new;
-            m_run = m_new;
-            sh.corr[ring][r] = corr;
-            float sum = 0.f;
-            // 16 positions at a time: their two terms take the columns of their scores, 8 each
-#pragma unroll 1
-            for (int c = 0; c < G::BN / 16; c++) {
-                float s[16];
-                tmem_ld16(s_cols(t) + lanes + 16 * c, s);
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float4 k = ks[4 * c + e], v = pv[4 * c + e];
-                    float p[4] = {bt_ex2(fmaf(s[4 * e] * k.x, fac, -ref)), bt_ex2(fmaf(s[4 * e + 1] * k.y, fac, -ref)),
-                                  bt_ex2(fmaf(s[4 * e + 2] * k.z, fac, -ref)),
-                                  bt_ex2(fmaf(s[4 * e + 3] * k.w, fac, -ref))};
-                    if (16 * c + 16 > n) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (16 * c + 4 * e + i >= n) p[i] = 0.f;
-                    }
-                    sum += (p[0] + p[1]) + (p[2] + p[3]);
-                    ba_split(p[0] * v.x, p[1] * v.y, &hi[2 * e], &lo[2 * e]);
-                    ba_split(p[2] * v.z, p[3] * v.w, &hi[2 * e + 1], &lo[2 * e + 1]);
-                }
-                tmem_st8(s_cols(t) + lanes + 16 * c, hi);
-                tmem_st8(s_cols(t) + lanes + 16 * c + 8, lo);
-            }
-            tmem_wait_st();
-            l_run = l_run * corr + sum;
-            tc_fence_before();
-            mbar_arrive(&sh.p_full[t & 1]);
-        }
-        if (tile * BT_ROWS + r < n_rows) {
-            const long long o = 2 * part_of(r);
-            a.part_ml[o] = ok ? m_run : __uint_as_float(0x7fffffffu);
-            a.part_ml[o + 1] = ok ? l_run : __uint_as_float(0x7fffffffu);
-        }
-    } else if (warp < BT_SOFT + BT_OUT) {
-        // -------------------------------------------------------- output --
-        const int w = warp - BT_SOFT, r = 32 * (w & 3) + lane;
-        constexpr int NC = HD / 2;                 // columns of this thread
-        const int c0 = (w >> 2) * NC;
-        const uint32_t lanes = (uint32_t)(32 * (w & 3)) << 16;
-        float acc[NC];
+        float m_run = -INFINITY, l_run = 0.f, acc[NC];
 #pragma unroll
         for (int e = 0; e < NC; e++) acc[e] = 0.f;
         bool ok = true;
-        for (int t = 0; t < nt; t++) {
-            const int ring = t & (BT_RING - 1);
-            ok = __all_sync(0xffffffffu, bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead));
-            if (!ok) break;
+        // the weights of tile t
+        auto soft = [&](int t) {
+            const int ring = t & (BT_RING - 1), n = min(G::BN, p1 - p0 - t * G::BN);
+            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.sc_full[ring], (t / BT_RING) & 1, &sh.dead) &&
+                                             bt_wait(&sh.s_full[t & 1], (t / 2) & 1, &sh.dead));
+            if (!ok) return;
             tc_fence_after();
-            const float corr = sh.corr[ring][r], vs = sh.vscale[ring];
+            const float4 *ks = reinterpret_cast<const float4 *>(sh.ks[ring]);
+            const float4 *pv = reinterpret_cast<const float4 *>(sh.pv[ring]);
+            float m, sum;
+            if (n == G::BN) bt_soft<G::BN, false>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
+            else bt_soft<G::BN, true>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
+            sh.mt[ring][r] = m;
+            sh.lt[ring][r] = sum;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh.p_full[t & 1]);
+            mbar_arrive(&sh.m_full[ring]);
+        };
+        // tile t's output to the registers
+        auto add = [&](int t) {
+            const int ring = t & (BT_RING - 1);
+            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead) &&
+                                             bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead));
+            if (!ok) return;
+            tc_fence_after();
+            const float m = sh.mt[ring][r], m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
+            const float corr = bt_ex2(m_run - ref), w = bt_ex2(m - ref), f = w * sh.vscale[ring];
+            l_run = l_run * corr + sh.lt[ring][r] * w;
+            m_run = m_new;
 #pragma unroll
             for (int c = 0; c < NC / 16; c++) {
-                float v[16];
+                uint32_t v[16];
                 tmem_ld16(o_cols(t) + lanes + c0 + 16 * c, v);
+                tmem_wait_ld16(v);
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[16 * c + e] = fmaf(v[e], vs, acc[16 * c + e] * corr);
+                for (int e = 0; e < 16; e++)
+                    acc[16 * c + e] = fmaf(__uint_as_float(v[e]), f, acc[16 * c + e] * corr);
             }
             tc_fence_before();
             mbar_arrive(&sh.o_empty[t & 1]);
+        };
+        for (int t = group; t < nt + 2; t += 2) {
+            if (t < nt && ok) soft(t);
+            if (t >= 2 && ok) add(t - 2);
+            if (t >= 1 && t - 1 < nt && ok) add(t - 1);
         }
         if (tile * BT_ROWS + r < n_rows) {
-            float4 *o = reinterpret_cast<float4 *>(a.part_o + part_of(r) * HD + c0);
             const float nan = __uint_as_float(0x7fffffffu);
+            float4 *o = reinterpret_cast<float4 *>(a.part_o + part_of(r) * HD + c0);
 #pragma unroll
             for (int e = 0; e < NC / 4; e++)
                 o[e] = ok ? make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3])
                           : make_float4(nan, nan, nan, nan);
+            if (group == 0) {
+                float2 *ml = reinterpret_cast<float2 *>(a.part_ml + 2 * part_of(r));
+                *ml = ok ? make_float2(m_run, l_run) : make_float2(nan, nan);
+            }
         }
-    } else if (warp < BT_SOFT + BT_OUT + BT_FEED) {
+    } else if (warp < BT_SOFT + G::FEED) {
         // --------------------------------------------------------- feeding --
-        const int f = tid - 32 * (BT_SOFT + BT_OUT);
+        const int f = tid - 32 * BT_SOFT;
         const uint8_t *kb = static_cast<const uint8_t *>(a.pre.k) + row0 * HD * (F32 ? 4 : 1);
         const uint8_t *vb = static_cast<const uint8_t *>(a.pre.v) + row0 * HD * (F32 ? 4 : 1);
         const float *ksc = F32 ? nullptr : a.pre.ks + row0, *vsc = F32 ? nullptr : a.pre.vs + row0;
@@ -489,20 +545,20 @@ k_ba_prefix(const BaArgs a) {
             const uint32_t free_parity = ((t / 2) & 1) ^ 1;
             uint8_t *kt = smem + G::K_AT + st * G::K_STAGE, *vt = smem + G::V_AT + st * G::V_STAGE;
             // The keys of tile t - 2 are done: its scores were issued behind the output of tile t - 4,
-            // which waited for the output warps to be done with tile t - 6, so the ring's slot is
+            // which waited for all to be done with the output of tile t - 6, so the ring's slot is
             // free too.
             if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
-            if (!bt_feed_all(ok)) break;
+            if (!bt_feed_all<G::FEED>(ok)) break;
             float vscale;
             if constexpr (F32) {
-                const float km = ba_pow2(bt_feed_max(x.max_k(), sh.wmax[0]));
-                const float vm = ba_pow2(bt_feed_max(x.max_v(), sh.wmax[1]));
+                const float km = ba_pow2(bt_feed_max<G::FEED>(x.max_k(), sh.wmax[0]));
+                const float vm = ba_pow2(bt_feed_max<G::FEED>(x.max_v(), sh.wmax[1]));
                 x.store_k(kt, G::K_TERM, 0x1p14f / km);
                 if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
                 vscale = vm;
             } else {
                 x.template store_k<FMT>(kt);
-                const float vm = ba_pow2(bt_feed_max(f < 128 ? fabsf(x.vs) : 0.f, sh.wmax[st]));
+                const float vm = ba_pow2(bt_feed_max<G::FEED>(fabsf(x.vs), sh.wmax[st]));
                 if (f < G::BN) sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vm);
                 vscale = vm;
             }
@@ -577,7 +633,7 @@ k_ba_prefix(const BaArgs a) {
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == BT_SOFT + BT_OUT + BT_FEED) {
+    if (warp == BT_SOFT + G::FEED) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::COLS)
                      : "memory");
