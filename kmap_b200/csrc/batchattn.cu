@@ -24,6 +24,7 @@
 #include "batchattn_tc.cuh"
 #include "rows.cuh"
 #include "serve.cuh"
+#include "sm100.cuh"
 
 namespace kllm {
 namespace {
@@ -35,16 +36,51 @@ __device__ __forceinline__ void ba_split32(float x, uint32_t *hi, uint32_t *lo) 
     *lo = __float_as_uint(x - __uint_as_float(*hi));
 }
 
+// A warp's ring of key and value rows in shared memory: each stage holds
+// PT positions (and their scales), copied 16 bytes at a time by the warp's own
+// lanes, so no warp waits for another.  16-byte pieces are permuted within a
+// row by the row's number (ba_turn) so that the fragments' reads, by four
+// lanes a key row and eight lanes a value row, meet no bank twice.
+template <int HD, int FMT>
+struct BaRing {
+    static constexpr bool F32 = FMT == KLLM_KV_F32;
+    static constexpr int PT = F32 ? 16 : 32;             // positions of a turn
+    static constexpr int ROW = HD * (F32 ? 4 : 1);       // bytes
+    static constexpr int PIECES = ROW / 16;              // of a row
+    static constexpr int KV = PT * ROW;                  // bytes of a stage's keys, or values
+    static constexpr int STAGE = 2 * KV + (F32 ? 0 : 2 * PT * 4);
+    static constexpr int STAGES = F32 ? (HD == 128 ? 2 : 3) : HD == 128 ? 3 : 4;
+    static constexpr int SMEM = BA_WARPS * STAGES * STAGE;
+    // the join of the warps (in the rings' place) must fit
+    static_assert(SMEM >= BA_WARPS * BA_ROWS * (HD + 2) * 4, "ring below the join's size");
+};
+
+template <int HD, int FMT>
+__device__ __forceinline__ int ba_turn(int row) {
+    if constexpr (FMT == KLLM_KV_F32) return (row & 6) ^ ((row & 1) << 2);
+    else return HD == 128 ? row & 7 : HD == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
+}
+
+__device__ __forceinline__ void ba_cp16(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void ba_cp4(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0)
+                 : "memory");
+}
+
 // One part of eight query rows of one kv head.  grid: the prefix's
 // (kv head, row tile, part), then the sequences' (sequence, kv head, row tile,
-// part); four warps take turns at blocks of 8 NT positions.
+// part); four warps take turns at blocks of PT positions, each with the next
+// blocks on their way into its ring.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(BA_THREADS, FMT == KLLM_KV_F32 ? 2 : 3)
+__global__ void __launch_bounds__(BA_THREADS, 2)
 k_ba_part(const BaArgs a) {
-    constexpr bool F32 = FMT == KLLM_KV_F32;
-    constexpr int NT = F32 ? 2 : 4;         // 8-position tiles per turn
-    __shared__ float sm_o[BA_WARPS][BA_ROWS][HD];
-    __shared__ float sm_ml[BA_WARPS][BA_ROWS][2];
+    using G = BaRing<HD, FMT>;
+    constexpr bool F32 = G::F32;
+    constexpr int NT = G::PT / 8;           // 8-position tiles per turn
+    extern __shared__ __align__(128) uint8_t ring[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
     // which item
     int b = blockIdx.x, kvh, seq = 0, tile, part, len;
@@ -63,7 +99,43 @@ k_ba_part(const BaArgs a) {
     }
     const BaSide &S = pre ? a.pre : a.own;
     const int p0 = part * S.chunk, p1 = min(len, p0 + S.chunk);
-    if (p0 >= p1) return;
+    if (p0 >= p1) {
+        pdl_wait();
+        return;
+    }
+    // cache rows of this (sequence, kv head)
+    const long long at = (long long)seq * S.seq_stride + (long long)kvh * S.max_pos * HD;
+    const uint8_t *kb = static_cast<const uint8_t *>(S.k) + at * (F32 ? 4 : 1);
+    const uint8_t *vb = static_cast<const uint8_t *>(S.v) + at * (F32 ? 4 : 1);
+    const long long sat = (long long)seq * S.scale_stride + (long long)kvh * S.max_pos;
+    uint8_t *mine = ring + warp * G::STAGES * G::STAGE;
+    const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
+    // turn n of this warp: positions p0 + (4 n + warp) PT ..
+    const int turns = (p1 - p0 + G::PT - 1) / G::PT;
+    const int n_turns = (turns - warp + BA_WARPS - 1) / BA_WARPS;
+    auto fetch = [&](int n) {
+        if (n < n_turns) {
+            const int j0 = p0 + (BA_WARPS * n + warp) * G::PT;
+            const uint32_t st = mine_at + (n % G::STAGES) * G::STAGE;
+#pragma unroll
+            for (int e = 0; e < G::PT * G::PIECES / 32; e++) {
+                const int q = e * 32 + lane, r = q / G::PIECES, c = q % G::PIECES;
+                const uint32_t d = st + r * G::ROW + ((c ^ ba_turn<HD, FMT>(r)) << 4);
+                const long long off = (long long)(j0 + r) * G::ROW + 16 * c;
+                const bool in = j0 + r < p1;
+                ba_cp16(d, kb + (in ? off : 0), in);
+                ba_cp16(d + G::KV, vb + (in ? off : 0), in);
+            }
+            if constexpr (!F32) {
+                const bool in = j0 + lane < p1;
+                ba_cp4(st + 2 * G::KV + 4 * lane, S.ks + sat + (in ? j0 + lane : 0), in);
+                ba_cp4(st + 2 * G::KV + 4 * (G::PT + lane), S.vs + sat + (in ? j0 + lane : 0), in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int n = 0; n < G::STAGES - 1; n++) fetch(n);
     // this lane's query row
     const int n_rows = pre ? a.n_seq * a.groups : a.groups, row = tile * BA_ROWS + g;
     const int qs = pre ? row / a.groups : seq, qh = kvh * a.groups + (pre ? row % a.groups : row);
@@ -99,13 +171,6 @@ k_ba_part(const BaArgs a) {
             ba_split(x2, x3, &qa[ks][2], &qa[ks][3]);
         }
     }
-    // cache rows of this (sequence, kv head)
-    constexpr int ES = F32 ? 4 : 1;
-    const long long at = (long long)seq * S.seq_stride + (long long)kvh * S.max_pos * HD;
-    const uint8_t *kb = static_cast<const uint8_t *>(S.k) + at * ES;
-    const uint8_t *vb = static_cast<const uint8_t *>(S.v) + at * ES;
-    const float *ksc = F32 ? nullptr : S.ks + (long long)seq * S.scale_stride + (long long)kvh * S.max_pos;
-    const float *vsc = F32 ? nullptr : S.vs + (long long)seq * S.scale_stride + (long long)kvh * S.max_pos;
     float m_run = -INFINITY, l_run = 0.f, sv = 0x1p-110f;   // sv: value scale in use (8-bit)
     float o[HD / 8][4];
 #pragma unroll
@@ -113,28 +178,31 @@ k_ba_part(const BaArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) o[t][e] = 0.f;
 
-    for (int j0 = p0 + warp * 8 * NT; j0 < p1; j0 += BA_WARPS * 8 * NT) {
+#pragma unroll 1
+    for (int turn = 0; turn < n_turns; turn++) {
+        const int j0 = p0 + (BA_WARPS * turn + warp) * G::PT;
+        asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 2) : "memory");
+        __syncwarp();
+        fetch(turn + G::STAGES - 1);
+        const uint8_t *kt = mine + (turn % G::STAGES) * G::STAGE, *vt = kt + G::KV;
+        const float *ksc = reinterpret_cast<const float *>(kt + 2 * G::KV), *vsc = ksc + G::PT;
         float s[NT][2];   // log2 scores of row g, positions j0 + 8 t + 2 i + {0, 1}
         float vs[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float c[4] = {0.f, 0.f, 0.f, 0.f};
-            const int jk = j0 + 8 * t + g;        // the key row this lane loads
-            const bool in = jk < p1;
+            const int r = 8 * t + g;              // the key row this lane reads
             if constexpr (F32) {
-                float4 kw[HD / 16];
-#pragma unroll
-                for (int u = 0; u < HD / 16; u++)
-                    ba_ld<16>(reinterpret_cast<uint32_t *>(&kw[u]),
-                              kb + ((long long)jk * HD + 16 * u + 4 * i) * 4, in);
                 float cl[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < HD / 16; u++) {
+                    const float4 k = *reinterpret_cast<const float4 *>(
+                        kt + r * G::ROW + (((4 * u + i) ^ ba_turn<HD, FMT>(r)) << 4));
                     uint32_t h[4], l[4];
-                    ba_split32(kw[u].x, &h[0], &l[0]);
-                    ba_split32(kw[u].y, &h[1], &l[1]);
-                    ba_split32(kw[u].z, &h[2], &l[2]);
-                    ba_split32(kw[u].w, &h[3], &l[3]);
+                    ba_split32(k.x, &h[0], &l[0]);
+                    ba_split32(k.y, &h[1], &l[1]);
+                    ba_split32(k.z, &h[2], &l[2]);
+                    ba_split32(k.w, &h[3], &l[3]);
                     ba_mma_tf32(c, qa[2 * u], h[0], h[1]);
                     ba_mma_tf32(cl, qa[2 * u], l[0], l[1]);
                     ba_mma_tf32(c, qa[2 * u + 1], h[2], h[3]);
@@ -144,18 +212,29 @@ k_ba_part(const BaArgs a) {
                 s[t][1] = (c[1] + ((c[3] + cl[1]) + cl[3])) * rowfac;
             } else {
                 uint32_t kw[HD / 16];
-                ba_ld<HD / 4>(kw, kb + (long long)jk * HD + i * (HD / 4), in);
+                if constexpr (HD == 128) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        *reinterpret_cast<uint4 *>(kw + 4 * e) = *reinterpret_cast<const uint4 *>(
+                            kt + r * G::ROW + (((2 * i + e) ^ ba_turn<HD, FMT>(r)) << 4));
+                } else if constexpr (HD == 64) {
+                    *reinterpret_cast<uint4 *>(kw) =
+                        *reinterpret_cast<const uint4 *>(kt + r * G::ROW + ((i ^ ba_turn<HD, FMT>(r)) << 4));
+                } else {
+                    *reinterpret_cast<uint2 *>(kw) = *reinterpret_cast<const uint2 *>(
+                        kt + r * G::ROW + (((i >> 1) ^ ba_turn<HD, FMT>(r)) << 4) + 8 * (i & 1));
+                }
+                float d[4] = {0.f, 0.f, 0.f, 0.f};      // two chains
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ks++) {
                     const uint32_t w = FMT == KLLM_KV_I8 ? kw[ks] ^ 0x80808080u : kw[ks];
-                    ba_mma_f16(c, qa[ks], ba_codes<FMT, 0>(w), ba_codes<FMT, 1>(w));
+                    ba_mma_f16(ks & 1 ? d : c, qa[ks], ba_codes<FMT, 0>(w), ba_codes<FMT, 1>(w));
                 }
-                const int j = j0 + 8 * t + 2 * i;
-                const float k0 = j < p1 ? __ldg(ksc + j) : 0.f, k1 = j + 1 < p1 ? __ldg(ksc + j + 1) : 0.f;
-                vs[t][0] = j < p1 ? __ldg(vsc + j) : 0.f;
-                vs[t][1] = j + 1 < p1 ? __ldg(vsc + j + 1) : 0.f;
-                s[t][0] = (c[0] + c[2]) * (k0 * rowfac);
-                s[t][1] = (c[1] + c[3]) * (k1 * rowfac);
+                const float2 k2 = *reinterpret_cast<const float2 *>(ksc + 8 * t + 2 * i);
+                const float2 v2 = *reinterpret_cast<const float2 *>(vsc + 8 * t + 2 * i);
+                vs[t][0] = v2.x, vs[t][1] = v2.y;
+                s[t][0] = ((c[0] + d[0]) + (c[2] + d[2])) * (k2.x * rowfac);
+                s[t][1] = ((c[1] + d[1]) + (c[3] + d[3])) * (k2.y * rowfac);
             }
             if (j0 + 8 * t + 2 * i >= p1) s[t][0] = -INFINITY;
             if (j0 + 8 * t + 2 * i + 1 >= p1) s[t][1] = -INFINITY;
@@ -200,14 +279,13 @@ k_ba_part(const BaArgs a) {
                 uint32_t pa[4];
                 ba_split32(s[t][0], &pa[0], &pa[1]);
                 ba_split32(s[t][1], &pa[2], &pa[3]);
-                const int jv = j0 + 8 * t + 2 * i;
+                const int r = 8 * t + 2 * i;
 #pragma unroll
                 for (int u = 0; u < HD / 32; u++) {
-                    float4 v0, v1;
-                    ba_ld<16>(reinterpret_cast<uint32_t *>(&v0), vb + ((long long)jv * HD + 32 * u + 4 * g) * 4,
-                              jv < p1);
-                    ba_ld<16>(reinterpret_cast<uint32_t *>(&v1),
-                              vb + ((long long)(jv + 1) * HD + 32 * u + 4 * g) * 4, jv + 1 < p1);
+                    const float4 v0 = *reinterpret_cast<const float4 *>(
+                        vt + r * G::ROW + (((8 * u + g) ^ ba_turn<HD, FMT>(r)) << 4));
+                    const float4 v1 = *reinterpret_cast<const float4 *>(
+                        vt + (r + 1) * G::ROW + (((8 * u + g) ^ ba_turn<HD, FMT>(r + 1)) << 4));
                     const float x[4] = {v0.x, v0.y, v0.z, v0.w}, y[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -227,11 +305,19 @@ k_ba_part(const BaArgs a) {
                 ba_split(s[t + 1][0] * (vs[t + 1][0] * isv), s[t + 1][1] * (vs[t + 1][1] * isv),
                          &pa[2], &pa[3]);
                 uint32_t vw[4][HD / 32];
-                const int jv = j0 + 8 * t + 2 * i;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int j = jv + (e & 1) + 8 * (e >> 1);
-                    ba_ld<HD / 8>(vw[e], vb + (long long)j * HD + g * (HD / 8), j < p1);
+                    const int r = 8 * t + 2 * i + (e & 1) + 8 * (e >> 1);
+                    const int tn = ba_turn<HD, FMT>(r);
+                    if constexpr (HD == 128)
+                        *reinterpret_cast<uint4 *>(vw[e]) =
+                            *reinterpret_cast<const uint4 *>(vt + r * G::ROW + ((g ^ tn) << 4));
+                    else if constexpr (HD == 64)
+                        *reinterpret_cast<uint2 *>(vw[e]) = *reinterpret_cast<const uint2 *>(
+                            vt + r * G::ROW + (((g >> 1) ^ tn) << 4) + 8 * (g & 1));
+                    else
+                        vw[e][0] = *reinterpret_cast<const uint32_t *>(
+                            vt + r * G::ROW + (((g >> 2) ^ tn) << 4) + 4 * (g & 3));
                     if constexpr (FMT == KLLM_KV_I8)
 #pragma unroll
                         for (int w = 0; w < HD / 32; w++) vw[e][w] ^= 0x80808080u;
@@ -249,8 +335,14 @@ k_ba_part(const BaArgs a) {
                 }
             }
         }
+        __syncwarp();      // the stage may be filled again
     }
-    // join the four warps, in warp order
+    // join the four warps, in warp order, where the rings were
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float(*sm_o)[BA_ROWS][HD] = reinterpret_cast<float(*)[BA_ROWS][HD]>(ring);
+    float(*sm_ml)[BA_ROWS][2] =
+        reinterpret_cast<float(*)[BA_ROWS][2]>(ring + BA_WARPS * BA_ROWS * HD * sizeof(float));
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
     if (i == 0) {
@@ -288,6 +380,8 @@ k_ba_part(const BaArgs a) {
             a.part_ml[2 * out + 1] = l;
         }
     }
+    // done only when the launch before (the prefix's) is: the join waits for this one alone
+    pdl_wait();
 }
 
 // Row (sequence, head) of the output from its parts, one warp per row.
@@ -298,8 +392,9 @@ k_ba_merge(const float *__restrict__ part_ml, const float *__restrict__ part_o, 
            int nh, float *__restrict__ out, long long out_stride, int terms, void *terms_out) {
     constexpr int VEC = HD / 32;
     const int R = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (R >= n_seq * nh) return;
+    if (R >= n_seq * nh) return;       // (the launch's completion needs no wait of this warp)
     const int seq = R / nh, h = R % nh, parts = parts_pre + parts_own;
+    pdl_wait();
     if (own_len && own_len[seq] < 0) return;
     const int len = ba_len(own_len, own_cap, seq);
     const int n = parts_pre + (len > 0 ? (len + chunk_own - 1) / chunk_own : 0);
@@ -322,6 +417,7 @@ k_ba_merge(const float *__restrict__ part_ml, const float *__restrict__ part_o, 
         for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
         L += l;
         const int c = min(32, n - p0);
+#pragma unroll 4
         for (int p = 0; p < c; p++) {
             const float wp = __shfl_sync(0xffffffffu, w, p);
             float v[VEC];
@@ -340,7 +436,7 @@ k_ba_merge(const float *__restrict__ part_ml, const float *__restrict__ part_o, 
     }
 }
 
-// How a call is cut: enough blocks for three per SM, at least 128 positions each.
+// How a call is cut.
 struct BaCut {
     int tiles_pre = 0, tiles_own = 0, own_cap = 0;
     int parts_pre = 0, chunk_pre = 0, parts_own = 0, chunk_own = 0;
@@ -348,11 +444,15 @@ struct BaCut {
     size_t rows = 0, bytes = 0;
 };
 
-void ba_split_range(long long items, int len, int *parts, int *chunk) {
-    const long long want = std::max<long long>(1, (148 * 3 + items - 1) / items);
-    const long long most = (len + 127) / 128;
-    const int n = (int)std::min(want, most);
-    *chunk = ((len + n - 1) / n + 31) / 32 * 32;
+// `items` ranges of up to len positions into parts of at least 128 positions
+// (a turn of each warp), as many as give every SM its two blocks twice over,
+// and of at most 512 where the lengths are only bounds (blocks past a length
+// end at once, the others even out).
+void ba_split_range(long long items, int len, bool bound, int *parts, int *chunk) {
+    const long long want = std::max<long long>(1, (148 * 4 + items - 1) / items);
+    const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : 1;
+    const int n = (int)std::min(std::max(want, least), most);
+    *chunk = ((len + n - 1) / n + 127) / 128 * 128;
     *parts = (len + *chunk - 1) / *chunk;
 }
 
@@ -373,12 +473,13 @@ BaCut ba_cut(const kllm_batch_attn &a) {
             x.chunk_pre = ((pre + n - 1) / n + 127) / 128 * 128;
             x.parts_pre = (pre + x.chunk_pre - 1) / x.chunk_pre;
         } else {
-            ba_split_range(items, pre, &x.parts_pre, &x.chunk_pre);
+            ba_split_range(items, pre, false, &x.parts_pre, &x.chunk_pre);
         }
     }
     if (x.own_cap > 0) {
         x.tiles_own = (groups + BA_ROWS - 1) / BA_ROWS;
-        ba_split_range((long long)a.n_seq * c->n_kv * x.tiles_own, x.own_cap, &x.parts_own, &x.chunk_own);
+        ba_split_range((long long)a.n_seq * c->n_kv * x.tiles_own, x.own_cap, true, &x.parts_own,
+                       &x.chunk_own);
     }
     x.rows = (size_t)a.n_seq * a.n_heads;
     const size_t parts = x.parts_pre + x.parts_own;
@@ -471,19 +572,42 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
         set_error("kllm_batch_attention: %lld blocks", blocks);
         return false;
     }
-    if (x.wide) {
-        if (!ba_prepare(reinterpret_cast<const void *>(k_ba_prefix<HD, FMT>), bt_smem<HD, FMT>())) return false;
-        k_ba_prefix<HD, FMT><<<(unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, bt_smem<HD, FMT>(), s>>>(k);
+    // each launch but the first may start while the one before drains; the
+    // join waits for the parts' launch, which ends only when the prefix's has
+    bool first = true;
+    auto launch = [&](auto kernel, unsigned grid, unsigned block, size_t smem, auto... args) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(block);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = first ? 0 : 1;
+        first = false;
         g_launches++;
+        return KLLM_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    };
+    if (x.wide) {
+        auto kernel = k_ba_prefix<HD, FMT>;
+        constexpr size_t smem = bt_smem<HD, FMT>();
+        if (!ba_prepare(reinterpret_cast<const void *>(kernel), smem) ||
+            !launch(kernel, (unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
+            return false;
     }
     if (blocks) {
-        k_ba_part<HD, FMT><<<(unsigned)blocks, BA_THREADS, 0, s>>>(k);
-        g_launches++;
+        auto kernel = k_ba_part<HD, FMT>;
+        constexpr size_t smem = BaRing<HD, FMT>::SMEM;
+        if (!ba_prepare(reinterpret_cast<const void *>(kernel), smem) ||
+            !launch(kernel, (unsigned)blocks, BA_THREADS, smem, k))
+            return false;
     }
-    k_ba_merge<HD><<<(unsigned)((x.rows + 3) / 4), 128, 0, s>>>(
-        k.part_ml, k.part_o, x.parts_pre, x.parts_own, k.own.chunk, k.own_len, x.own_cap, a.n_seq,
-        a.n_heads, a.out, a.out_stride, terms, terms_out);
-    g_launches++;
+    if (!launch(k_ba_merge<HD>, (unsigned)((x.rows + 3) / 4), 128, 0, (const float *)k.part_ml,
+                (const float *)k.part_o, x.parts_pre, x.parts_own, k.own.chunk, k.own_len, x.own_cap,
+                a.n_seq, a.n_heads, a.out, a.out_stride, terms, terms_out))
+        return false;
     return KLLM_CUDA(cudaGetLastError());
 }
 

@@ -123,23 +123,5 @@ __device__ __forceinline__ void ba_fetch(uint32_t (&w)[1], const void *p, bool i
         : "l"(p), "r"((uint32_t)in));
 }
 
-template <int BYTES>
-__device__ __forceinline__ void ba_ld(uint32_t *w, const void *p, bool in) {
-    if constexpr (BYTES >= 16) {
-#pragma unroll
-        for (int i = 0; i < BYTES / 16; i++) {
-            uint4 t = make_uint4(0, 0, 0, 0);
-            if (in) t = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-            w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
-        }
-    } else if constexpr (BYTES == 8) {
-        uint2 t = make_uint2(0, 0);
-        if (in) t = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = t.x, w[1] = t.y;
-    } else {
-        w[0] = in ? __ldg(reinterpret_cast<const uint32_t *>(p)) : 0u;
-    }
-}
-
 }  // namespace
 }  // namespace kllm
