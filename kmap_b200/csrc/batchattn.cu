@@ -9,9 +9,8 @@
 //
 // Products of fp32 queries and weights run on the tensor cores without
 // losing them to 16 bits: a row of q (and of p) is split into two terms,
-// hi = rn(x), lo = rn(x - hi), and both go through one product as two rows
-// of the same 16-row operand, so a tile is eight query rows by both terms.
-// Codes of 8 bits are exact in fp16; fp32 rows run as two tf32 terms each.
+// hi = rn(x), lo = rn(x - hi), and both go through one product as two columns
+// of the same operand.  Codes of 8 bits are exact in fp16; fp32 rows run as two tf32 terms each.
 // Scores carry scale * log2(e) * (the key row's scale); a weight carries the
 // value row's scale over the largest scale met so far (a power of two), so
 // p's fp16 terms stay in range whatever the scales are.
@@ -40,46 +39,62 @@ __device__ __forceinline__ void ba_split32(float x, uint32_t *hi, uint32_t *lo) 
 // PT positions (and their scales), copied 16 bytes at a time by the warp's own
 // lanes, so no warp waits for another.  16-byte pieces are permuted within a
 // row by the row's number (ba_turn) so that the fragments' reads, by four
-// lanes a key row and eight lanes a value row, meet no bank twice.
+// lanes a key row and eight lanes a value row, meet no bank twice (head dim
+// 128 and fp32; at most twice for 8-bit rows below 128 bytes).
 template <int HD, int FMT>
 struct BaRing {
     static constexpr bool F32 = FMT == KLLM_KV_F32;
     static constexpr int PT = F32 ? 16 : 32;             // positions of a turn
+    static constexpr int WARPS = F32 ? 2 : 4;            // of a block
     static constexpr int ROW = HD * (F32 ? 4 : 1);       // bytes
     static constexpr int PIECES = ROW / 16;              // of a row
     static constexpr int KV = PT * ROW;                  // bytes of a stage's keys, or values
     static constexpr int STAGE = 2 * KV + (F32 ? 0 : 2 * PT * 4);
-    static constexpr int STAGES = F32 ? (HD == 128 ? 2 : 3) : HD == 128 ? 3 : 4;
-    static constexpr int SMEM = BA_WARPS * STAGES * STAGE;
-    // the join of the warps (in the rings' place) must fit
-    static_assert(SMEM >= BA_WARPS * BA_ROWS * (HD + 2) * 4, "ring below the join's size");
+    static constexpr int STAGES = ROW >= 128 ? 2 : 3;
+    static constexpr int RINGS = WARPS * STAGES * STAGE;
+    // the join of the warps takes the rings' place
+    static constexpr int JOIN = WARPS * 8 * (HD + 2) * 4;
+    static constexpr int SMEM = RINGS > JOIN ? RINGS : JOIN;
 };
 
 template <int HD, int FMT>
 __device__ __forceinline__ int ba_turn(int row) {
-    if constexpr (FMT == KLLM_KV_F32) return (row & 6) ^ ((row & 1) << 2);
+    if constexpr (FMT == KLLM_KV_F32) return ((row & 1) << 2) | (row & 2);
     else return HD == 128 ? row & 7 : HD == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
 }
 
-__device__ __forceinline__ void ba_cp16(uint32_t dst, const void *src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+__device__ __forceinline__ void ba_cp16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                  : "memory");
 }
-__device__ __forceinline__ void ba_cp4(uint32_t dst, const void *src, bool in) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0)
+__device__ __forceinline__ void ba_cp4(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                  : "memory");
 }
 
-// One part of eight query rows of one kv head.  grid: the prefix's
-// (kv head, row tile, part), then the sequences' (sequence, kv head, row tile,
-// part); four warps take turns at blocks of PT positions, each with the next
-// blocks on their way into its ring.
-template <int HD, int FMT>
-__global__ void __launch_bounds__(BA_THREADS, 2)
+// an 8 x 8 matrix of 16-bit values, a row in four lanes, transposed
+__device__ __forceinline__ uint32_t ba_transpose(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// One part of 4 NB query rows of one kv head.  grid: the prefix's (kv head,
+// row tile, part), then the sequences' (sequence, kv head, row tile, part);
+// the block's warps take turns at PT positions, each with its next turn on its
+// way into its ring.
+//
+// The keys are the products' 16-row side, four query rows in two terms each
+// its 8 columns: scores [16 positions][row, term], so that lane 4 g + i has
+// row i's scores of positions g and g + 8, both terms.  The weights' two terms,
+// as 16-bit pairs, are transposed within the warp into the other product's
+// 8 columns: output [16 dims][row, term] = V^T [16 dims][16 positions] . P.
+template <int HD, int FMT, int NB>
+__global__ void __launch_bounds__(32 * BaRing<HD, FMT>::WARPS, BaRing<HD, FMT>::F32 ? 3 : NB == 1 ? 3 : 2)
 k_ba_part(const BaArgs a) {
     using G = BaRing<HD, FMT>;
     constexpr bool F32 = G::F32;
-    constexpr int NT = G::PT / 8;           // 8-position tiles per turn
+    constexpr int W = G::WARPS, RT = 4 * NB, NT = G::PT / 16, DT = HD / 16;
     extern __shared__ __align__(128) uint8_t ring[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
     // which item
@@ -110,204 +125,278 @@ k_ba_part(const BaArgs a) {
     const long long sat = (long long)seq * S.scale_stride + (long long)kvh * S.max_pos;
     uint8_t *mine = ring + warp * G::STAGES * G::STAGE;
     const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(mine);
-    // turn n of this warp: positions p0 + (4 n + warp) PT ..
+    // turn n of this warp: positions p0 + (W n + warp) PT ..
     const int turns = (p1 - p0 + G::PT - 1) / G::PT;
-    const int n_turns = (turns - warp + BA_WARPS - 1) / BA_WARPS;
+    const int n_turns = (turns - warp + W - 1) / W;
+    // each lane copies the same pieces of every stage: rows r0, r0 + RS, .. (ba_turn repeats with them)
+    constexpr int RS = 32 / G::PIECES > 0 ? 32 / G::PIECES : 1, CS = G::PIECES > 32 ? G::PIECES / 32 : 1;
+    const int r0 = lane / G::PIECES, c0 = lane % G::PIECES;
     auto fetch = [&](int n) {
         if (n < n_turns) {
-            const int j0 = p0 + (BA_WARPS * n + warp) * G::PT;
+            const int j0 = p0 + (W * n + warp) * G::PT, left = p1 - j0;
             const uint32_t st = mine_at + (n % G::STAGES) * G::STAGE;
+            const uint8_t *ks = kb + (long long)j0 * G::ROW, *vs = vb + (long long)j0 * G::ROW;
 #pragma unroll
-            for (int e = 0; e < G::PT * G::PIECES / 32; e++) {
-                const int q = e * 32 + lane, r = q / G::PIECES, c = q % G::PIECES;
-                const uint32_t d = st + r * G::ROW + ((c ^ ba_turn<HD, FMT>(r)) << 4);
-                const long long off = (long long)(j0 + r) * G::ROW + 16 * c;
-                const bool in = j0 + r < p1;
-                ba_cp16(d, kb + (in ? off : 0), in);
-                ba_cp16(d + G::KV, vb + (in ? off : 0), in);
+            for (int e = 0; e < G::PT / RS; e++) {
+                const int r = r0 + e * RS;
+                const int bytes = r < left ? 16 : 0, row = r < left ? r : 0;
+#pragma unroll
+                for (int q = 0; q < CS; q++) {
+                    const int c = c0 + 32 * q;
+                    const uint32_t d = st + r * G::ROW + ((c ^ ba_turn<HD, FMT>(r)) << 4);
+                    ba_cp16(d, ks + row * G::ROW + 16 * c, bytes);
+                    ba_cp16(d + G::KV, vs + row * G::ROW + 16 * c, bytes);
+                }
             }
             if constexpr (!F32) {
-                const bool in = j0 + lane < p1;
-                ba_cp4(st + 2 * G::KV + 4 * lane, S.ks + sat + (in ? j0 + lane : 0), in);
-                ba_cp4(st + 2 * G::KV + 4 * (G::PT + lane), S.vs + sat + (in ? j0 + lane : 0), in);
+                const int bytes = lane < left ? 4 : 0, row = lane < left ? lane : 0;
+                ba_cp4(st + 2 * G::KV + 4 * lane, S.ks + sat + j0 + row, bytes);
+                ba_cp4(st + 2 * G::KV + 4 * (G::PT + lane), S.vs + sat + j0 + row, bytes);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int n = 0; n < G::STAGES - 1; n++) fetch(n);
-    // this lane's query row
-    const int n_rows = pre ? a.n_seq * a.groups : a.groups, row = tile * BA_ROWS + g;
-    const int qs = pre ? row / a.groups : seq, qh = kvh * a.groups + (pre ? row % a.groups : row);
-    const bool have = row < n_rows;
-    const float *qp = a.q + (long long)qs * a.q_stride + (long long)qh * HD;
-    uint32_t qa[F32 ? HD / 8 : HD / 16][4];
-    float rowfac = a.qk;
-    if constexpr (F32) {
+    // the queries' column of this lane: row g / 2's term g % 2
+    const int n_rows = pre ? a.n_seq * a.groups : a.groups;
+    uint32_t qb[NB][F32 ? HD / 8 : HD / 16][2];
+    float fac[NB];       // of row i's scores
 #pragma unroll
-        for (int u = 0; u < HD / 16; u++)
+    for (int nb = 0; nb < NB; nb++) {
+        const int row = tile * RT + 4 * nb + (g >> 1);
+        const bool have = row < n_rows, low = g & 1;
+        const int qs = pre ? row / a.groups : seq, qh = kvh * a.groups + (pre ? row % a.groups : row);
+        const float *qp = a.q + (long long)qs * a.q_stride + (long long)qh * HD;
+        if constexpr (F32) {
+            fac[nb] = a.qk;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int d = 16 * u + 4 * i + 2 * e;
-                const float x = have ? qp[d] : 0.f, y = have ? qp[d + 1] : 0.f;
-                ba_split32(x, &qa[2 * u + e][0], &qa[2 * u + e][1]);
-                ba_split32(y, &qa[2 * u + e][2], &qa[2 * u + e][3]);
+            for (int u = 0; u < HD / 16; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = have ? qp[16 * u + 4 * i + e] : 0.f;
+                    uint32_t h, l;
+                    ba_split32(x, &h, &l);
+                    qb[nb][2 * u + (e >> 1)][e & 1] = low ? l : h;
+                }
+        } else {
+            // the row brought to [2^13, 2^14) by a power of two
+            float m = 0.f;
+#pragma unroll
+            for (int d = 0; d < HD / 4; d++) m = fmaxf(m, have ? fabsf(qp[i * (HD / 4) + d]) : 0.f);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float up = ba_pow2(m), f = 0x1p14f / up;
+            fac[nb] = __shfl_sync(0xffffffffu, a.qk * up * 0x1p-14f, 8 * i);
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ks++) {
+                const float *p = qp + i * (HD / 4) + 4 * ks;
+                uint32_t h[2], l[2];
+                ba_split(have ? p[0] * f : 0.f, have ? p[1] * f : 0.f, &h[0], &l[0]);
+                ba_split(have ? p[2] * f : 0.f, have ? p[3] * f : 0.f, &h[1], &l[1]);
+                qb[nb][ks][0] = low ? l[0] : h[0];
+                qb[nb][ks][1] = low ? l[1] : h[1];
             }
-    } else {
-        // the row brought to [2^13, 2^14) by a power of two
-        float m = 0.f;
-#pragma unroll
-        for (int d = 0; d < HD / 4; d++) m = fmaxf(m, have ? fabsf(qp[i * (HD / 4) + d]) : 0.f);
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float up = ba_pow2(m), f = 0x1p14f / up;
-        rowfac = a.qk * up * 0x1p-14f;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ks++) {
-            const int d = i * (HD / 4) + 4 * ks;
-            const float x0 = have ? qp[d] * f : 0.f, x1 = have ? qp[d + 1] * f : 0.f;
-            const float x2 = have ? qp[d + 2] * f : 0.f, x3 = have ? qp[d + 3] * f : 0.f;
-            ba_split(x0, x1, &qa[ks][0], &qa[ks][1]);
-            ba_split(x2, x3, &qa[ks][2], &qa[ks][3]);
         }
     }
-    float m_run = -INFINITY, l_run = 0.f, sv = 0x1p-110f;   // sv: value scale in use (8-bit)
-    float o[HD / 8][4];
+    // of row 4 nb + i: maximum and sum; of the warp: the value scale in use (8-bit)
+    float m_run[NB], l_run[NB], sv = 0x1p-110f, o[NB][DT][4];
 #pragma unroll
-    for (int t = 0; t < HD / 8; t++)
+    for (int nb = 0; nb < NB; nb++) {
+        m_run[nb] = -INFINITY, l_run[nb] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[t][e] = 0.f;
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[nb][t][e] = 0.f;
+    }
 
 #pragma unroll 1
     for (int turn = 0; turn < n_turns; turn++) {
-        const int j0 = p0 + (BA_WARPS * turn + warp) * G::PT;
+        const int left = p1 - p0 - (W * turn + warp) * G::PT;
         asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 2) : "memory");
         __syncwarp();
         fetch(turn + G::STAGES - 1);
         const uint8_t *kt = mine + (turn % G::STAGES) * G::STAGE, *vt = kt + G::KV;
         const float *ksc = reinterpret_cast<const float *>(kt + 2 * G::KV), *vsc = ksc + G::PT;
-        float s[NT][2];   // log2 scores of row g, positions j0 + 8 t + 2 i + {0, 1}
-        float vs[NT][2];
+        float s[NB][NT][2];   // log2 scores of row 4 nb + i, positions 16 t + g + {0, 8}
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            const int r = 8 * t + g;              // the key row this lane reads
+            float c[NB][4], d[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[nb][e] = d[nb][e] = 0.f;
+            const int r = 16 * t + g;             // this lane reads key rows r and r + 8
+            const int tn = ba_turn<HD, FMT>(r);   // (the same of both)
             if constexpr (F32) {
-                float cl[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < HD / 16; u++) {
-                    const float4 k = *reinterpret_cast<const float4 *>(
-                        kt + r * G::ROW + (((4 * u + i) ^ ba_turn<HD, FMT>(r)) << 4));
-                    uint32_t h[4], l[4];
-                    ba_split32(k.x, &h[0], &l[0]);
-                    ba_split32(k.y, &h[1], &l[1]);
-                    ba_split32(k.z, &h[2], &l[2]);
-                    ba_split32(k.w, &h[3], &l[3]);
-                    ba_mma_tf32(c, qa[2 * u], h[0], h[1]);
-                    ba_mma_tf32(cl, qa[2 * u], l[0], l[1]);
-                    ba_mma_tf32(c, qa[2 * u + 1], h[2], h[3]);
-                    ba_mma_tf32(cl, qa[2 * u + 1], l[2], l[3]);
-                }
-                s[t][0] = (c[0] + ((c[2] + cl[0]) + cl[2])) * rowfac;
-                s[t][1] = (c[1] + ((c[3] + cl[1]) + cl[3])) * rowfac;
-            } else {
-                uint32_t kw[HD / 16];
-                if constexpr (HD == 128) {
+                    const uint8_t *p = kt + r * G::ROW + (((4 * u + i) ^ tn) << 4);
+                    const float4 x = *reinterpret_cast<const float4 *>(p);
+                    const float4 y = *reinterpret_cast<const float4 *>(p + 8 * G::ROW);
+                    uint32_t h[2][4], l[2][4];
+                    ba_split32(x.x, &h[0][0], &l[0][0]);
+                    ba_split32(y.x, &h[0][1], &l[0][1]);
+                    ba_split32(x.y, &h[0][2], &l[0][2]);
+                    ba_split32(y.y, &h[0][3], &l[0][3]);
+                    ba_split32(x.z, &h[1][0], &l[1][0]);
+                    ba_split32(y.z, &h[1][1], &l[1][1]);
+                    ba_split32(x.w, &h[1][2], &l[1][2]);
+                    ba_split32(y.w, &h[1][3], &l[1][3]);
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        *reinterpret_cast<uint4 *>(kw + 4 * e) = *reinterpret_cast<const uint4 *>(
-                            kt + r * G::ROW + (((2 * i + e) ^ ba_turn<HD, FMT>(r)) << 4));
-                } else if constexpr (HD == 64) {
-                    *reinterpret_cast<uint4 *>(kw) =
-                        *reinterpret_cast<const uint4 *>(kt + r * G::ROW + ((i ^ ba_turn<HD, FMT>(r)) << 4));
-                } else {
-                    *reinterpret_cast<uint2 *>(kw) = *reinterpret_cast<const uint2 *>(
-                        kt + r * G::ROW + (((i >> 1) ^ ba_turn<HD, FMT>(r)) << 4) + 8 * (i & 1));
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            ba_mma_tf32(c[nb], h[e], qb[nb][2 * u + e][0], qb[nb][2 * u + e][1]);
+                            ba_mma_tf32(d[nb], l[e], qb[nb][2 * u + e][0], qb[nb][2 * u + e][1]);
+                        }
                 }
-                float d[4] = {0.f, 0.f, 0.f, 0.f};      // two chains
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        s[nb][t][e] = (c[nb][2 * e] + ((c[nb][2 * e + 1] + d[nb][2 * e]) + d[nb][2 * e + 1])) * fac[nb];
+            } else {
+                uint32_t kw[2][HD / 16];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint8_t *p = kt + (r + 8 * e) * G::ROW;
+                    if constexpr (HD == 128) {
+                        *reinterpret_cast<uint4 *>(kw[e]) = *reinterpret_cast<const uint4 *>(p + (((2 * i) ^ tn) << 4));
+                        *reinterpret_cast<uint4 *>(kw[e] + 4) =
+                            *reinterpret_cast<const uint4 *>(p + (((2 * i + 1) ^ tn) << 4));
+                    } else if constexpr (HD == 64) {
+                        *reinterpret_cast<uint4 *>(kw[e]) = *reinterpret_cast<const uint4 *>(p + ((i ^ tn) << 4));
+                    } else {
+                        *reinterpret_cast<uint2 *>(kw[e]) =
+                            *reinterpret_cast<const uint2 *>(p + (((i >> 1) ^ tn) << 4) + 8 * (i & 1));
+                    }
+                }
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ks++) {
-                    const uint32_t w = FMT == KLLM_KV_I8 ? kw[ks] ^ 0x80808080u : kw[ks];
-                    ba_mma_f16(ks & 1 ? d : c, qa[ks], ba_codes<FMT, 0>(w), ba_codes<FMT, 1>(w));
+                    const uint32_t x = FMT == KLLM_KV_I8 ? kw[0][ks] ^ 0x80808080u : kw[0][ks];
+                    const uint32_t y = FMT == KLLM_KV_I8 ? kw[1][ks] ^ 0x80808080u : kw[1][ks];
+                    const uint32_t ka[4] = {ba_codes<FMT, 0>(x), ba_codes<FMT, 0>(y), ba_codes<FMT, 1>(x),
+                                            ba_codes<FMT, 1>(y)};
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+                        ba_mma_f16(ks & 1 ? d[nb] : c[nb], ka, qb[nb][ks][0], qb[nb][ks][1]);
                 }
-                const float2 k2 = *reinterpret_cast<const float2 *>(ksc + 8 * t + 2 * i);
-                const float2 v2 = *reinterpret_cast<const float2 *>(vsc + 8 * t + 2 * i);
-                vs[t][0] = v2.x, vs[t][1] = v2.y;
-                s[t][0] = ((c[0] + d[0]) + (c[2] + d[2])) * (k2.x * rowfac);
-                s[t][1] = ((c[1] + d[1]) + (c[3] + d[3])) * (k2.y * rowfac);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        s[nb][t][e] = ((c[nb][2 * e] + d[nb][2 * e]) + (c[nb][2 * e + 1] + d[nb][2 * e + 1])) *
+                                      (ksc[r + 8 * e] * fac[nb]);
             }
-            if (j0 + 8 * t + 2 * i >= p1) s[t][0] = -INFINITY;
-            if (j0 + 8 * t + 2 * i + 1 >= p1) s[t][1] = -INFINITY;
-        }
-        float mx = m_run, svx = 0.f;
+            if (left < G::PT) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            mx = fmaxf(mx, fmaxf(s[t][0], s[t][1]));
-            if constexpr (!F32) svx = fmaxf(svx, fmaxf(fabsf(vs[t][0]), fabsf(vs[t][1])));
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if (r + 8 * e >= left) s[nb][t][e] = -INFINITY;
+            }
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        float corr = m_run == -INFINITY ? 0.f : exp2f(m_run - mx);
-        float isv = 1.f;
-        l_run *= corr;
+        // the value rows' scales, relative to the largest met
+        float vs[NT][2], down = 1.f;
         if constexpr (!F32) {
-            svx = fmaxf(svx, __shfl_xor_sync(0xffffffffu, svx, 1));
-            svx = fmaxf(svx, __shfl_xor_sync(0xffffffffu, svx, 2));
-            const float svn = fmaxf(sv, ba_pow2(svx));   // the same in every lane of the warp
-            corr *= sv / svn;
-            sv = svn;
-            isv = 0x1p14f / svn;
+            float most = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    vs[t][e] = vsc[16 * t + g + 8 * e];
+                    most = fmaxf(most, fabsf(vs[t][e]));
+                }
+            if (__any_sync(0xffffffffu, most >= sv)) {      // (of the warp: rare)
+#pragma unroll
+                for (int x = 16; x; x >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                const float up = fmaxf(sv, ba_pow2(most));
+                down = sv / up;
+                sv = up;
+            }
+            const float isv = 0x1p14f / sv;
+#pragma unroll
+            for (int t = 0; t < NT; t++) vs[t][0] *= isv, vs[t][1] *= isv;
         }
-        if (__any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll
-            for (int t = 0; t < HD / 8; t++)
+        for (int nb = 0; nb < NB; nb++) {
+            float mx = m_run[nb];
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[t][e] *= corr;
-        }
-        m_run = mx;
-        const float mref = mx == -INFINITY ? 0.f : mx;
+            for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(s[nb][t][0], s[nb][t][1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float ref = mx == -INFINITY ? 0.f : mx, corr = ba_ex2(m_run[nb] - ref);
+            if (__any_sync(0xffffffffu, corr * down != 1.f)) {
+                l_run[nb] *= corr;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            s[t][0] = exp2f(s[t][0] - mref);
-            s[t][1] = exp2f(s[t][1] - mref);
-            l_run += s[t][0] + s[t][1];
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[nb][t][e] *= corr * down;
+            }
+            m_run[nb] = mx;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                s[nb][t][0] = ba_ex2(s[nb][t][0] - ref);
+                s[nb][t][1] = ba_ex2(s[nb][t][1] - ref);
+                l_run[nb] += s[nb][t][0] + s[nb][t][1];
+            }
         }
         // P.V
         if constexpr (F32) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                uint32_t pa[4];
-                ba_split32(s[t][0], &pa[0], &pa[1]);
-                ba_split32(s[t][1], &pa[2], &pa[3]);
-                const int r = 8 * t + 2 * i;
+            for (int t = 0; t < G::PT / 8; t++) {      // 8 positions: rows i and i + 4 of them
+                uint32_t pb[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float p = __shfl_sync(0xffffffffu, s[nb][t >> 1][t & 1], 4 * (i + 4 * e) + (g >> 1));
+                        uint32_t h, l;
+                        ba_split32(p, &h, &l);
+                        pb[nb][e] = g & 1 ? l : h;
+                    }
+                const int r = 8 * t + i, tn = ba_turn<HD, FMT>(r);      // (the same of r + 4)
 #pragma unroll
                 for (int u = 0; u < HD / 32; u++) {
-                    const float4 v0 = *reinterpret_cast<const float4 *>(
-                        vt + r * G::ROW + (((8 * u + g) ^ ba_turn<HD, FMT>(r)) << 4));
-                    const float4 v1 = *reinterpret_cast<const float4 *>(
-                        vt + (r + 1) * G::ROW + (((8 * u + g) ^ ba_turn<HD, FMT>(r + 1)) << 4));
-                    const float x[4] = {v0.x, v0.y, v0.z, v0.w}, y[4] = {v1.x, v1.y, v1.z, v1.w};
+                    const uint8_t *p = vt + r * G::ROW + (((8 * u + g) ^ tn) << 4);
+                    const float4 x = *reinterpret_cast<const float4 *>(p);
+                    const float4 y = *reinterpret_cast<const float4 *>(p + 4 * G::ROW);
+                    uint32_t h[2][4], l[2][4];
+                    ba_split32(x.x, &h[0][0], &l[0][0]);
+                    ba_split32(x.y, &h[0][1], &l[0][1]);
+                    ba_split32(y.x, &h[0][2], &l[0][2]);
+                    ba_split32(y.y, &h[0][3], &l[0][3]);
+                    ba_split32(x.z, &h[1][0], &l[1][0]);
+                    ba_split32(x.w, &h[1][1], &l[1][1]);
+                    ba_split32(y.z, &h[1][2], &l[1][2]);
+                    ba_split32(y.w, &h[1][3], &l[1][3]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        uint32_t h0, l0, h1, l1;
-                        ba_split32(x[e], &h0, &l0);
-                        ba_split32(y[e], &h1, &l1);
-                        ba_mma_tf32(o[4 * u + e], pa, l0, l1);
-                        ba_mma_tf32(o[4 * u + e], pa, h0, h1);
-                    }
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            ba_mma_tf32(o[nb][2 * u + e], l[e], pb[nb][0], pb[nb][1]);
+                            ba_mma_tf32(o[nb][2 * u + e], h[e], pb[nb][0], pb[nb][1]);
+                        }
                 }
             }
         } else {
 #pragma unroll
-            for (int t = 0; t < NT; t += 2) {   // 16 positions
-                uint32_t pa[4];
-                ba_split(s[t][0] * (vs[t][0] * isv), s[t][1] * (vs[t][1] * isv), &pa[0], &pa[1]);
-                ba_split(s[t + 1][0] * (vs[t + 1][0] * isv), s[t + 1][1] * (vs[t + 1][1] * isv),
-                         &pa[2], &pa[3]);
+            for (int t = 0; t < NT; t++) {   // 16 positions
+                uint32_t pb[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float p = s[nb][t][e] * vs[t][e];
+                        const float h = __half2float(__float2half_rn(p));
+                        pb[nb][e] = ba_transpose(ba_h2(h, p - h));
+                    }
                 uint32_t vw[4][HD / 32];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int r = 8 * t + 2 * i + (e & 1) + 8 * (e >> 1);
+                    const int r = 16 * t + 2 * i + (e & 1) + 8 * (e >> 1);
                     const int tn = ba_turn<HD, FMT>(r);
                     if constexpr (HD == 128)
                         *reinterpret_cast<uint4 *>(vw[e]) =
@@ -328,53 +417,66 @@ k_ba_part(const BaArgs a) {
                     const uint32_t x23 = ba_prmt(vw[0][w], vw[1][w], 0x7362);
                     const uint32_t y01 = ba_prmt(vw[2][w], vw[3][w], 0x5140);
                     const uint32_t y23 = ba_prmt(vw[2][w], vw[3][w], 0x7362);
-                    ba_mma_f16(o[4 * w], pa, ba_codes<FMT, 0>(x01), ba_codes<FMT, 0>(y01));
-                    ba_mma_f16(o[4 * w + 1], pa, ba_codes<FMT, 1>(x01), ba_codes<FMT, 1>(y01));
-                    ba_mma_f16(o[4 * w + 2], pa, ba_codes<FMT, 0>(x23), ba_codes<FMT, 0>(y23));
-                    ba_mma_f16(o[4 * w + 3], pa, ba_codes<FMT, 1>(x23), ba_codes<FMT, 1>(y23));
+                    const uint32_t va[4] = {ba_codes<FMT, 0>(x01), ba_codes<FMT, 1>(x01), ba_codes<FMT, 0>(y01),
+                                            ba_codes<FMT, 1>(y01)};
+                    const uint32_t wa[4] = {ba_codes<FMT, 0>(x23), ba_codes<FMT, 1>(x23), ba_codes<FMT, 0>(y23),
+                                            ba_codes<FMT, 1>(y23)};
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        ba_mma_f16(o[nb][2 * w], va, pb[nb][0], pb[nb][1]);
+                        ba_mma_f16(o[nb][2 * w + 1], wa, pb[nb][0], pb[nb][1]);
+                    }
                 }
             }
         }
         __syncwarp();      // the stage may be filled again
     }
-    // join the four warps, in warp order, where the rings were
+    // join the warps, in warp order, where the rings were
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    float(*sm_o)[BA_ROWS][HD] = reinterpret_cast<float(*)[BA_ROWS][HD]>(ring);
-    float(*sm_ml)[BA_ROWS][2] =
-        reinterpret_cast<float(*)[BA_ROWS][2]>(ring + BA_WARPS * BA_ROWS * HD * sizeof(float));
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    if (i == 0) {
-        sm_ml[warp][g][0] = m_run;
-        sm_ml[warp][g][1] = l_run;
+    float(*sm_o)[8][HD] = reinterpret_cast<float(*)[8][HD]>(ring);
+    float(*sm_ml)[8][2] = reinterpret_cast<float(*)[8][2]>(ring + W * 8 * HD * sizeof(float));
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], x);
+        if (g == 0) {
+            sm_ml[warp][4 * nb + i][0] = m_run[nb];
+            sm_ml[warp][4 * nb + i][1] = l_run[nb];
+        }
     }
     __syncthreads();
-    float M = sm_ml[0][g][0];
 #pragma unroll
-    for (int w = 1; w < BA_WARPS; w++) M = fmaxf(M, sm_ml[w][g][0]);
-    float f = m_run == -INFINITY ? 0.f : exp2f(m_run - M);
-    if constexpr (!F32) f *= sv * 0x1p-14f;
+    for (int nb = 0; nb < NB; nb++) {
+        const int rr = 4 * nb + i;
+        float M = sm_ml[0][rr][0];
 #pragma unroll
-    for (int t = 0; t < HD / 8; t++) {
-        // dims of columns 2 i and 2 i + 1 of tile t
-        const int d0 = F32 ? 32 * (t / 4) + 4 * (2 * i) + t % 4 : 2 * i * (HD / 8) + t;
-        const int d1 = F32 ? d0 + 4 : d0 + HD / 8;
-        sm_o[warp][g][d0] = (o[t][0] + o[t][2]) * f;
-        sm_o[warp][g][d1] = (o[t][1] + o[t][3]) * f;
+        for (int w = 1; w < W; w++) M = fmaxf(M, sm_ml[w][rr][0]);
+        float f = m_run[nb] == -INFINITY ? 0.f : exp2f(m_run[nb] - M);
+        if constexpr (!F32) f *= sv * 0x1p-14f;
+#pragma unroll
+        for (int t = 0; t < DT; t++) {
+            // dims of rows g and g + 8 of tile t
+            const int d = F32 ? 32 * (t >> 1) + 4 * g + 2 * (t & 1) : g * (HD / 8) + 2 * t;
+            *reinterpret_cast<float2 *>(&sm_o[warp][rr][d]) =
+                make_float2((o[nb][t][0] + o[nb][t][1]) * f, (o[nb][t][2] + o[nb][t][3]) * f);
+        }
     }
     __syncthreads();
     const int parts = a.pre.parts + a.own.parts, pi = pre ? part : a.pre.parts + part;
-    for (int x = tid; x < BA_ROWS * HD; x += BA_THREADS) {
-        const int rr = x / HD, d = x % HD, R = tile * BA_ROWS + rr;
+    for (int x = tid; x < RT * HD; x += 32 * W) {
+        const int rr = x / HD, d = x % HD, R = tile * RT + rr;
         if (R >= n_rows) break;
         const int rs = pre ? R / a.groups : seq, rh = kvh * a.groups + (pre ? R % a.groups : R);
         const long long out = ((long long)rs * a.nh + rh) * parts + pi;
-        a.part_o[out * HD + d] = (sm_o[0][rr][d] + sm_o[1][rr][d]) + (sm_o[2][rr][d] + sm_o[3][rr][d]);
+        float v = sm_o[0][rr][d];
+#pragma unroll
+        for (int w = 1; w < W; w++) v += sm_o[w][rr][d];
+        a.part_o[out * HD + d] = v;
         if (d == 0) {
             float mm = sm_ml[0][rr][0], l = 0.f;
-            for (int w = 1; w < BA_WARPS; w++) mm = fmaxf(mm, sm_ml[w][rr][0]);
-            for (int w = 0; w < BA_WARPS; w++)
+            for (int w = 1; w < W; w++) mm = fmaxf(mm, sm_ml[w][rr][0]);
+            for (int w = 0; w < W; w++)
                 if (sm_ml[w][rr][0] != -INFINITY) l += sm_ml[w][rr][1] * exp2f(sm_ml[w][rr][0] - mm);
             a.part_ml[2 * out] = mm;
             a.part_ml[2 * out + 1] = l;
@@ -441,6 +543,7 @@ struct BaCut {
     int tiles_pre = 0, tiles_own = 0, own_cap = 0;
     int parts_pre = 0, chunk_pre = 0, parts_own = 0, chunk_own = 0;
     bool wide = false;      // the prefix by 128-row tiles
+    int nb = 1;             // four query rows a tile, or eight
     size_t rows = 0, bytes = 0;
 };
 
@@ -460,12 +563,14 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const kllm_kv_cache *c = a.prefix ? a.prefix : a.own;
     BaCut x;
     const int groups = a.n_heads / c->n_kv;
+    x.nb = groups > 4 ? 2 : 1;
+    const int tile = 4 * x.nb;
     x.own_cap = a.own ? std::min(a.max_len, a.own->max_pos) : 0;
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
         x.wide = rows >= 32 && pre >= 256;
-        x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : BA_ROWS) - 1) / (x.wide ? BT_ROWS : BA_ROWS));
+        x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : tile) - 1) / (x.wide ? BT_ROWS : tile));
         const long long items = (long long)c->n_kv * x.tiles_pre;
         if (x.wide) {
             // one block an SM: as many parts as fill them once
@@ -477,7 +582,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
         }
     }
     if (x.own_cap > 0) {
-        x.tiles_own = (groups + BA_ROWS - 1) / BA_ROWS;
+        x.tiles_own = (groups + tile - 1) / tile;
         ba_split_range((long long)a.n_seq * c->n_kv * x.tiles_own, x.own_cap, true, &x.parts_own,
                        &x.chunk_own);
     }
@@ -598,10 +703,10 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
             return false;
     }
     if (blocks) {
-        auto kernel = k_ba_part<HD, FMT>;
-        constexpr size_t smem = BaRing<HD, FMT>::SMEM;
-        if (!ba_prepare(reinterpret_cast<const void *>(kernel), smem) ||
-            !launch(kernel, (unsigned)blocks, BA_THREADS, smem, k))
+        auto kernel = x.nb == 1 ? k_ba_part<HD, FMT, 1> : k_ba_part<HD, FMT, 2>;
+        using G = BaRing<HD, FMT>;
+        if (!ba_prepare(reinterpret_cast<const void *>(kernel), G::SMEM) ||
+            !launch(kernel, (unsigned)blocks, 32 * G::WARPS, G::SMEM, k))
             return false;
     }
     if (!launch(k_ba_merge<HD>, (unsigned)((x.rows + 3) / 4), 128, 0, (const float *)k.part_ml,

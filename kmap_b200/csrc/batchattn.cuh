@@ -11,8 +11,6 @@
 namespace kllm {
 namespace {
 
-constexpr int BA_THREADS = 128, BA_WARPS = 4, BA_ROWS = 8;
-
 struct BaSide {
     const void *k, *v;
     const float *ks, *vs;
@@ -44,6 +42,12 @@ __device__ __forceinline__ uint32_t ba_prmt(uint32_t a, uint32_t b, uint32_t sel
 __device__ __forceinline__ uint32_t ba_h2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float ba_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // hi and lo fp16 terms of a pair

@@ -88,12 +88,6 @@ __device__ __forceinline__ bool bt_wait(uint64_t *bar, uint32_t parity, int *dea
     return true;
 }
 
-__device__ __forceinline__ float bt_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Two columns' scores times their keys' scales, and the maximum with them.
 __device__ __forceinline__ float bt_max16(const uint32_t (&x)[16], const float4 *ks, float mx, bool cut,
                                           int n) {
@@ -126,7 +120,7 @@ __device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4
         const float2 k = reinterpret_cast<const float2 *>(ks)[e], v = reinterpret_cast<const float2 *>(pv)[e];
         const float2 y = __ffma2_rn(
             __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), k), f, r);
-        float2 p = make_float2(bt_ex2(y.x), bt_ex2(y.y));
+        float2 p = make_float2(ba_ex2(y.x), ba_ex2(y.y));
         if (cut) {
             if (2 * e >= n) p.x = 0.f;
             if (2 * e + 1 >= n) p.y = 0.f;
@@ -493,7 +487,7 @@ k_ba_prefix(const BaArgs a) {
             if (!ok) return;
             tc_fence_after();
             const float m = sh.mt[ring][r], m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = bt_ex2(m_run - ref), w = bt_ex2(m - ref), f = w * sh.vscale[ring];
+            const float corr = ba_ex2(m_run - ref), w = ba_ex2(m - ref), f = w * sh.vscale[ring];
             l_run = l_run * corr + sh.lt[ring][r] * w;
             m_run = m_new;
 #pragma unroll
