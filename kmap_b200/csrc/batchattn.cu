@@ -98,20 +98,37 @@ k_ba_part(const BaArgs a) {
     extern __shared__ __align__(128) uint8_t ring[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
     // which item
-    int b = blockIdx.x, kvh, seq = 0, tile, part, len;
+    int b = blockIdx.x, kvh, seq = 0, tile, part;
     const int n_pre = a.wide ? 0 : a.nkv * a.tiles_pre * a.pre.parts;
     const bool pre = b < n_pre;
     if (pre) {
         part = b % a.pre.parts, b /= a.pre.parts;
         tile = b % a.tiles_pre, kvh = b / a.tiles_pre;
-        len = a.prefix_len;
     } else {
         b -= n_pre;
         part = b % a.own.parts, b /= a.own.parts;
         tile = b % a.tiles_own, b /= a.tiles_own;
         kvh = b % a.nkv, seq = b / a.nkv;
-        len = ba_len(a.own_len, a.own_cap, seq);
     }
+    // the queries, on their way while the length is read (row 0's for rows past the last)
+    const int n_rows = pre ? a.n_seq * a.groups : a.groups;
+    float qx[NB][HD / 4];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        int row = tile * RT + 4 * nb + (g >> 1);
+        row = row < n_rows ? row : 0;
+        const int qs = pre ? row / a.groups : seq, qh = kvh * a.groups + (pre ? row % a.groups : row);
+        const float *qp = a.q + (long long)qs * a.q_stride + (long long)qh * HD + (F32 ? 4 * i : i * (HD / 4));
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+            const float *p = qp + (F32 ? 16 : 4) * d;
+            float4 x;
+            if (a.q_vec) x = __ldg(reinterpret_cast<const float4 *>(p));
+            else x = make_float4(p[0], p[1], p[2], p[3]);
+            qx[nb][4 * d] = x.x, qx[nb][4 * d + 1] = x.y, qx[nb][4 * d + 2] = x.z, qx[nb][4 * d + 3] = x.w;
+        }
+    }
+    const int len = pre ? a.prefix_len : ba_len(a.own_len, a.own_cap, seq);
     const BaSide &S = pre ? a.pre : a.own;
     const int p0 = part * S.chunk, p1 = min(len, p0 + S.chunk);
     if (p0 >= p1) {
@@ -159,44 +176,39 @@ k_ba_part(const BaArgs a) {
 #pragma unroll
     for (int n = 0; n < G::STAGES - 1; n++) fetch(n);
     // the queries' column of this lane: row g / 2's term g % 2
-    const int n_rows = pre ? a.n_seq * a.groups : a.groups;
     uint32_t qb[NB][F32 ? HD / 8 : HD / 16][2];
     float fac[NB];       // of row i's scores
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        const int row = tile * RT + 4 * nb + (g >> 1);
-        const bool have = row < n_rows, low = g & 1;
-        const int qs = pre ? row / a.groups : seq, qh = kvh * a.groups + (pre ? row % a.groups : row);
-        const float *qp = a.q + (long long)qs * a.q_stride + (long long)qh * HD;
+        const bool have = tile * RT + 4 * nb + (g >> 1) < n_rows, low = g & 1;
+        if (!have)
+#pragma unroll
+            for (int d = 0; d < HD / 4; d++) qx[nb][d] = 0.f;
         if constexpr (F32) {
             fac[nb] = a.qk;
 #pragma unroll
-            for (int u = 0; u < HD / 16; u++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = have ? qp[16 * u + 4 * i + e] : 0.f;
-                    uint32_t h, l;
-                    ba_split32(x, &h, &l);
-                    qb[nb][2 * u + (e >> 1)][e & 1] = low ? l : h;
-                }
+            for (int d = 0; d < HD / 4; d++) {
+                uint32_t h, l;
+                ba_split32(qx[nb][d], &h, &l);
+                qb[nb][d >> 1][d & 1] = low ? l : h;
+            }
         } else {
             // the row brought to [2^13, 2^14) by a power of two
             float m = 0.f;
 #pragma unroll
-            for (int d = 0; d < HD / 4; d++) m = fmaxf(m, have ? fabsf(qp[i * (HD / 4) + d]) : 0.f);
+            for (int d = 0; d < HD / 4; d++) m = fmaxf(m, fabsf(qx[nb][d]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const float up = ba_pow2(m), f = 0x1p14f / up;
             fac[nb] = __shfl_sync(0xffffffffu, a.qk * up * 0x1p-14f, 8 * i);
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ks++) {
-                const float *p = qp + i * (HD / 4) + 4 * ks;
-                uint32_t h[2], l[2];
-                ba_split(have ? p[0] * f : 0.f, have ? p[1] * f : 0.f, &h[0], &l[0]);
-                ba_split(have ? p[2] * f : 0.f, have ? p[3] * f : 0.f, &h[1], &l[1]);
-                qb[nb][ks][0] = low ? l[0] : h[0];
-                qb[nb][ks][1] = low ? l[1] : h[1];
-            }
+            for (int ks = 0; ks < HD / 16; ks++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    uint32_t h, l;
+                    ba_split(qx[nb][4 * ks + 2 * e] * f, qx[nb][4 * ks + 2 * e + 1] * f, &h, &l);
+                    qb[nb][ks][e] = low ? l : h;
+                }
         }
     }
     // of row 4 nb + i: maximum and sum; of the warp: the value scale in use (8-bit)
@@ -569,7 +581,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
-        x.wide = rows >= 32 && pre >= 256;
+        x.wide = rows > 8 && pre >= 256;
         x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : tile) - 1) / (x.wide ? BT_ROWS : tile));
         const long long items = (long long)c->n_kv * x.tiles_pre;
         if (x.wide) {
@@ -655,6 +667,7 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     k.own = side(a.own, x.parts_own, x.chunk_own);
     k.q = a.q;
     k.q_stride = a.q_stride;
+    k.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.n_seq == 1 || a.q_stride % 4 == 0);
     k.own_len = a.own ? a.own_len : nullptr;
     k.n_seq = a.n_seq;
     k.nh = a.n_heads;

@@ -23,6 +23,7 @@ struct BaArgs {
     BaSide pre, own;
     const float *q;
     long long q_stride;
+    bool q_vec;                 // rows of q start on 16 bytes
     const int *own_len;
     int n_seq, nh, nkv, groups, prefix_len, own_cap;
     int tiles_pre, tiles_own;   // row tiles: of n_seq * groups, of groups
