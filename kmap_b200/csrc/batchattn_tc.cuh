@@ -109,41 +109,54 @@ __device__ __forceinline__ float bt_max16(const uint32_t (&x)[16], const float4 
     return mx;
 }
 
-// 16 columns' weights p = 2^(score - ref), their sum, and the fp16 terms of
-// p times their values' scales.
+// 16 columns' weights p = 2^(score - ref) to the tensor memory: the fp16 terms
+// of p times their values' scales, the first in columns at.., the second 8
+// columns behind.  Returns the weights' sum with them.
 __device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4 *ks, const float4 *pv,
-                                           float fac, float ref, float2 sum, bool cut, int n,
-                                           uint32_t (&hi)[8], uint32_t (&lo)[8]) {
-    const float2 f = make_float2(fac, fac), r = make_float2(-ref, -ref);
+                                           float fac, float ref, float2 sum, bool cut, int n, uint32_t at) {
+    const float2 f = make_float2(fac, fac), r = make_float2(-ref, -ref), minus = make_float2(-1.f, -1.f);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float2 k = reinterpret_cast<const float2 *>(ks)[e], v = reinterpret_cast<const float2 *>(pv)[e];
-        const float2 y = __ffma2_rn(
-            __fmul2_rn(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), k), f, r);
-        float2 p = make_float2(ba_ex2(y.x), ba_ex2(y.y));
-        if (cut) {
-            if (2 * e >= n) p.x = 0.f;
-            if (2 * e + 1 >= n) p.y = 0.f;
+    for (int q = 0; q < 2; q++) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float4 k = ks[2 * q + e], v = pv[2 * q + e];
+            const uint32_t *s = x + 8 * q + 4 * e;
+            const float2 a = __ffma2_rn(
+                __fmul2_rn(make_float2(__uint_as_float(s[0]), __uint_as_float(s[1])), make_float2(k.x, k.y)), f, r);
+            const float2 b = __ffma2_rn(
+                __fmul2_rn(make_float2(__uint_as_float(s[2]), __uint_as_float(s[3])), make_float2(k.z, k.w)), f, r);
+            float2 p = make_float2(ba_ex2(a.x), ba_ex2(a.y)), w = make_float2(ba_ex2(b.x), ba_ex2(b.y));
+            if (cut) {
+                if (8 * q + 4 * e >= n) p.x = 0.f;
+                if (8 * q + 4 * e + 1 >= n) p.y = 0.f;
+                if (8 * q + 4 * e + 2 >= n) w.x = 0.f;
+                if (8 * q + 4 * e + 3 >= n) w.y = 0.f;
+            }
+            sum = __fadd2_rn(sum, __fadd2_rn(p, w));
+            p = __fmul2_rn(p, make_float2(v.x, v.y));
+            w = __fmul2_rn(w, make_float2(v.z, v.w));
+            const __half2 ph = __float22half2_rn(p), wh = __float22half2_rn(w);
+            const __half2 pl = __float22half2_rn(__ffma2_rn(__half22float2(ph), minus, p));
+            const __half2 wl = __float22half2_rn(__ffma2_rn(__half22float2(wh), minus, w));
+            hi[2 * e] = *reinterpret_cast<const uint32_t *>(&ph);
+            hi[2 * e + 1] = *reinterpret_cast<const uint32_t *>(&wh);
+            lo[2 * e] = *reinterpret_cast<const uint32_t *>(&pl);
+            lo[2 * e + 1] = *reinterpret_cast<const uint32_t *>(&wl);
         }
-        sum = __fadd2_rn(sum, p);
-        p = __fmul2_rn(p, v);
-        const __half2 h = __float22half2_rn(p);
-        const float2 g = __half22float2(h);
-        const __half2 l = __float22half2_rn(__fadd2_rn(p, make_float2(-g.x, -g.y)));
-        hi[e] = *reinterpret_cast<const uint32_t *>(&h);
-        lo[e] = *reinterpret_cast<const uint32_t *>(&l);
+        tmem_st4(at + 4 * q, hi);
+        tmem_st4(at + 8 + 4 * q, lo);
     }
     return sum;
 }
 
 // The softmax of one row of a tile: scores in columns at.., their maximum (in
 // log2, *m) and the weights' sum relative to it; the weights' two terms take
-// the columns of their scores, 8 columns each for 16 positions.  While 16
-// columns are worked on the next 16 are on their way.
+// the columns of their scores, 8 columns each for 16 positions.
 template <int BN, bool CUT>
 __device__ __forceinline__ void bt_soft(uint32_t at, const float4 *ks, const float4 *pv, float fac, int n,
                                         float *m, float *sum) {
-    uint32_t s0[16], s1[16], hi[8], lo[8];
+    uint32_t s0[16], s1[16];
     float mx = -INFINITY;
     tmem_ld16(at, s0);
 #pragma unroll 1
@@ -158,17 +171,10 @@ __device__ __forceinline__ void bt_soft(uint32_t at, const float4 *ks, const flo
     const float top = mx * fac, ref = top == -INFINITY ? 0.f : top;
     float2 t = make_float2(0.f, 0.f);
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = 0; c < BN; c += 16) {
         tmem_wait_ld16(s0);
-        tmem_ld16(at + c + 16, s1);
-        t = bt_exp16(s0, ks + c / 4, pv + c / 4, fac, ref, t, CUT, n - c, hi, lo);
-        tmem_st8(at + c, hi);
-        tmem_st8(at + c + 8, lo);
-        tmem_wait_ld16(s1);
-        if (c + 32 < BN) tmem_ld16(at + c + 32, s0);
-        t = bt_exp16(s1, ks + c / 4 + 4, pv + c / 4 + 4, fac, ref, t, CUT, n - c - 16, hi, lo);
-        tmem_st8(at + c + 16, hi);
-        tmem_st8(at + c + 24, lo);
+        t = bt_exp16(s0, ks + c / 4, pv + c / 4, fac, ref, t, CUT, n - c, at + c);
+        if (c + 16 < BN) tmem_ld16(at + c + 16, s0);
     }
     *m = top;
     *sum = t.x + t.y;
