@@ -79,6 +79,57 @@ __device__ __forceinline__ uint32_t ba_transpose(uint32_t x) {
     return y;
 }
 
+// The output of row (seq, h), by one warp, VEC = HD / 32 dims a lane: the join
+// of n parts from `at` on and one more (its maximum m, sum l and o).
+template <int HD>
+__device__ __forceinline__ void ba_join(const BaArgs &a, long long at, int n, float m, float l,
+                                        float (&o)[HD / 32], int seq, int h, int lane) {
+    constexpr int VEC = HD / 32;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
+    const float *po = a.part_o + at * HD + VEC * lane;
+    // the first 32 parts' statistics, a part a lane
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (lane < n) mine = ml[lane];
+    float M = fmaxf(m, mine.x);
+    for (int p = lane + 32; p < n; p += 32) M = fmaxf(M, ml[p].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    const float ref = M == -INFINITY ? 0.f : M;
+    // (a part whose scores are all -infinity has no finite sums to give: NaN, as in one pass)
+    const bool none = m == -INFINITY && l == 0.f;
+    const float w0 = none ? 0.f : exp2f(m - ref);
+    float L = l * w0;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) o[e] *= w0;
+    for (int p0 = 0; p0 < n; p0 += 32) {
+        if (p0) mine = p0 + lane < n ? ml[p0 + lane] : make_float2(-INFINITY, 0.f);
+        const float w = p0 + lane < n ? exp2f(mine.x - ref) : 0.f;
+        float s = p0 + lane < n ? mine.y * w : 0.f;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        L += s;
+        const int c = min(32, n - p0);
+#pragma unroll 8
+        for (int p = 0; p < c; p++) {
+            const float wp = __shfl_sync(0xffffffffu, w, p);
+            float v[VEC];
+            bd_load<VEC>(po + (long long)(p0 + p) * HD, v);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) o[e] = fmaf(wp, v[e], o[e]);
+        }
+    }
+    const bool empty = n == 0 && none;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const float v = empty ? 0.f : o[e] / L;
+        if (a.terms_out)
+            bd_emit(v, ((size_t)seq * a.nh + h) * HD + VEC * lane + e, a.terms, (size_t)a.n_seq * a.nh * HD,
+                    a.terms_out);
+        else
+            a.out[(long long)seq * a.out_stride + (long long)h * HD + VEC * lane + e] = v;
+    }
+}
+
 // One part of 4 NB query rows of one kv head.  grid: the prefix's (kv head,
 // row tile, part), then the sequences' (sequence, kv head, row tile, part);
 // the block's warps take turns at PT positions, each with its next turn on its
@@ -99,13 +150,13 @@ k_ba_part(const BaArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
     // which item
     int b = blockIdx.x, kvh, seq = 0, tile, part;
-    const int n_pre = a.wide ? 0 : a.nkv * a.tiles_pre * a.pre.parts;
-    const bool pre = b < n_pre;
+    const bool pre = b < a.blocks_pre;
+    pdl_launch_dependents();
     if (pre) {
         part = b % a.pre.parts, b /= a.pre.parts;
         tile = b % a.tiles_pre, kvh = b / a.tiles_pre;
     } else {
-        b -= n_pre;
+        b -= a.blocks_pre;
         part = b % a.own.parts, b /= a.own.parts;
         tile = b % a.tiles_own, b /= a.tiles_own;
         kvh = b % a.nkv, seq = b / a.nkv;
@@ -128,10 +179,11 @@ k_ba_part(const BaArgs a) {
             qx[nb][4 * d] = x.x, qx[nb][4 * d + 1] = x.y, qx[nb][4 * d + 2] = x.z, qx[nb][4 * d + 3] = x.w;
         }
     }
-    const int len = pre ? a.prefix_len : ba_len(a.own_len, a.own_cap, seq);
+    const int own = pre ? 0 : a.own_len[seq], len = pre ? a.prefix_len : min(own, a.own_cap);
     const BaSide &S = pre ? a.pre : a.own;
-    const int p0 = part * S.chunk, p1 = min(len, p0 + S.chunk);
-    if (p0 >= p1) {
+    const int p0 = part * S.chunk, p1 = max(min(len, p0 + S.chunk), p0);
+    const bool join = a.join && !pre;
+    if ((p0 >= p1 && !join) || own < 0) {
         pdl_wait();
         return;
     }
@@ -476,78 +528,54 @@ k_ba_part(const BaArgs a) {
     }
     __syncthreads();
     const int parts = a.pre.parts + a.own.parts, pi = pre ? part : a.pre.parts + part;
-    for (int x = tid; x < RT * HD; x += 32 * W) {
-        const int rr = x / HD, d = x % HD, R = tile * RT + rr;
+    // a warp takes a row: its part's maximum and sum, VEC dims a lane
+    constexpr int VEC = HD / 32;
+    // (dependent launches: the join below, and the one in k_ba_merge, wait for this
+    // launch alone, so none of its blocks ends before the launch before does)
+    if (!join) pdl_wait();
+    for (int rr = warp; rr < RT; rr += W) {
+        const int R = tile * RT + rr;
         if (R >= n_rows) break;
         const int rs = pre ? R / a.groups : seq, rh = kvh * a.groups + (pre ? R % a.groups : R);
-        const long long out = ((long long)rs * a.nh + rh) * parts + pi;
-        float v = sm_o[0][rr][d];
+        float m = sm_ml[0][rr][0], l = 0.f, v[VEC];
 #pragma unroll
-        for (int w = 1; w < W; w++) v += sm_o[w][rr][d];
-        a.part_o[out * HD + d] = v;
-        if (d == 0) {
-            float mm = sm_ml[0][rr][0], l = 0.f;
-            for (int w = 1; w < W; w++) mm = fmaxf(mm, sm_ml[w][rr][0]);
-            for (int w = 0; w < W; w++)
-                if (sm_ml[w][rr][0] != -INFINITY) l += sm_ml[w][rr][1] * exp2f(sm_ml[w][rr][0] - mm);
-            a.part_ml[2 * out] = mm;
-            a.part_ml[2 * out + 1] = l;
+        for (int w = 1; w < W; w++) m = fmaxf(m, sm_ml[w][rr][0]);
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            if (sm_ml[w][rr][0] != -INFINITY) l += sm_ml[w][rr][1] * exp2f(sm_ml[w][rr][0] - m);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            v[e] = sm_o[0][rr][VEC * lane + e];
+#pragma unroll
+            for (int w = 1; w < W; w++) v[e] += sm_o[w][rr][VEC * lane + e];
+        }
+        const long long at = ((long long)rs * a.nh + rh) * parts;
+        if (join) {
+            pdl_wait();
+            ba_join<HD>(a, at, a.pre.parts, m, l, v, rs, rh, lane);
+        } else {
+            float *o = a.part_o + (at + pi) * HD + VEC * lane;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) o[e] = v[e];
+            if (lane == 0) a.part_ml[2 * (at + pi)] = m, a.part_ml[2 * (at + pi) + 1] = l;
         }
     }
-    // done only when the launch before (the prefix's) is: the join waits for this one alone
-    pdl_wait();
+    if (join) pdl_wait();
 }
 
-// Row (sequence, head) of the output from its parts, one warp per row.
+// Rows whose parts lie in memory, one warp per row.
 template <int HD>
 __global__ void __launch_bounds__(128)
-k_ba_merge(const float *__restrict__ part_ml, const float *__restrict__ part_o, int parts_pre,
-           int parts_own, int chunk_own, const int *__restrict__ own_len, int own_cap, int n_seq,
-           int nh, float *__restrict__ out, long long out_stride, int terms, void *terms_out) {
-    constexpr int VEC = HD / 32;
+k_ba_merge(const BaArgs a) {
     const int R = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (R >= n_seq * nh) return;       // (the launch's completion needs no wait of this warp)
-    const int seq = R / nh, h = R % nh, parts = parts_pre + parts_own;
+    if (R >= a.n_seq * a.nh) return;
+    const int seq = R / a.nh, h = R % a.nh;
     pdl_wait();
-    if (own_len && own_len[seq] < 0) return;
-    const int len = ba_len(own_len, own_cap, seq);
-    const int n = parts_pre + (len > 0 ? (len + chunk_own - 1) / chunk_own : 0);
-    const float *ml = part_ml + (long long)R * parts * 2, *po = part_o + (long long)R * parts * HD;
-    float M = -INFINITY;
-    for (int p = lane; p < n; p += 32) M = fmaxf(M, ml[2 * p]);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    float L = 0.f, acc[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; e++) acc[e] = 0.f;
-    for (int p0 = 0; p0 < n; p0 += 32) {
-        float w = 0.f, l = 0.f;
-        if (p0 + lane < n) {
-            const float m = ml[2 * (p0 + lane)];
-            w = m == -INFINITY && M != -INFINITY ? 0.f : exp2f(m - M);
-            l = ml[2 * (p0 + lane) + 1] * w;
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        L += l;
-        const int c = min(32, n - p0);
-#pragma unroll 4
-        for (int p = 0; p < c; p++) {
-            const float wp = __shfl_sync(0xffffffffu, w, p);
-            float v[VEC];
-            bd_load<VEC>(po + (long long)(p0 + p) * HD + VEC * lane, v);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) acc[e] = fmaf(wp, v[e], acc[e]);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        const float v = n ? acc[e] / L : 0.f;
-        if (terms_out)
-            bd_emit(v, (size_t)R * HD + VEC * lane + e, terms, (size_t)n_seq * nh * HD, terms_out);
-        else
-            out[(long long)seq * out_stride + (long long)h * HD + VEC * lane + e] = v;
-    }
+    const int own = a.own_len ? a.own_len[seq] : 0, len = min(own, a.own_cap);
+    if (own < 0) return;
+    const int n = a.pre.parts + (len > 0 ? (len + a.own.chunk - 1) / a.own.chunk : 0);
+    float v[HD / 32] = {};
+    ba_join<HD>(a, (long long)R * (a.pre.parts + a.own.parts), n, -INFINITY, 0.f, v, seq, h, lane);
 }
 
 // How a call is cut.
@@ -556,6 +584,7 @@ struct BaCut {
     int parts_pre = 0, chunk_pre = 0, parts_own = 0, chunk_own = 0;
     bool wide = false;      // the prefix by 128-row tiles
     int nb = 1;             // four query rows a tile, or eight
+    bool join = false;      // own positions in one part, joined where they are computed
     size_t rows = 0, bytes = 0;
 };
 
@@ -581,7 +610,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
-        x.wide = rows > 8 && pre >= 256;
+        x.wide = rows > 8 && pre >= 256 && (c->format != KLLM_KV_F32 || rows >= 64);
         x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : tile) - 1) / (x.wide ? BT_ROWS : tile));
         const long long items = (long long)c->n_kv * x.tiles_pre;
         if (x.wide) {
@@ -595,8 +624,15 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     }
     if (x.own_cap > 0) {
         x.tiles_own = (groups + tile - 1) / tile;
-        ba_split_range((long long)a.n_seq * c->n_kv * x.tiles_own, x.own_cap, true, &x.parts_own,
-                       &x.chunk_own);
+        const long long items = (long long)a.n_seq * c->n_kv * x.tiles_own;
+        if (x.own_cap <= 256 || (x.own_cap <= 1024 && items >= 296)) {
+            // short, or as many items as blocks at a time: one part, and no launch for the join
+            x.parts_own = 1;
+            x.chunk_own = x.own_cap;
+            x.join = true;
+        } else {
+            ba_split_range(items, x.own_cap, true, &x.parts_own, &x.chunk_own);
+        }
     }
     x.rows = (size_t)a.n_seq * a.n_heads;
     const size_t parts = x.parts_pre + x.parts_own;
@@ -682,16 +718,20 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     const size_t parts = x.parts_pre + x.parts_own;
     k.part_o = reinterpret_cast<float *>(static_cast<char *>(a.workspace) +
                                          (x.rows * parts * 2 * 4 + 15) / 16 * 16);
-    k.wide = x.wide;
+    k.join = x.join;
+    k.out = a.out;
+    k.out_stride = a.out_stride;
+    k.terms = terms;
+    k.terms_out = terms_out;
     const long long pre_blocks = (long long)k.nkv * x.tiles_pre * x.parts_pre;
-    const long long blocks = (x.wide ? 0 : pre_blocks) +
-                             (long long)a.n_seq * k.nkv * x.tiles_own * x.parts_own;
-    if (pre_blocks > 0x7fffffffll || blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
-        set_error("kllm_batch_attention: %lld blocks", blocks);
+    const long long own_blocks = (long long)a.n_seq * k.nkv * x.tiles_own * x.parts_own;
+    if (pre_blocks + own_blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
+        set_error("kllm_batch_attention: %lld blocks", pre_blocks + own_blocks);
         return false;
     }
-    // each launch but the first may start while the one before drains; the
-    // join waits for the parts' launch, which ends only when the prefix's has
+    // Each launch but the first may start beside the one before, and waits
+    // for it where it needs it: the sequences' blocks before they join or end,
+    // k_ba_merge at once.
     bool first = true;
     auto launch = [&](auto kernel, unsigned grid, unsigned block, size_t smem, auto... args) {
         cudaLaunchConfig_t cfg = {};
@@ -715,17 +755,16 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
             !launch(kernel, (unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
             return false;
     }
-    if (blocks) {
+    auto part = [&](long long pre, long long own) {
         auto kernel = x.nb == 1 ? k_ba_part<HD, FMT, 1> : k_ba_part<HD, FMT, 2>;
         using G = BaRing<HD, FMT>;
-        if (!ba_prepare(reinterpret_cast<const void *>(kernel), G::SMEM) ||
-            !launch(kernel, (unsigned)blocks, 32 * G::WARPS, G::SMEM, k))
-            return false;
-    }
-    if (!launch(k_ba_merge<HD>, (unsigned)((x.rows + 3) / 4), 128, 0, (const float *)k.part_ml,
-                (const float *)k.part_o, x.parts_pre, x.parts_own, k.own.chunk, k.own_len, x.own_cap,
-                a.n_seq, a.n_heads, a.out, a.out_stride, terms, terms_out))
-        return false;
+        k.blocks_pre = (int)pre;
+        return pre + own == 0 || (ba_prepare(reinterpret_cast<const void *>(kernel), G::SMEM) &&
+                                  launch(kernel, (unsigned)(pre + own), 32 * G::WARPS, G::SMEM, k));
+    };
+    const long long narrow = x.wide ? 0 : pre_blocks;
+    if (x.join ? !part(narrow, 0) || !part(0, own_blocks) : !part(narrow, own_blocks)) return false;
+    if (!x.join && !launch(k_ba_merge<HD>, (unsigned)((x.rows + 3) / 4), 128, 0, k)) return false;
     return KLLM_CUDA(cudaGetLastError());
 }
 

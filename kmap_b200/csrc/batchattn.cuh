@@ -27,14 +27,15 @@ struct BaArgs {
     const int *own_len;
     int n_seq, nh, nkv, groups, prefix_len, own_cap;
     int tiles_pre, tiles_own;   // row tiles: of n_seq * groups, of groups
-    bool wide;                  // the prefix runs by itself, in tiles of 128 rows (batchattn_tc.cuh)
+    int blocks_pre;             // of this launch: the first take the prefix's items, the rest the sequences'
+    bool join;                  // the sequences' blocks join their rows' parts and write the output
     float qk;                   // scale * log2(e)
     float *part_ml, *part_o;    // [n_seq * nh][parts][2], [n_seq * nh][parts][HD]
+    float *out;
+    long long out_stride;
+    int terms;                  // as bd_emit
+    void *terms_out;
 };
-
-__device__ __forceinline__ int ba_len(const int *own_len, int cap, int i) {
-    return min(own_len ? own_len[i] : 0, cap);
-}
 
 __device__ __forceinline__ uint32_t ba_prmt(uint32_t a, uint32_t b, uint32_t sel) {
     return __byte_perm(a, b, sel);

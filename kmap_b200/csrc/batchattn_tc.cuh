@@ -381,6 +381,7 @@ k_ba_prefix(const BaArgs a) {
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     BtShared &sh = *reinterpret_cast<BtShared *>(smem + G::END);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
     int b = blockIdx.x;
     const int part = b % a.pre.parts;
     b /= a.pre.parts;
