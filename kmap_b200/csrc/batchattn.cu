@@ -63,15 +63,6 @@ __device__ __forceinline__ int ba_turn(int row) {
     else return HD == 128 ? row & 7 : HD == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
 }
 
-__device__ __forceinline__ void ba_cp16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void ba_cp4(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
-}
-
 // an 8 x 8 matrix of 16-bit values, a row in four lanes, transposed
 __device__ __forceinline__ uint32_t ba_transpose(uint32_t x) {
     uint32_t y;

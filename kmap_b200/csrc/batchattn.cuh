@@ -129,5 +129,15 @@ __device__ __forceinline__ void ba_fetch(uint32_t (&w)[1], const void *p, bool i
         : "l"(p), "r"((uint32_t)in));
 }
 
+// Asynchronous copies to shared memory, zeros past `bytes`.
+__device__ __forceinline__ void ba_cp16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void ba_cp4(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+
 }  // namespace
 }  // namespace kllm

@@ -198,17 +198,18 @@ __device__ __forceinline__ float bt_feed_max(float m, float *wmax) {
     return m;
 }
 
-// whether all feeding threads say yes: they leave their loop together
-template <int FEED>
-__device__ __forceinline__ bool bt_feed_all(bool yes) {
+// Whether all of a role's THREADS threads say yes (so that they leave their
+// loop together); the feeding warps' barrier is 2, the softmax warps' 3.
+template <int THREADS, int BAR = 3>
+__device__ __forceinline__ bool bt_all(bool yes) {
     uint32_t all;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 q, %1, 0;\n\t"
-        "barrier.cta.red.and.pred p, 2, %2, q;\n\t"
+        "barrier.cta.red.and.pred p, %3, %2, q;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(all)
-        : "r"((uint32_t)yes), "n"(32 * FEED)
+        : "r"((uint32_t)yes), "n"(THREADS), "n"(BAR)
         : "memory");
     return all != 0;
 }
@@ -413,34 +414,61 @@ k_ba_prefix(const BaArgs a) {
                      ::"r"(smem_u32(&sh.tmem)), "r"(G::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // The queries: LPR lanes a row, four dims each.  q times scale * log2(e), brought to
+    // A softmax warp's 16 rows of the tile, row k of them by lane k: (k / RPW, k % RPW) is its place
+    // in a loop of 16 / RPW turns, HD / 4 lanes a row (small loops: code that runs once costs its
+    // own fetch).
+    constexpr int LPR = HD / 4, RPW = 32 / LPR, TURNS = 16 / RPW;
+    const int my_row = ((lane % 16 / RPW) * BT_SOFT + warp) * RPW + lane % RPW, sub = lane / LPR, dim = 4 * (lane % LPR);
+    const int R = tile * BT_ROWS + my_row, R_seq = R / a.groups, R_head = kvh * a.groups + R % a.groups;
+    const uint32_t have = __ballot_sync(0xffffffffu, R < n_rows && lane < 16);
+    // The queries, raw into the place of keys and values, then times scale * log2(e), brought to
     // [2^13, 2^14) by a power of two, in two fp16 terms.
-    {
-        constexpr int LPR = HD / 4, RPW = 32 / LPR, WARPS = G::THREADS / 32;
-#pragma unroll 2
-        for (int r0 = warp * RPW; r0 < BT_ROWS; r0 += WARPS * RPW) {
-            const int r = r0 + lane / LPR, i = lane % LPR, R = tile * BT_ROWS + r;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (R < n_rows && r < BT_ROWS) {
-                const float *q = a.q + (long long)(R / a.groups) * a.q_stride +
-                                 (long long)(kvh * a.groups + R % a.groups) * HD + 4 * i;
-                x = make_float4(q[0] * a.qk, q[1] * a.qk, q[2] * a.qk, q[3] * a.qk);
+    if (warp < BT_SOFT) {
+        const long long q_at = (long long)R_seq * a.q_stride + (long long)R_head * HD;
+        float *raw = reinterpret_cast<float *>(smem + G::K_AT);
+#pragma unroll 4
+        for (int e = 0; e < TURNS; e++) {
+            const int k = e * RPW + sub, r = (e * BT_SOFT + warp) * RPW + sub;
+            const long long at = __shfl_sync(0xffffffffu, q_at, k);
+            const uint32_t d = smem_u32(raw + r * HD + dim);
+            const int bytes = have >> k & 1;
+            const float *q = a.q + (bytes ? at + dim : 0);
+            if (a.q_vec) {
+                ba_cp16(d, q, 16 * bytes);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) ba_cp4(d + 4 * i, q + (bytes ? i : 0), 4 * bytes);
             }
-            float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // (each lane reads what it copied)
+#pragma unroll 2
+        for (int e = 0; e < TURNS; e++) {
+            const int r = (e * BT_SOFT + warp) * RPW + sub, i = dim / 4;
+            const float4 x = *reinterpret_cast<const float4 *>(raw + r * HD + dim);
+            const float4 y = make_float4(x.x * a.qk, x.y * a.qk, x.z * a.qk, x.w * a.qk);
+            float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
 #pragma unroll
             for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const float up = ba_pow2(m), f = 0x1p14f / up;
-            if (r < BT_ROWS) {
-                if (i == 0) sh.rowfac[r] = up * 0x1p-14f;
-                uint2 h, l;
-                ba_split(x.x * f, x.y * f, &h.x, &l.x);
-                ba_split(x.z * f, x.w * f, &h.y, &l.y);
-                uint8_t *t = bt_at(smem + G::Q_AT + (i >> 4) * (BT_ROWS * 128), r, (i & 15) >> 1) + 8 * (i & 1);
-                *reinterpret_cast<uint2 *>(t) = h;
-                *reinterpret_cast<uint2 *>(t + G::Q_TERM) = l;
-            }
+            if (i == 0) sh.rowfac[r] = up * 0x1p-14f;
+            uint2 h, l;
+            ba_split(y.x * f, y.y * f, &h.x, &l.x);
+            ba_split(y.z * f, y.w * f, &h.y, &l.y);
+            uint8_t *t = bt_at(smem + G::Q_AT + (i >> 4) * (BT_ROWS * 128), r, (i & 15) >> 1) + 8 * (i & 1);
+            *reinterpret_cast<uint2 *>(t) = h;
+            *reinterpret_cast<uint2 *>(t + G::Q_TERM) = l;
         }
         fence_async_shared();
+    } else if (warp < BT_SOFT + G::FEED) {
+        // the first tile's rows towards L2 meanwhile
+        const long long at = (long long)kvh * a.pre.max_pos + p0;
+        constexpr int ROW = HD * (F32 ? 4 : 1);
+        const int bytes = min(G::BN, p1 - p0) * ROW;
+        for (int o = (tid - 32 * BT_SOFT) * 128; o < bytes; o += 32 * G::FEED * 128) {
+            prefetch_l2_line(static_cast<const uint8_t *>(a.pre.k) + at * ROW + o);
+            prefetch_l2_line(static_cast<const uint8_t *>(a.pre.v) + at * ROW + o);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -514,18 +542,30 @@ k_ba_prefix(const BaArgs a) {
             if (t >= 2 && ok) add(t - 2);
             if (t >= 1 && t - 1 < nt && ok) add(t - 1);
         }
-        if (tile * BT_ROWS + r < n_rows) {
-            const float nan = __uint_as_float(0x7fffffffu);
-            float4 *o = reinterpret_cast<float4 *>(a.part_o + part_of(r) * HD + c0);
+        // The rows' sums to memory, by way of the operands' place (all products are done), so that a
+        // warp writes whole rows.
+        constexpr int PITCH = HD + 4;
+        static_assert(BT_ROWS * PITCH * 4 <= G::V_AT, "rows of fp32 in the place of Q and K");
+        float *rows = reinterpret_cast<float *>(smem);
+        ok = bt_all<32 * BT_SOFT>(ok);
 #pragma unroll
-            for (int e = 0; e < NC / 4; e++)
-                o[e] = ok ? make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3])
-                          : make_float4(nan, nan, nan, nan);
-            if (group == 0) {
-                float2 *ml = reinterpret_cast<float2 *>(a.part_ml + 2 * part_of(r));
-                *ml = ok ? make_float2(m_run, l_run) : make_float2(nan, nan);
-            }
+        for (int e = 0; e < NC / 4; e++)
+            *reinterpret_cast<float4 *>(rows + r * PITCH + c0 + 4 * e) =
+                make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+        bt_all<32 * BT_SOFT>(true);
+        const float nan = __uint_as_float(0x7fffffffu);
+        const long long part_at = ((long long)R_seq * a.nh + R_head) * parts + part;
+#pragma unroll 4
+        for (int e = 0; e < TURNS; e++) {
+            const int k = e * RPW + sub, q = (e * BT_SOFT + warp) * RPW + sub;
+            const long long at = __shfl_sync(0xffffffffu, part_at, k);
+            const float4 v = *reinterpret_cast<const float4 *>(rows + q * PITCH + dim);
+            if (have >> k & 1)
+                *reinterpret_cast<float4 *>(a.part_o + at * HD + dim) = ok ? v : make_float4(nan, nan, nan, nan);
         }
+        if (group == 0 && tile * BT_ROWS + r < n_rows)
+            *reinterpret_cast<float2 *>(a.part_ml + 2 * part_of(r)) =
+                ok ? make_float2(m_run, l_run) : make_float2(nan, nan);
     } else if (warp < BT_SOFT + G::FEED) {
         // --------------------------------------------------------- feeding --
         const int f = tid - 32 * BT_SOFT;
@@ -549,7 +589,7 @@ k_ba_prefix(const BaArgs a) {
             // which waited for all to be done with the output of tile t - 6, so the ring's slot is
             // free too.
             if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
-            if (!bt_feed_all<G::FEED>(ok)) break;
+            if (!bt_all<32 * G::FEED, 2>(ok)) break;
             float vscale;
             if constexpr (F32) {
                 const float km = ba_pow2(bt_feed_max<G::FEED>(x.max_k(), sh.wmax[0]));
