@@ -100,32 +100,67 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
                              vec, nz, plane);
         }
     }
+    // (what no row of the warp needs is left out)
+    uint32_t most[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int h = h0 + u * HPW + sub;
-        const bool isq = h < a.n_heads, isk = !isq && h < a.n_heads + c.n_kv;
+        const bool turned = rope && h < a.n_heads + c.n_kv;
         float4 y = x[u];
-        // the partner values live half a row of lanes away
-        float4 o;
-        o.x = __shfl_xor_sync(0xffffffffu, y.x, LPR / 2);
-        o.y = __shfl_xor_sync(0xffffffffu, y.y, LPR / 2);
-        o.z = __shfl_xor_sync(0xffffffffu, y.z, LPR / 2);
-        o.w = __shfl_xor_sync(0xffffffffu, y.w, LPR / 2);
-        if (rope && (isq || isk)) {
+        if (__any_sync(0xffffffffu, turned)) {
+            // the partner values live half a row of lanes away
+            float4 o;
+            o.x = __shfl_xor_sync(0xffffffffu, y.x, LPR / 2);
+            o.y = __shfl_xor_sync(0xffffffffu, y.y, LPR / 2);
+            o.z = __shfl_xor_sync(0xffffffffu, y.z, LPR / 2);
+            o.w = __shfl_xor_sync(0xffffffffu, y.w, LPR / 2);
             if (d < HD / 2) o = make_float4(-o.x, -o.y, -o.z, -o.w);
-            y.x = __fadd_rn(__fmul_rn(y.x, cs.x), __fmul_rn(o.x, sn.x));
-            y.y = __fadd_rn(__fmul_rn(y.y, cs.y), __fmul_rn(o.y, sn.y));
-            y.z = __fadd_rn(__fmul_rn(y.z, cs.z), __fmul_rn(o.z, sn.z));
-            y.w = __fadd_rn(__fmul_rn(y.w, cs.w), __fmul_rn(o.w, sn.w));
+            if (turned) {
+                y.x = __fadd_rn(__fmul_rn(y.x, cs.x), __fmul_rn(o.x, sn.x));
+                y.y = __fadd_rn(__fmul_rn(y.y, cs.y), __fmul_rn(o.y, sn.y));
+                y.z = __fadd_rn(__fmul_rn(y.z, cs.z), __fmul_rn(o.z, sn.z));
+                y.w = __fadd_rn(__fmul_rn(y.w, cs.w), __fmul_rn(o.w, sn.w));
+            }
+            x[u] = y;
         }
         // the row's maximum, by bit patterns: an infinity or a NaN wins
-        uint32_t m = max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
-                         max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
-        if constexpr (FMT != KLLM_KV_F32)
+        if (FMT != KLLM_KV_F32 && __any_sync(0xffffffffu, h >= a.n_heads)) {
+            uint32_t m =
+                max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
+                    max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
 #pragma unroll
             for (int o2 = LPR / 2; o2; o2 >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o2));
+            most[u] = m;
+        } else {
+            most[u] = 0;
+        }
+    }
+    // Row k of the warp's U HPW by lane k: its two divisions, once for all of them, and its scale.
+    float inv = 0.f;
+    constexpr float Q = FMT == KLLM_KV_I8 ? 127.f : 448.f;
+    if constexpr (FMT != KLLM_KV_F32) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t t = __shfl_sync(0xffffffffu, most[u], lane % HPW * LPR);
+            if (lane / HPW == u) m = t;
+        }
+        const bool fine = m < 0x7f800000u;
+        const float amax = fmaxf(__uint_as_float(m), 0x1p-100f);
+        inv = fine ? __fdiv_rn(Q, amax) : 0.f;
+        const int h = h0 + lane - a.n_heads;
+        if (lane < U * HPW && h >= 0 && h < 2 * c.n_kv)
+            (h < c.n_kv ? c.k_scale : c.v_scale)[(long long)s * c.scale_stride +
+                                                 (long long)(h < c.n_kv ? h : h - c.n_kv) * c.max_pos + p] =
+                fine ? fminf(__fdiv_rn(amax, Q), __fdiv_rz(FLT_MAX, Q)) : __uint_as_float(0x7fffffffu);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int h = h0 + u * HPW + sub;
+        const float f = FMT == KLLM_KV_F32 ? 0.f : __shfl_sync(0xffffffffu, inv, u * HPW + sub);
         if (h >= heads) continue;
-        if (isq) {
+        const float4 y = x[u];
+        if (h < a.n_heads) {
             float *q = a.q_out + ((long long)r * a.n_heads + h) * HD + d;
             if (vec) {
                 *reinterpret_cast<float4 *>(q) = y;
@@ -134,25 +169,17 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
             }
             continue;
         }
+        const bool isk = h < a.n_heads + c.n_kv;
         const int hh = isk ? h - a.n_heads : h - a.n_heads - c.n_kv;
-        const long long row = (long long)hh * c.max_pos + p;
+        const long long at = (long long)s * c.seq_stride + ((long long)hh * c.max_pos + p) * HD + d;
         void *dst = isk ? c.k : c.v;
         if constexpr (FMT == KLLM_KV_F32) {
-            *reinterpret_cast<float4 *>(static_cast<float *>(dst) + (long long)s * c.seq_stride +
-                                        row * HD + d) = y;
+            *reinterpret_cast<float4 *>(static_cast<float *>(dst) + at) = y;
         } else {
-            constexpr float Q = FMT == KLLM_KV_I8 ? 127.f : 448.f;
-            const float amax = fmaxf(__uint_as_float(m), 0x1p-100f);
-            const bool fine = m < 0x7f800000u;
-            const float inv = __fdiv_rn(Q, amax);
-            const float4 t = make_float4(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv),
-                                         __fmul_rn(y.z, inv), __fmul_rn(y.w, inv));
-            *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(dst) + (long long)s * c.seq_stride +
-                                          row * HD + d) = fine ? kv_codes<FMT>(t) : 0u;
-            if (d == 0)
-                (isk ? c.k_scale : c.v_scale)[(long long)s * c.scale_stride + row] =
-                    fine ? fminf(__fdiv_rn(amax, Q), __fdiv_rz(FLT_MAX, Q))
-                         : __uint_as_float(0x7fffffffu);
+            // (f is 0 for a row that is not finite: its codes are zeros, and NaN * 0 is none)
+            const uint32_t codes = kv_codes<FMT>(make_float4(__fmul_rn(y.x, f), __fmul_rn(y.y, f),
+                                                             __fmul_rn(y.z, f), __fmul_rn(y.w, f)));
+            *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(dst) + at) = f == 0.f ? 0u : codes;
         }
     }
 }
