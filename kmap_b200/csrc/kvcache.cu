@@ -88,17 +88,15 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
         sn = kv_load4(sp, vec);
     }
     float4 x[U];
+    // where head h of the row's q, k and v would be, h counted through all three
+    const int hk = a.n_heads, hv = a.n_heads + c.n_kv;
+    const long long row = (long long)r * a.row_stride + d;
+    const float *bq = a.q + row, *bk = a.k + row - hk * a.head_stride, *bv = a.v + row - hv * a.head_stride;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int h = h0 + u * HPW + sub;
         x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h < heads) {
-            const bool isq = h < a.n_heads, isk = h < a.n_heads + c.n_kv;
-            const float *b = isq ? a.q : isk ? a.k : a.v;
-            const int hh = isq ? h : isk ? h - a.n_heads : h - a.n_heads - c.n_kv;
-            x[u] = kv_source(b + (long long)r * a.row_stride + (long long)hh * a.head_stride + d,
-                             vec, nz, plane);
-        }
+        if (h < heads) x[u] = kv_source((h < hk ? bq : h < hv ? bk : bv) + h * a.head_stride, vec, nz, plane);
     }
     // (what no row of the warp needs is left out)
     uint32_t most[U];
@@ -154,6 +152,10 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
                                                  (long long)(h < c.n_kv ? h : h - c.n_kv) * c.max_pos + p] =
                 fine ? fminf(__fdiv_rn(amax, Q), __fdiv_rz(FLT_MAX, Q)) : __uint_as_float(0x7fffffffu);
     }
+    constexpr int ES = FMT == KLLM_KV_F32 ? 4 : 1;
+    const long long head = (long long)c.max_pos * HD * ES, at = ((long long)s * c.seq_stride + p * HD + d) * ES;
+    uint8_t *dk = static_cast<uint8_t *>(c.k) + at - hk * head, *dv = static_cast<uint8_t *>(c.v) + at - hv * head;
+    float *dq = a.q_out + (long long)r * a.n_heads * HD + d;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int h = h0 + u * HPW + sub;
@@ -161,7 +163,7 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
         if (h >= heads) continue;
         const float4 y = x[u];
         if (h < a.n_heads) {
-            float *q = a.q_out + ((long long)r * a.n_heads + h) * HD + d;
+            float *q = dq + h * HD;
             if (vec) {
                 *reinterpret_cast<float4 *>(q) = y;
             } else {
@@ -169,17 +171,14 @@ k_kv_append(const kllm_kv_cache c, const kllm_kv_rows a, int nz, long long plane
             }
             continue;
         }
-        const bool isk = h < a.n_heads + c.n_kv;
-        const int hh = isk ? h - a.n_heads : h - a.n_heads - c.n_kv;
-        const long long at = (long long)s * c.seq_stride + ((long long)hh * c.max_pos + p) * HD + d;
-        void *dst = isk ? c.k : c.v;
+        uint8_t *dst = (h < hv ? dk : dv) + h * head;
         if constexpr (FMT == KLLM_KV_F32) {
-            *reinterpret_cast<float4 *>(static_cast<float *>(dst) + at) = y;
+            *reinterpret_cast<float4 *>(dst) = y;
         } else {
             // (f is 0 for a row that is not finite: its codes are zeros, and NaN * 0 is none)
             const uint32_t codes = kv_codes<FMT>(make_float4(__fmul_rn(y.x, f), __fmul_rn(y.y, f),
                                                              __fmul_rn(y.z, f), __fmul_rn(y.w, f)));
-            *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(dst) + at) = f == 0.f ? 0u : codes;
+            *reinterpret_cast<uint32_t *>(dst) = f == 0.f ? 0u : codes;
         }
     }
 }
