@@ -28,10 +28,11 @@
 namespace kllm {
 namespace {
 
-// tf32 terms: the upper 11 significand bits, and the rest (13 bits, of which
-// the product takes 11)
+// tf32 terms: x to the nearest of 11 significand bits, and the rest, which the
+// product cuts to 11: it has either sign, so the cuts do not lean one way, and
+// a NaN stays in it.
 __device__ __forceinline__ void ba_split32(float x, uint32_t *hi, uint32_t *lo) {
-    *hi = __float_as_uint(x) & 0xffffe000u;
+    *hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     *lo = __float_as_uint(x - __uint_as_float(*hi));
 }
 
@@ -601,7 +602,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
-        x.wide = rows > 8 && pre >= 256 && (c->format != KLLM_KV_F32 || rows >= 64);
+        x.wide = rows > 8 && pre >= 256;
         x.tiles_pre = (int)((rows + (x.wide ? BT_ROWS : tile) - 1) / (x.wide ? BT_ROWS : tile));
         const long long items = (long long)c->n_kv * x.tiles_pre;
         if (x.wide) {

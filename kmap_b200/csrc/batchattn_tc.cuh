@@ -19,7 +19,7 @@
 // next tile's loads in flight in registers); one that issues the products.
 // A tile's weights are relative to the tile's own maximum, so that the two
 // groups need nothing of one another; the running maximum is applied where O
-// is added up.  Keys, values, S/P and O have two buffers each; S of the next
+// is added up.  Keys and values (8 bits), S/P and O have two buffers each; S of the next
 // tile is issued before P.V of this one, so that the tensor cores work while
 // the softmax does.  Every wait is bounded; one that gives up leaves NaN in
 // the part's sums.
@@ -42,7 +42,8 @@ constexpr int BT_ROWS = 128, BT_RING = 8;
 template <int HD, int FMT>
 struct BtGeom {
     static constexpr bool F32 = FMT == KLLM_KV_F32;
-    static constexpr int FEED = F32 ? 8 : 4;                     // warps
+    static constexpr int FEED = 4;                               // warps
+    static constexpr int ST = F32 ? 1 : 2;                       // buffers of keys, of values
     static constexpr int THREADS = 32 * (BT_SOFT + FEED + 1);
     static constexpr int BN = F32 ? 64 : 128;                    // positions of a tile
     static constexpr int KT = F32 ? 2 : 1;                       // terms of a key or value
@@ -51,15 +52,16 @@ struct BtGeom {
     static constexpr int Q_TERM = KB * BT_ROWS * 128;
     static constexpr int K_TERM = KB * BN * 128, V_TERM = VB * HD * 128;
     static constexpr int K_STAGE = KT * K_TERM, V_STAGE = KT * V_TERM;
-    static constexpr int Q_AT = 0, K_AT = 2 * Q_TERM, V_AT = K_AT + 2 * K_STAGE;
-    static constexpr int END = V_AT + 2 * V_STAGE;
+    static constexpr int Q_AT = 0, K_AT = 2 * Q_TERM, V_AT = K_AT + ST * K_STAGE;
+    static constexpr int RAW_AT = V_AT + ST * V_STAGE, RAW = F32 ? BN * HD * 4 : 0;      // fp32 keys, values
+    static constexpr int END = RAW_AT + 2 * RAW;
     static constexpr int S_COLS = BN, O_COLS = HD < 32 ? 32 : HD;
     static constexpr int COLS = 2 * (S_COLS + O_COLS) > 256 ? 512 : 2 * (S_COLS + O_COLS) > 128 ? 256 : 128;
 };
 
 struct BtShared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
-    uint64_t sc_full[BT_RING], m_full[BT_RING];
+    uint64_t sc_full[BT_RING], m_full[BT_RING], vs_full[BT_RING];
     uint32_t tmem;
     int dead;
     float wmax[2][8];
@@ -293,81 +295,95 @@ struct BtFeed8 {
     }
 };
 
-// The same of an fp32 tile of 64 positions: K, four dims of rows in turn; V, four
-// dims of 8 positions in a row.
+// The same of an fp32 tile of 64 positions, which comes to shared memory as it
+// is, copied by the threads that will read it (no barrier, few registers):
+// K, 16-byte pieces in a row; V, the pieces of four dims of 8 positions, moved
+// within a row by the position so that eight lanes' reads meet eight banks.
 template <int HD>
 struct BtFeed32 {
-    static constexpr int LPR = HD / 4, RPP = 256 / LPR, NK = (64 + RPP - 1) / RPP;
-    static constexpr int ITEMS = 8 * (HD / 4);
-    float4 k[NK], v[8];
+    static constexpr int PIECES = HD / 4, NK = 64 * PIECES / 128, ITEMS = 8 * PIECES, NV = (ITEMS + 127) / 128;
+    uint8_t *raw_k, *raw_v;
 
-    __device__ __forceinline__ void load_k(const uint8_t *kb, int j0, int n) {
-        const int t = threadIdx.x - 32 * BT_SOFT;
-#pragma unroll
-        for (int p = 0; p < NK; p++) {
-            const int r = p * RPP + t / LPR;
-            uint32_t w[4];
-            ba_fetch(w, kb + ((long long)(j0 + r) * HD + 4 * (t % LPR)) * 4, r < n);
-            k[p] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
-                               __uint_as_float(w[3]));
-        }
-    }
-    __device__ __forceinline__ void load_v(const uint8_t *vb, int j0, int n) {
-        const int t = threadIdx.x - 32 * BT_SOFT;
-        const int pg = t & 7, dg = t >> 3;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int r = pg * 8 + j;
-            uint32_t w[4];
-            ba_fetch(w, vb + ((long long)(j0 + r) * HD + 4 * dg) * 4, t < ITEMS && r < n);
-            v[j] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
-                               __uint_as_float(w[3]));
-        }
-    }
+    static __device__ __forceinline__ int thread() { return threadIdx.x - 32 * BT_SOFT; }
     static __device__ __forceinline__ float most(float4 x) {
         return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
     }
+    __device__ __forceinline__ float4 *v_at(int row, int dg) const {
+        return reinterpret_cast<float4 *>(raw_v) + row * PIECES + (dg ^ ((row >> 3) & 7));
+    }
+    __device__ __forceinline__ void load_k(const uint8_t *kb, int j0, int n) {
+#pragma unroll 4
+        for (int e = 0; e < NK; e++) {
+            const int q = e * 128 + thread(), bytes = q / PIECES < n ? 16 : 0;
+            ba_cp16(smem_u32(raw_k + 16 * q), kb + (bytes ? (long long)j0 * HD * 4 + 16 * q : 0), bytes);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *vb, int j0, int n) {
+#pragma unroll
+        for (int e = 0; e < NV; e++) {
+            const int t = e * 128 + thread(), pg = t & 7, dg = t >> 3;
+            if (t < ITEMS)
+#pragma unroll 4
+                for (int j = 0; j < 8; j++) {
+                    const int r = pg * 8 + j, bytes = r < n ? 16 : 0;
+                    ba_cp16(smem_u32(v_at(r, dg)), vb + (bytes ? ((long long)(j0 + r) * HD + 4 * dg) * 4 : 0), bytes);
+                }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // all but the last group of copies are there
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
     __device__ __forceinline__ float max_k() const {
         float m = 0.f;
-#pragma unroll
-        for (int p = 0; p < NK; p++) m = fmaxf(m, most(k[p]));
+#pragma unroll 4
+        for (int e = 0; e < NK; e++) m = fmaxf(m, most(reinterpret_cast<const float4 *>(raw_k)[e * 128 + thread()]));
         return m;
     }
     __device__ __forceinline__ float max_v() const {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, most(v[j]));
+        for (int e = 0; e < NV; e++) {
+            const int t = e * 128 + thread();
+            if (t < ITEMS)
+#pragma unroll 4
+                for (int j = 0; j < 8; j++) m = fmaxf(m, most(*v_at((t & 7) * 8 + j, t >> 3)));
+        }
         return m;
     }
     __device__ __forceinline__ void store_k(uint8_t *tile, int term, float f) const {
-        const int t = threadIdx.x - 32 * BT_SOFT;
-#pragma unroll
-        for (int p = 0; p < NK; p++) {
-            const int r = p * RPP + t / LPR, i = t % LPR, blk = i >> 4;
-            if (RPP * NK > 64 && r >= 64) continue;
+#pragma unroll 4
+        for (int e = 0; e < NK; e++) {
+            const int q = e * 128 + thread(), r = q / PIECES, i = q % PIECES, blk = i >> 4;
+            const float4 x = reinterpret_cast<const float4 *>(raw_k)[q];
             uint2 h, l;
-            ba_split(k[p].x * f, k[p].y * f, &h.x, &l.x);
-            ba_split(k[p].z * f, k[p].w * f, &h.y, &l.y);
+            ba_split(x.x * f, x.y * f, &h.x, &l.x);
+            ba_split(x.z * f, x.w * f, &h.y, &l.y);
             uint8_t *a = bt_at(tile + blk * (64 * 128), r, (i & 15) >> 1) + 8 * (i & 1);
             *reinterpret_cast<uint2 *>(a) = h;
             *reinterpret_cast<uint2 *>(a + term) = l;
         }
     }
     __device__ __forceinline__ void store_v(uint8_t *tile, int term, float f) const {
-        const int t = threadIdx.x - 32 * BT_SOFT;
-        if (t >= ITEMS) return;
-        const int pg = t & 7, dg = t >> 3;
+#pragma unroll 1
+        for (int e = 0; e < NV; e++) {
+            const int t = e * 128 + thread(), pg = t & 7, dg = t >> 3;
+            if (t >= ITEMS) break;
+            uint32_t h[4][4], l[4][4];      // [dim][positions 2 i, 2 i + 1]
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            uint4 h, l;
-            auto x = [&](int j) { return (e == 0 ? v[j].x : e == 1 ? v[j].y : e == 2 ? v[j].z : v[j].w) * f; };
-            ba_split(x(0), x(1), &h.x, &l.x);
-            ba_split(x(2), x(3), &h.y, &l.y);
-            ba_split(x(4), x(5), &h.z, &l.z);
-            ba_split(x(6), x(7), &h.w, &l.w);
-            uint8_t *a = bt_at(tile, 4 * dg + e, pg);
-            *reinterpret_cast<uint4 *>(a) = h;
-            *reinterpret_cast<uint4 *>(a + term) = l;
+            for (int i = 0; i < 4; i++) {
+                const float4 x = *v_at(pg * 8 + 2 * i, dg), y = *v_at(pg * 8 + 2 * i + 1, dg);
+                ba_split(x.x * f, y.x * f, &h[0][i], &l[0][i]);
+                ba_split(x.y * f, y.y * f, &h[1][i], &l[1][i]);
+                ba_split(x.z * f, y.z * f, &h[2][i], &l[2][i]);
+                ba_split(x.w * f, y.w * f, &h[3][i], &l[3][i]);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                uint8_t *a = bt_at(tile, 4 * dg + d, pg);
+                *reinterpret_cast<uint4 *>(a) = make_uint4(h[d][0], h[d][1], h[d][2], h[d][3]);
+                *reinterpret_cast<uint4 *>(a + term) = make_uint4(l[d][0], l[d][1], l[d][2], l[d][3]);
+            }
         }
     }
 };
@@ -405,6 +421,7 @@ k_ba_prefix(const BaArgs a) {
         for (int i = 0; i < BT_RING; i++) {
             mbar_init(&sh.sc_full[i], 32 * G::FEED);
             mbar_init(&sh.m_full[i], 128);
+            mbar_init(&sh.vs_full[i], 32 * G::FEED);
         }
         sh.dead = 0;
         mbar_fence_init();
@@ -518,6 +535,7 @@ k_ba_prefix(const BaArgs a) {
         auto add = [&](int t) {
             const int ring = t & (BT_RING - 1);
             ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead) &&
+                                             bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead) &&
                                              bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead));
             if (!ok) return;
             tc_fence_after();
@@ -573,56 +591,63 @@ k_ba_prefix(const BaArgs a) {
         const uint8_t *vb = static_cast<const uint8_t *>(a.pre.v) + row0 * HD * (F32 ? 4 : 1);
         const float *ksc = F32 ? nullptr : a.pre.ks + row0, *vsc = F32 ? nullptr : a.pre.vs + row0;
         std::conditional_t<F32, BtFeed32<HD>, BtFeed8<HD>> x;
+        if constexpr (F32) x.raw_k = smem + G::RAW_AT, x.raw_v = smem + G::RAW_AT + G::RAW;
         auto load_k = [&](int t) {
             if constexpr (F32) x.load_k(kb, p0 + t * G::BN, p1 - p0 - t * G::BN);
-            else x.load_k(kb, ksc, vsc, p0 + t * G::BN, min(128, p1 - p0 - t * G::BN));
+            else if (t < nt) x.load_k(kb, ksc, vsc, p0 + t * G::BN, min(128, p1 - p0 - t * G::BN));
         };
-        auto load_v = [&](int t) { x.load_v(vb, p0 + t * G::BN, p1 - p0 - t * G::BN); };
+        auto load_v = [&](int t) {
+            if (F32 || t < nt) x.load_v(vb, p0 + t * G::BN, p1 - p0 - t * G::BN);
+        };
         load_k(0);
         load_v(0);
         bool ok = true;
         for (int t = 0; t < nt; t++) {
-            const int st = t & 1, ring = t & (BT_RING - 1);
-            const uint32_t free_parity = ((t / 2) & 1) ^ 1;
+            const int st = t % G::ST, ring = t & (BT_RING - 1);
+            const uint32_t free_parity = ((t / G::ST) & 1) ^ 1;
             uint8_t *kt = smem + G::K_AT + st * G::K_STAGE, *vt = smem + G::V_AT + st * G::V_STAGE;
-            // The keys of tile t - 2 are done: its scores were issued behind the output of tile t - 4,
-            // which waited for all to be done with the output of tile t - 6, so the ring's slot is
-            // free too.
-            if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
+            // The scores of tile t - ST are done.  They were issued behind the output of tile
+            // t - ST - 2 at least, which waited for all to be done with that of tile t - ST - 4: the
+            // ring's slot, tile t - 8's, is free too.
+            if (t >= G::ST) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
             if (!bt_all<32 * G::FEED, 2>(ok)) break;
-            float vscale;
+            float vscale = 0.f;
             if constexpr (F32) {
+                x.wait();
                 const float km = ba_pow2(bt_feed_max<G::FEED>(x.max_k(), sh.wmax[0]));
-                const float vm = ba_pow2(bt_feed_max<G::FEED>(x.max_v(), sh.wmax[1]));
                 x.store_k(kt, G::K_TERM, 0x1p14f / km);
                 if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
-                vscale = vm;
             } else {
                 x.template store_k<FMT>(kt);
-                const float vm = ba_pow2(bt_feed_max<G::FEED>(fabsf(x.vs), sh.wmax[st]));
-                if (f < G::BN) sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vm);
-                vscale = vm;
+                vscale = ba_pow2(bt_feed_max<G::FEED>(fabsf(x.vs), sh.wmax[st]));
+                if (f < G::BN) sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vscale);
             }
-            if (f == 0) sh.vscale[ring] = F32 ? vscale * 0x1p-14f * 0x1p-14f : vscale * 0x1p-14f;
             fence_async_shared();
             mbar_arrive(&sh.k_full[st]);
             mbar_arrive(&sh.sc_full[ring]);
-            if (t + 1 < nt) load_k(t + 1);
-            if (t >= 2) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead);
+            load_k(t + 1);      // (F32: nothing behind the last tile, but a group of copies)
+            if (t >= G::ST) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead);
+            if constexpr (F32) {
+                x.wait();
+                vscale = ba_pow2(bt_feed_max<G::FEED>(x.max_v(), sh.wmax[1]));
+            }
+            if (f == 0) sh.vscale[ring] = F32 ? vscale * 0x1p-14f * 0x1p-14f : vscale * 0x1p-14f;
             if (ok) {
                 if constexpr (F32) x.store_v(vt, G::V_TERM, 0x1p14f / vscale);
                 else x.template store_v<FMT>(vt);
                 fence_async_shared();
                 mbar_arrive(&sh.v_full[st]);
+                mbar_arrive(&sh.vs_full[ring]);
             }
-            if (t + 1 < nt) load_v(t + 1);
+            load_v(t + 1);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (lane == 0) {
         // -------------------------------------------------------- products --
         constexpr uint32_t s_idesc = umma_idesc_f16(128, G::BN), o_idesc = umma_idesc_f16(128, HD);
         const uint32_t qa = smem_u32(smem + G::Q_AT);
         auto scores = [&](int t) {
-            const uint32_t kt = smem_u32(smem + G::K_AT + (t & 1) * G::K_STAGE), d = s_cols(t);
+            const uint32_t kt = smem_u32(smem + G::K_AT + t % G::ST * G::K_STAGE), d = s_cols(t);
             uint32_t acc = 0;
             // small terms first
 #pragma unroll
@@ -636,10 +661,10 @@ k_ba_prefix(const BaArgs a) {
                 }
             }
             umma_commit(&sh.s_full[t & 1]);
-            umma_commit(&sh.k_empty[t & 1]);
+            umma_commit(&sh.k_empty[t % G::ST]);
         };
         auto output = [&](int t) {
-            const uint32_t vt = smem_u32(smem + G::V_AT + (t & 1) * G::V_STAGE), d = o_cols(t), p = s_cols(t);
+            const uint32_t vt = smem_u32(smem + G::V_AT + t % G::ST * G::V_STAGE), d = o_cols(t), p = s_cols(t);
             uint32_t acc = 0;
 #pragma unroll
             for (int c = (F32 ? 2 : 1); c >= 0; c--) {
@@ -652,20 +677,20 @@ k_ba_prefix(const BaArgs a) {
                 }
             }
             umma_commit(&sh.o_full[t & 1]);
-            umma_commit(&sh.v_empty[t & 1]);
+            umma_commit(&sh.v_empty[t % G::ST]);
         };
         bool ok = bt_wait(&sh.k_full[0], 0, &sh.dead);
         tc_fence_after();
         if (ok) scores(0);
         for (int t = 0; t < nt && ok; t++) {
             if (t + 1 < nt) {
-                ok = bt_wait(&sh.k_full[(t + 1) & 1], ((t + 1) / 2) & 1, &sh.dead);
+                ok = bt_wait(&sh.k_full[(t + 1) % G::ST], ((t + 1) / G::ST) & 1, &sh.dead);
                 tc_fence_after();
                 if (!ok) break;
                 scores(t + 1);
             }
             ok = bt_wait(&sh.p_full[t & 1], (t / 2) & 1, &sh.dead) &&
-                 bt_wait(&sh.v_full[t & 1], (t / 2) & 1, &sh.dead) &&
+                 bt_wait(&sh.v_full[t % G::ST], (t / G::ST) & 1, &sh.dead) &&
                  (t < 2 || bt_wait(&sh.o_empty[t & 1], ((t / 2) & 1) ^ 1, &sh.dead));
             tc_fence_after();
             if (ok) output(t);
