@@ -42,7 +42,7 @@ constexpr int BT_ROWS = 128, BT_RING = 8;
 template <int HD, int FMT>
 struct BtGeom {
     static constexpr bool F32 = FMT == KLLM_KV_F32;
-    static constexpr int FEED = 4;                               // warps
+    static constexpr int FEED = F32 ? 8 : 4;                     // warps
     static constexpr int ST = F32 ? 1 : 2;                       // buffers of keys, of values
     static constexpr int THREADS = 32 * (BT_SOFT + FEED + 1);
     static constexpr int BN = F32 ? 64 : 128;                    // positions of a tile
@@ -64,7 +64,7 @@ struct BtShared {
     uint64_t sc_full[BT_RING], m_full[BT_RING], vs_full[BT_RING];
     uint32_t tmem;
     int dead;
-    float wmax[2][8];
+    float wmax[2][4];
     float vscale[BT_RING];               // what O of the tile is in units of
     float rowfac[BT_ROWS];
     float mt[BT_RING][BT_ROWS], lt[BT_RING][BT_ROWS];     // a tile's maximum and sum of weights, per row
@@ -188,20 +188,19 @@ __device__ __forceinline__ uint8_t *bt_at(uint8_t *tile, int r, int c) {
 }
 
 // the largest |x| of the feeding warps' threads (all call it)
-template <int FEED>
+template <int BAR>
 __device__ __forceinline__ float bt_feed_max(float m, float *wmax) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int w = (threadIdx.x >> 5) - BT_SOFT;
-    if ((threadIdx.x & 31) == 0) wmax[w] = m;
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * FEED) : "memory");
+    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5 & 3] = m;
+    asm volatile("bar.sync %0, 128;" ::"n"(BAR) : "memory");
 #pragma unroll
-    for (int i = 0; i < FEED; i++) m = fmaxf(m, wmax[i]);
+    for (int i = 0; i < 4; i++) m = fmaxf(m, wmax[i]);
     return m;
 }
 
 // Whether all of a role's THREADS threads say yes (so that they leave their
-// loop together); the feeding warps' barrier is 2, the softmax warps' 3.
+// loop together); the feeding warps' barriers are 2 and 5, the softmax warps' 3.
 template <int THREADS, int BAR = 3>
 __device__ __forceinline__ bool bt_all(bool yes) {
     uint32_t all;
@@ -304,7 +303,7 @@ struct BtFeed32 {
     static constexpr int PIECES = HD / 4, NK = 64 * PIECES / 128, ITEMS = 8 * PIECES, NV = (ITEMS + 127) / 128;
     uint8_t *raw_k, *raw_v;
 
-    static __device__ __forceinline__ int thread() { return threadIdx.x - 32 * BT_SOFT; }
+    static __device__ __forceinline__ int thread() { return threadIdx.x & 127; }
     static __device__ __forceinline__ float most(float4 x) {
         return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
     }
@@ -317,7 +316,6 @@ struct BtFeed32 {
             const int q = e * 128 + thread(), bytes = q / PIECES < n ? 16 : 0;
             ba_cp16(smem_u32(raw_k + 16 * q), kb + (bytes ? (long long)j0 * HD * 4 + 16 * q : 0), bytes);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     }
     __device__ __forceinline__ void load_v(const uint8_t *vb, int j0, int n) {
 #pragma unroll
@@ -330,13 +328,15 @@ struct BtFeed32 {
                     ba_cp16(smem_u32(v_at(r, dg)), vb + (bytes ? ((long long)(j0 + r) * HD + 4 * dg) * 4 : 0), bytes);
                 }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    // all but the last group of copies are there
-    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+    // the 64 rows from j0 on towards L2
+    static __device__ __forceinline__ void prefetch(const uint8_t *b, int j0, int n) {
+        for (int o = thread() * 128; o < n * HD * 4; o += 128 * 128) prefetch_l2_line(b + (long long)j0 * HD * 4 + o);
+    }
     __device__ __forceinline__ float max_k() const {
         float m = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int e = 0; e < NK; e++) m = fmaxf(m, most(reinterpret_cast<const float4 *>(raw_k)[e * 128 + thread()]));
         return m;
     }
@@ -352,7 +352,7 @@ struct BtFeed32 {
         return m;
     }
     __device__ __forceinline__ void store_k(uint8_t *tile, int term, float f) const {
-#pragma unroll 4
+#pragma unroll 8
         for (int e = 0; e < NK; e++) {
             const int q = e * 128 + thread(), r = q / PIECES, i = q % PIECES, blk = i >> 4;
             const float4 x = reinterpret_cast<const float4 *>(raw_k)[q];
@@ -409,9 +409,9 @@ k_ba_prefix(const BaArgs a) {
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.k_full[i], 32 * G::FEED);
+            mbar_init(&sh.k_full[i], 128);
             mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 32 * G::FEED);
+            mbar_init(&sh.v_full[i], 128);
             mbar_init(&sh.v_empty[i], 1);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_full[i], 128);
@@ -419,9 +419,9 @@ k_ba_prefix(const BaArgs a) {
             mbar_init(&sh.o_empty[i], 32 * BT_SOFT);
         }
         for (int i = 0; i < BT_RING; i++) {
-            mbar_init(&sh.sc_full[i], 32 * G::FEED);
+            mbar_init(&sh.sc_full[i], 128);
             mbar_init(&sh.m_full[i], 128);
-            mbar_init(&sh.vs_full[i], 32 * G::FEED);
+            mbar_init(&sh.vs_full[i], 128);
         }
         sh.dead = 0;
         mbar_fence_init();
@@ -434,17 +434,20 @@ k_ba_prefix(const BaArgs a) {
     // A softmax warp's 16 rows of the tile, row k of them by lane k: (k / RPW, k % RPW) is its place
     // in a loop of 16 / RPW turns, HD / 4 lanes a row (small loops: code that runs once costs its
     // own fetch).
-    constexpr int LPR = HD / 4, RPW = 32 / LPR, TURNS = 16 / RPW;
+    constexpr int LPR = HD / 4, RPW = 32 / LPR;
     const int my_row = ((lane % 16 / RPW) * BT_SOFT + warp) * RPW + lane % RPW, sub = lane / LPR, dim = 4 * (lane % LPR);
     const int R = tile * BT_ROWS + my_row, R_seq = R / a.groups, R_head = kvh * a.groups + R % a.groups;
     const uint32_t have = __ballot_sync(0xffffffffu, R < n_rows && lane < 16);
+    // Rows of the tile, to the next 32: warps without any leave S, P and O as they are (a row of them
+    // needs nothing of another).
+    const int there = min(BT_ROWS, (n_rows - tile * BT_ROWS + 31) / 32 * 32), turns = there / (8 * RPW);
     // The queries, raw into the place of keys and values, then times scale * log2(e), brought to
     // [2^13, 2^14) by a power of two, in two fp16 terms.
     if (warp < BT_SOFT) {
         const long long q_at = (long long)R_seq * a.q_stride + (long long)R_head * HD;
         float *raw = reinterpret_cast<float *>(smem + G::K_AT);
 #pragma unroll 4
-        for (int e = 0; e < TURNS; e++) {
+        for (int e = 0; e < turns; e++) {
             const int k = e * RPW + sub, r = (e * BT_SOFT + warp) * RPW + sub;
             const long long at = __shfl_sync(0xffffffffu, q_at, k);
             const uint32_t d = smem_u32(raw + r * HD + dim);
@@ -460,7 +463,7 @@ k_ba_prefix(const BaArgs a) {
         asm volatile("cp.async.wait_all;" ::: "memory");
         // (each lane reads what it copied)
 #pragma unroll 2
-        for (int e = 0; e < TURNS; e++) {
+        for (int e = 0; e < turns; e++) {
             const int r = (e * BT_SOFT + warp) * RPW + sub, i = dim / 4;
             const float4 x = *reinterpret_cast<const float4 *>(raw + r * HD + dim);
             const float4 y = make_float4(x.x * a.qk, x.y * a.qk, x.z * a.qk, x.w * a.qk);
@@ -507,6 +510,7 @@ k_ba_prefix(const BaArgs a) {
         constexpr int NC = HD / 2;                 // columns of O of this thread
         const int c0 = group * NC;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const bool rows_here = 32 * (warp & 3) < there;
         const float fac = sh.rowfac[r];
         float m_run = -INFINITY, l_run = 0.f, acc[NC];
 #pragma unroll
@@ -521,12 +525,14 @@ k_ba_prefix(const BaArgs a) {
             tc_fence_after();
             const float4 *ks = reinterpret_cast<const float4 *>(sh.ks[ring]);
             const float4 *pv = reinterpret_cast<const float4 *>(sh.pv[ring]);
-            float m, sum;
-            if (n == G::BN) bt_soft<G::BN, false>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
-            else bt_soft<G::BN, true>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
-            sh.mt[ring][r] = m;
-            sh.lt[ring][r] = sum;
-            tmem_wait_st();
+            if (rows_here) {
+                float m, sum;
+                if (n == G::BN) bt_soft<G::BN, false>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
+                else bt_soft<G::BN, true>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
+                sh.mt[ring][r] = m;
+                sh.lt[ring][r] = sum;
+                tmem_wait_st();
+            }
             tc_fence_before();
             mbar_arrive(&sh.p_full[t & 1]);
             mbar_arrive(&sh.m_full[ring]);
@@ -535,22 +541,24 @@ k_ba_prefix(const BaArgs a) {
         auto add = [&](int t) {
             const int ring = t & (BT_RING - 1);
             ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead) &&
-                                             bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead) &&
+                                             (!F32 || bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead)) &&
                                              bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead));
             if (!ok) return;
             tc_fence_after();
-            const float m = sh.mt[ring][r], m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = ba_ex2(m_run - ref), w = ba_ex2(m - ref), f = w * sh.vscale[ring];
-            l_run = l_run * corr + sh.lt[ring][r] * w;
-            m_run = m_new;
+            if (rows_here) {
+                const float m = sh.mt[ring][r], m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
+                const float corr = ba_ex2(m_run - ref), w = ba_ex2(m - ref), f = w * sh.vscale[ring];
+                l_run = l_run * corr + sh.lt[ring][r] * w;
+                m_run = m_new;
 #pragma unroll
-            for (int c = 0; c < NC / 16; c++) {
-                uint32_t v[16];
-                tmem_ld16(o_cols(t) + lanes + c0 + 16 * c, v);
-                tmem_wait_ld16(v);
+                for (int c = 0; c < NC / 16; c++) {
+                    uint32_t v[16];
+                    tmem_ld16(o_cols(t) + lanes + c0 + 16 * c, v);
+                    tmem_wait_ld16(v);
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    acc[16 * c + e] = fmaf(__uint_as_float(v[e]), f, acc[16 * c + e] * corr);
+                    for (int e = 0; e < 16; e++)
+                        acc[16 * c + e] = fmaf(__uint_as_float(v[e]), f, acc[16 * c + e] * corr);
+                }
             }
             tc_fence_before();
             mbar_arrive(&sh.o_empty[t & 1]);
@@ -568,13 +576,13 @@ k_ba_prefix(const BaArgs a) {
         ok = bt_all<32 * BT_SOFT>(ok);
 #pragma unroll
         for (int e = 0; e < NC / 4; e++)
-            *reinterpret_cast<float4 *>(rows + r * PITCH + c0 + 4 * e) =
+            if (rows_here) *reinterpret_cast<float4 *>(rows + r * PITCH + c0 + 4 * e) =
                 make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
         bt_all<32 * BT_SOFT>(true);
         const float nan = __uint_as_float(0x7fffffffu);
         const long long part_at = ((long long)R_seq * a.nh + R_head) * parts + part;
 #pragma unroll 4
-        for (int e = 0; e < TURNS; e++) {
+        for (int e = 0; e < turns; e++) {
             const int k = e * RPW + sub, q = (e * BT_SOFT + warp) * RPW + sub;
             const long long at = __shfl_sync(0xffffffffu, part_at, k);
             const float4 v = *reinterpret_cast<const float4 *>(rows + q * PITCH + dim);
@@ -586,62 +594,79 @@ k_ba_prefix(const BaArgs a) {
                 ok ? make_float2(m_run, l_run) : make_float2(nan, nan);
     } else if (warp < BT_SOFT + G::FEED) {
         // --------------------------------------------------------- feeding --
-        const int f = tid - 32 * BT_SOFT;
+        // Before the scales of a tile are written: the scores of tile t - ST are done.  They were issued
+        // behind the output of tile t - 4 or a later one, which waited for all to be done with that of
+        // tile t - 6; so the ring's slot, tile t - 8's, is free.
+        const int f = tid & 127;
         const uint8_t *kb = static_cast<const uint8_t *>(a.pre.k) + row0 * HD * (F32 ? 4 : 1);
         const uint8_t *vb = static_cast<const uint8_t *>(a.pre.v) + row0 * HD * (F32 ? 4 : 1);
-        const float *ksc = F32 ? nullptr : a.pre.ks + row0, *vsc = F32 ? nullptr : a.pre.vs + row0;
-        std::conditional_t<F32, BtFeed32<HD>, BtFeed8<HD>> x;
-        if constexpr (F32) x.raw_k = smem + G::RAW_AT, x.raw_v = smem + G::RAW_AT + G::RAW;
-        auto load_k = [&](int t) {
-            if constexpr (F32) x.load_k(kb, p0 + t * G::BN, p1 - p0 - t * G::BN);
-            else if (t < nt) x.load_k(kb, ksc, vsc, p0 + t * G::BN, min(128, p1 - p0 - t * G::BN));
-        };
-        auto load_v = [&](int t) {
-            if (F32 || t < nt) x.load_v(vb, p0 + t * G::BN, p1 - p0 - t * G::BN);
-        };
-        load_k(0);
-        load_v(0);
         bool ok = true;
-        for (int t = 0; t < nt; t++) {
-            const int st = t % G::ST, ring = t & (BT_RING - 1);
-            const uint32_t free_parity = ((t / G::ST) & 1) ^ 1;
-            uint8_t *kt = smem + G::K_AT + st * G::K_STAGE, *vt = smem + G::V_AT + st * G::V_STAGE;
-            // The scores of tile t - ST are done.  They were issued behind the output of tile
-            // t - ST - 2 at least, which waited for all to be done with that of tile t - ST - 4: the
-            // ring's slot, tile t - 8's, is free too.
-            if (t >= G::ST) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
-            if (!bt_all<32 * G::FEED, 2>(ok)) break;
-            float vscale = 0.f;
-            if constexpr (F32) {
-                x.wait();
-                const float km = ba_pow2(bt_feed_max<G::FEED>(x.max_k(), sh.wmax[0]));
-                x.store_k(kt, G::K_TERM, 0x1p14f / km);
-                if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
+        auto left = [&](int t) { return min(G::BN, p1 - p0 - t * G::BN); };
+        if constexpr (F32) {
+            // four warps bring keys, four values
+            BtFeed32<HD> x = {smem + G::RAW_AT, smem + G::RAW_AT + G::RAW};
+            uint8_t *kt = smem + G::K_AT, *vt = smem + G::V_AT;
+            if (warp < BT_SOFT + 4) {
+                x.load_k(kb, p0, left(0));
+                for (int t = 0; t < nt; t++) {
+                    const int ring = t & (BT_RING - 1);
+                    if (t + 1 < nt) x.prefetch(kb, p0 + (t + 1) * G::BN, left(t + 1));
+                    x.wait();
+                    const float km = ba_pow2(bt_feed_max<1>(x.max_k(), sh.wmax[0]));
+                    if (t) ok = bt_wait(&sh.k_empty[0], (t & 1) ^ 1, &sh.dead);
+                    if (!bt_all<128, 2>(ok)) break;
+                    x.store_k(kt, G::K_TERM, 0x1p14f / km);
+                    if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
+                    fence_async_shared();
+                    mbar_arrive(&sh.k_full[0]);
+                    mbar_arrive(&sh.sc_full[ring]);
+                    if (t + 1 < nt) x.load_k(kb, p0 + (t + 1) * G::BN, left(t + 1));
+                }
             } else {
-                x.template store_k<FMT>(kt);
-                vscale = ba_pow2(bt_feed_max<G::FEED>(fabsf(x.vs), sh.wmax[st]));
-                if (f < G::BN) sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vscale);
+                x.load_v(vb, p0, left(0));
+                for (int t = 0; t < nt; t++) {
+                    const int ring = t & (BT_RING - 1);
+                    if (t + 1 < nt) x.prefetch(vb, p0 + (t + 1) * G::BN, left(t + 1));
+                    x.wait();
+                    const float vm = ba_pow2(bt_feed_max<4>(x.max_v(), sh.wmax[1]));
+                    if (t) ok = bt_wait(&sh.v_empty[0], (t & 1) ^ 1, &sh.dead);
+                    if (!bt_all<128, 5>(ok)) break;
+                    x.store_v(vt, G::V_TERM, 0x1p14f / vm);
+                    if (f == 0) sh.vscale[ring] = vm * 0x1p-14f * 0x1p-14f;
+                    fence_async_shared();
+                    mbar_arrive(&sh.v_full[0]);
+                    mbar_arrive(&sh.vs_full[ring]);
+                    if (t + 1 < nt) x.load_v(vb, p0 + (t + 1) * G::BN, left(t + 1));
+                }
             }
-            fence_async_shared();
-            mbar_arrive(&sh.k_full[st]);
-            mbar_arrive(&sh.sc_full[ring]);
-            load_k(t + 1);      // (F32: nothing behind the last tile, but a group of copies)
-            if (t >= G::ST) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead);
-            if constexpr (F32) {
-                x.wait();
-                vscale = ba_pow2(bt_feed_max<G::FEED>(x.max_v(), sh.wmax[1]));
-            }
-            if (f == 0) sh.vscale[ring] = F32 ? vscale * 0x1p-14f * 0x1p-14f : vscale * 0x1p-14f;
-            if (ok) {
-                if constexpr (F32) x.store_v(vt, G::V_TERM, 0x1p14f / vscale);
-                else x.template store_v<FMT>(vt);
+            x.wait();      // (nothing of it comes after the block)
+        } else {
+            const float *ksc = a.pre.ks + row0, *vsc = a.pre.vs + row0;
+            BtFeed8<HD> x;
+            x.load_k(kb, ksc, vsc, p0, left(0));
+            x.load_v(vb, p0, left(0));
+            for (int t = 0; t < nt; t++) {
+                const int st = t & 1, ring = t & (BT_RING - 1);
+                const uint32_t free_parity = ((t / 2) & 1) ^ 1;
+                if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
+                if (!bt_all<128, 2>(ok)) break;
+                x.template store_k<FMT>(smem + G::K_AT + st * G::K_STAGE);
+                const float vscale = ba_pow2(bt_feed_max<1>(fabsf(x.vs), sh.wmax[st]));
+                sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vscale);
+                if (f == 0) sh.vscale[ring] = vscale * 0x1p-14f;
                 fence_async_shared();
-                mbar_arrive(&sh.v_full[st]);
-                mbar_arrive(&sh.vs_full[ring]);
+                mbar_arrive(&sh.k_full[st]);
+                mbar_arrive(&sh.sc_full[ring]);
+                if (t + 1 < nt) x.load_k(kb, ksc, vsc, p0 + (t + 1) * G::BN, left(t + 1));
+                if (t >= 2) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead);
+                if (ok) {
+                    x.template store_v<FMT>(smem + G::V_AT + st * G::V_STAGE);
+                    fence_async_shared();
+                    mbar_arrive(&sh.v_full[st]);
+                }
+                if (t + 1 < nt) x.load_v(vb, p0 + (t + 1) * G::BN, left(t + 1));
             }
-            load_v(t + 1);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (lane == 0) {
         // -------------------------------------------------------- products --
         constexpr uint32_t s_idesc = umma_idesc_f16(128, G::BN), o_idesc = umma_idesc_f16(128, HD);
@@ -679,21 +704,21 @@ k_ba_prefix(const BaArgs a) {
             umma_commit(&sh.o_full[t & 1]);
             umma_commit(&sh.v_empty[t % G::ST]);
         };
-        bool ok = bt_wait(&sh.k_full[0], 0, &sh.dead);
-        tc_fence_after();
-        if (ok) scores(0);
-        for (int t = 0; t < nt && ok; t++) {
-            if (t + 1 < nt) {
-                ok = bt_wait(&sh.k_full[(t + 1) % G::ST], ((t + 1) / G::ST) & 1, &sh.dead);
+        // S of the next tile ahead of O of this one: the tensor cores work while the softmax does.
+        bool ok = true;
+        for (int t = 0; t <= nt && ok; t++) {
+            if (t < nt) {
+                ok = bt_wait(&sh.k_full[t % G::ST], (t / G::ST) & 1, &sh.dead);
                 tc_fence_after();
-                if (!ok) break;
-                scores(t + 1);
+                if (ok) scores(t);
             }
-            ok = bt_wait(&sh.p_full[t & 1], (t / 2) & 1, &sh.dead) &&
-                 bt_wait(&sh.v_full[t % G::ST], (t / G::ST) & 1, &sh.dead) &&
-                 (t < 2 || bt_wait(&sh.o_empty[t & 1], ((t / 2) & 1) ^ 1, &sh.dead));
+            const int u = t - 1;
+            if (u < 0 || !ok) continue;
+            ok = bt_wait(&sh.p_full[u & 1], (u / 2) & 1, &sh.dead) &&
+                 bt_wait(&sh.v_full[u % G::ST], (u / G::ST) & 1, &sh.dead) &&
+                 (u < 2 || bt_wait(&sh.o_empty[u & 1], ((u / 2) & 1) ^ 1, &sh.dead));
             tc_fence_after();
-            if (ok) output(t);
+            if (ok) output(u);
         }
     }
     __syncwarp();
