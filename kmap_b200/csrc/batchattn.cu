@@ -15,7 +15,6 @@
 // value row's scale over the largest scale met so far (a power of two), so
 // p's fp16 terms stay in range whatever the scales are.
 #include <algorithm>
-#include <cstdlib>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -55,8 +54,7 @@ struct BaRing {
     static constexpr int STAGES = ROW >= 128 ? 2 : 3;
     static constexpr int RINGS = WARPS * STAGES * STAGE;
     // the join of the warps takes the rings' place
-    static constexpr int ROWS = F32 ? 12 : 8;           // at most
-    static constexpr int JOIN = WARPS * ROWS * (HD + 2) * 4;
+    static constexpr int JOIN = WARPS * 8 * (HD + 2) * 4;
     static constexpr int SMEM = RINGS > JOIN ? RINGS : JOIN;
 };
 
@@ -492,8 +490,8 @@ k_ba_part(const BaArgs a) {
     // join the warps, in warp order, where the rings were
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    float(*sm_o)[G::ROWS][HD] = reinterpret_cast<float(*)[G::ROWS][HD]>(ring);
-    float(*sm_ml)[G::ROWS][2] = reinterpret_cast<float(*)[G::ROWS][2]>(ring + W * G::ROWS * HD * sizeof(float));
+    float(*sm_o)[8][HD] = reinterpret_cast<float(*)[8][HD]>(ring);
+    float(*sm_ml)[8][2] = reinterpret_cast<float(*)[8][2]>(ring + W * 8 * HD * sizeof(float));
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
@@ -582,24 +580,14 @@ struct BaCut {
     size_t rows = 0, bytes = 0;
 };
 
-// `items` ranges of `len` positions into parts of at least 128 positions (a
-// turn of each warp): as many as end first, when `slots` blocks run at a time.
-// A block costs about 128 positions' time beside its own.
-void ba_split_even(long long items, int len, int slots, int *parts, int *chunk) {
-    const int most = (int)std::min<long long>((len + 127) / 128, std::max<long long>(2 * slots / items, 1));
-    long long best = -1;
-    for (int n = 1; n <= most; n++) {
-        const int c = ((len + n - 1) / n + 127) / 128 * 128, p = (len + c - 1) / c;
-        const long long cost = (items * p + slots - 1) / slots * (c + 128);
-        if (best < 0 || cost < best) best = cost, *parts = p, *chunk = c;
-    }
-}
-
-// The same where the lengths are only bounds: parts of at most 512 positions
-// (blocks past a length end at once, the others even out).
-void ba_split_bound(long long items, int len, int *parts, int *chunk) {
+// `items` ranges of up to len positions into parts of at least 128 positions
+// (a turn of each warp), as many as give every SM its two blocks twice over,
+// and of at most 512 where the lengths are only bounds (blocks past a length
+// end at once, the others even out).
+void ba_split_range(long long items, int len, bool bound, int *parts, int *chunk) {
     const long long want = std::max<long long>(1, (148 * 4 + items - 1) / items);
-    const int n = (int)std::min<long long>(std::max<long long>(want, (len + 511) / 512), (len + 127) / 128);
+    const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : 1;
+    const int n = (int)std::min(std::max(want, least), most);
     *chunk = ((len + n - 1) / n + 127) / 128 * 128;
     *parts = (len + *chunk - 1) / *chunk;
 }
@@ -614,8 +602,14 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
-        x.wide = rows > (c->format == KLLM_KV_F32 ? atoi(getenv("BAW")) : 8) && pre >= 256;
-        x.nb_pre = c->format == KLLM_KV_F32 ? (int)std::min<long long>((rows + 3) / 4, atoi(getenv("BAN"))) : x.nb;
+        // The 128-row tiles' time hardly depends on the rows, the narrow tiles' goes with them.  8 bits:
+        // XXX.  fp32 (two terms to make of each key and value): 4000 positions of 32 kv heads of 128,
+        // 16 rows, 56 us narrow and 66 wide; 24 rows, 88 and 67; 1000 positions of 4 kv heads of 64, 128
+        // rows, 16.0 and 18.7; 192 rows, 22.8 and 18.8.
+        x.wide = c->format == KLLM_KV_F32 ? rows >= 24 && c->n_kv * rows * pre >= 1000000 : rows > 8 && pre >= 256;
+        // fp32 tiles are read once per tile: eight rows as soon as there are more than four (24 rows x 4000
+        // as above: 89 us, 95 in tiles of four)
+        x.nb_pre = c->format == KLLM_KV_F32 ? (rows > 4 ? 2 : 1) : x.nb;
         const int t = x.wide ? BT_ROWS : 4 * x.nb_pre;
         x.tiles_pre = (int)((rows + t - 1) / t);
         const long long items = (long long)c->n_kv * x.tiles_pre;
@@ -625,9 +619,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
             x.chunk_pre = ((pre + n - 1) / n + 127) / 128 * 128;
             x.parts_pre = (pre + x.chunk_pre - 1) / x.chunk_pre;
         } else {
-            // (of the launch bounds: fp32 3 blocks an SM, 8 bits 3 for four rows, 2 for eight)
-            ba_split_even(items, pre, 148 * (c->format == KLLM_KV_F32 || x.nb_pre == 1 ? 3 : 2), &x.parts_pre,
-                          &x.chunk_pre);
+            ba_split_range(items, pre, false, &x.parts_pre, &x.chunk_pre);
         }
     }
     if (x.own_cap > 0) {
@@ -639,7 +631,7 @@ BaCut ba_cut(const kllm_batch_attn &a) {
             x.chunk_own = x.own_cap;
             x.join = true;
         } else {
-            ba_split_bound(items, x.own_cap, &x.parts_own, &x.chunk_own);
+            ba_split_range(items, x.own_cap, true, &x.parts_own, &x.chunk_own);
         }
     }
     x.rows = (size_t)a.n_seq * a.n_heads;
@@ -766,8 +758,6 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     auto part = [&](long long pre, long long own) {
         const int nb = pre ? x.nb_pre : x.nb;
         auto kernel = nb == 1 ? k_ba_part<HD, FMT, 1> : k_ba_part<HD, FMT, 2>;
-        if constexpr (FMT == KLLM_KV_F32)
-            if (nb == 3) kernel = k_ba_part<HD, FMT, 3>;
         using G = BaRing<HD, FMT>;
         k.blocks_pre = (int)pre;
         return pre + own == 0 || (ba_prepare(reinterpret_cast<const void *>(kernel), G::SMEM) &&
