@@ -602,11 +602,18 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     const int pre = a.prefix ? a.prefix_len : 0;
     if (pre > 0) {
         const long long rows = (long long)a.n_seq * groups;
-        // The 128-row tiles' time hardly depends on the rows, the narrow tiles' goes with them.  8 bits:
-        // XXX.  fp32 (two terms to make of each key and value): 4000 positions of 32 kv heads of 128,
-        // 16 rows, 56 us narrow and 66 wide; 24 rows, 88 and 67; 1000 positions of 4 kv heads of 64, 128
-        // rows, 16.0 and 18.7; 192 rows, 22.8 and 18.8.
-        x.wide = c->format == KLLM_KV_F32 ? rows >= 24 && c->n_kv * rows * pre >= 1000000 : rows > 8 && pre >= 256;
+        // The 128-row tiles have a start of some 12 us and little time per row, the narrow tiles 6 us and
+        // theirs per row: which ends first goes with positions x rows x kv heads, and 24 rows leave the
+        // wide tiles too empty.  Measured, narrow and wide, in us:
+        //   8 bits  head dim 128, 32 kv heads: 32 rows x 2000  36.7 36.6, 48 x 1000  36.9 37.6, 64 x 1000
+        //           45 43, 64 x 4000  81 65, 24 x 4000  38 47; 8 kv heads: 32 x 4000  16.6 20.1, 48 x 4000
+        //           24 22; head dim 64, 4 kv heads: 256 x 500  15.1 15.7, 192 x 1000  14.1 14.4, 256 x 1000
+        //           17 14, 128 x 1000  13.7 14.3, 32 x 1000  8.2 12.5
+        //   fp32    head dim 128, 32 kv heads: 16 x 4000  56 66, 24 x 4000  88 67, 24 x 1000  31 33, 32 x
+        //           1000  42 37; head dim 64, 4 kv heads: 128 x 1000  16 19, 192 x 1000  23 19
+        const long long work = c->n_kv * rows * pre;
+        x.wide = c->format == KLLM_KV_F32 ? rows >= 24 && work >= 1000000
+                                          : rows >= 32 && work >= 12000ll * c->head_dim;
         // fp32 tiles are read once per tile: eight rows as soon as there are more than four (24 rows x 4000
         // as above: 89 us, 95 in tiles of four)
         x.nb_pre = c->format == KLLM_KV_F32 ? (rows > 4 ? 2 : 1) : x.nb;

@@ -202,3 +202,98 @@ def test_same_bits_again_and_in_a_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(o, w)
+
+
+# The prefix's tiles of 128 rows: enough positions x rows x kv heads, rows and
+# positions that end inside a tile.
+WIDE = [(128, 8, 2, 64, 3001), (128, 4, 4, 129, 3000), (64, 8, 1, 41, 2500), (64, 8, 8, 33, 4100),
+        (32, 8, 2, 35, 3700), (128, 8, 1, 37, 5300)]
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", WIDE)
+def test_128_row_tiles(gpu, fmt, hd, nh, nkv, n, P):
+    lens = np.arange(n) % 9 - (np.arange(n) % 13 == 5)
+    _check(fmt, nh, nkv, hd, n, P, lens, 8, n + P)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("kscale", [1e-6, 30.0])
+def test_128_row_tiles_magnitudes(gpu, fmt, kscale):
+    def scales(n):
+        return np.float32(2.0) ** (np.arange(n) * 7 % 41 - 20).astype(np.float32)[:, None]
+    _check(fmt, 8, 2, 64, 50, 2700, [3] * 50, 3, 6, kscale=kscale, vscale=scales, qpad=3)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("n,P", [(50, 2700), (5, 300)])
+def test_rows_spoil_only_what_sees_them(gpu, fmt, n, P):
+    """Queries of NaN and infinities, one position of a kv head with NaN: the
+    other rows and heads keep their bits."""
+    import torch
+
+    import servecases as S
+    rng = np.random.default_rng(14)
+    nh, nkv, hd = 8, 2, 64
+    pre, own = S.Cache(fmt, 1, nkv, P, hd), S.Cache(fmt, n, nkv, 16, hd)
+    for c, m, s in ((pre, P, 1), (own, 16, n)):
+        c.put("k", rng.standard_normal((s, nkv, m, hd)).astype(np.float32))
+        c.put("v", rng.standard_normal((s, nkv, m, hd)).astype(np.float32))
+    q = rng.standard_normal((n, nh * hd)).astype(np.float32)
+    lens = S.dev(np.full(n, 16, np.int32))
+    a, b, d = (torch.zeros(n, nh * hd, device="cuda") for _ in "abd")
+    S.run_attention(S.dev(q), a, nh, 0.125, pre, P, own, lens, 16)
+    q[1], q[3, :hd], q[4, hd:2 * hd] = np.nan, np.inf, -np.inf
+    S.run_attention(S.dev(q), b, nh, 0.125, pre, P, own, lens, 16)
+    at = P - 2                                          # of kv head 0
+    if fmt == "f32":
+        pre.v.view(-1)[at * hd:(at + 1) * hd] = float("nan")
+    else:
+        pre.vs.view(-1)[at] = float("nan")
+    S.run_attention(S.dev(q), d, nh, 0.125, pre, P, own, lens, 16)
+    a, b, d = (t.cpu().numpy().reshape(n, nh, hd) for t in (a, b, d))
+    spoilt = np.zeros((n, nh), bool)
+    spoilt[1] = spoilt[3, 0] = spoilt[4, 1] = True
+    assert np.isnan(b[spoilt]).all() and np.array_equal(a[~spoilt], b[~spoilt])
+    spoilt[:, :nh // nkv] = True
+    assert np.isnan(d[spoilt]).all() and np.array_equal(a[~spoilt], d[~spoilt])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "f32"])
+def test_two_calls_at_once(gpu, fmt):
+    """Two streams, each with its own workspace, over the same prefix."""
+    import torch
+
+    import kmap_b200 as K
+    import servecases as S
+    rng = np.random.default_rng(18)
+    nh, nkv, hd, n, P, mp = 8, 2, 128, 64, 3100, 300
+    pre = S.Cache(fmt, 1, nkv, P, hd)
+    pre.put("k", rng.standard_normal((1, nkv, P, hd)).astype(np.float32))
+    pre.put("v", rng.standard_normal((1, nkv, P, hd)).astype(np.float32))
+    calls = []
+    for _ in range(2):
+        own = S.Cache(fmt, n, nkv, mp, hd)
+        own.put("k", rng.standard_normal((n, nkv, mp, hd)).astype(np.float32))
+        own.put("v", rng.standard_normal((n, nkv, mp, hd)).astype(np.float32))
+        q = S.dev(rng.standard_normal((n, nh * hd)).astype(np.float32))
+        lens = S.dev(rng.integers(0, mp + 1, n).astype(np.int32))
+        o = torch.zeros(n, nh * hd, device="cuda")
+        a = K.BatchAttn(n, nh, P, mp, 0.1, q.data_ptr(), nh * hd, C.addressof(pre.c), C.addressof(own.c),
+                        lens.data_ptr(), o.data_ptr(), nh * hd, None, 0)
+        size = K.lib().kllm_batch_attention_workspace(C.byref(a))
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), size
+        stream = torch.cuda.Stream()
+        K.check(K.lib().kllm_batch_attention(C.byref(a), stream.cuda_stream))
+        torch.cuda.synchronize()
+        calls.append((a, stream, o, o.clone(), (own, q, lens, ws)))
+    for a, stream, o, want, _ in calls:
+        o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for a, stream, *_ in calls:
+            K.check(K.lib().kllm_batch_attention(C.byref(a), stream.cuda_stream))
+    torch.cuda.synchronize()
+    for a, stream, o, want, _ in calls:
+        assert torch.equal(o, want)
