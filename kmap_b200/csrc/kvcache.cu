@@ -251,8 +251,12 @@ template <int HD, int FMT>
 bool append_launch(cudaStream_t s, const KvAppend &a, bool vec) {
     const int heads = a.r.n_heads + 2 * a.c.n_kv, per = KV_THREADS / 32 * (128 / HD);
     // few rows: as many warps as there are head rows (latency); many rows:
-    // four head rows' loads in flight per warp, the angles loaded once for them
-    if ((long long)a.r.rows * heads <= 148ll * 8 * per) {
+    // four head rows' loads in flight per warp, the angles loaded once for
+    // them.  Append and read together, one and four, in us: 96 head rows of
+    // 128 (8 bits), 32 rows 4.8 5.4, 64 rows 6.4 5.8, 1000 rows 45 26; 48 of
+    // 128 (fp32), 64 rows 4.2 4.4, 200 rows 5.7 5.1; 40 of 64 (8 bits), 200
+    // rows 5.0 5.2, 400 rows 6.2 5.5.
+    if ((long long)a.r.rows * heads <= 148ll * 4 * per) {
         k_kv_append<HD, FMT, 1><<<dim3(a.r.rows, (heads + per - 1) / per), KV_THREADS, 0, s>>>(
             a.c, a.r, a.nz, a.plane, vec);
     } else {
@@ -268,7 +272,7 @@ bool read_launch(cudaStream_t s, const kllm_kv_cache &c, int rows, const int *se
                  int pos0, float *k, float *v, long long row_stride, long long head_stride,
                  bool vec) {
     const int heads = 2 * c.n_kv, per = KV_THREADS / 32 * (128 / HD);
-    if ((long long)rows * heads <= 148ll * 8 * per)
+    if ((long long)rows * heads <= 148ll * 4 * per)      // (as append_launch)
         k_kv_read<HD, FMT, 1><<<dim3(rows, (heads + per - 1) / per), KV_THREADS, 0, s>>>(
             c, seq, pos, pos0, k, v, row_stride, head_stride, vec);
     else
