@@ -284,6 +284,10 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  *   own_len[i] < 0      a padding row: out[i] is left as it was
  *   own_len[i] > own->max_pos or max_len: the smaller of those is taken
  *   no position at all  out[i] is zeros
+ * A row of q that holds an infinity or a NaN gets NaN, and so does every row
+ * that sees a position whose fp32 key or value is not finite, or whose scale
+ * is NaN; no other row changes by it.  fp32 keys and values are taken to 22 bits, q and
+ * p to 22.
  * max_len is an upper bound of the own lengths (it sizes the launch, so a
  * captured graph serves every length up to it).  Positions past the lengths
  * are not read.  workspace: kllm_batch_attention_workspace(a) bytes on 16

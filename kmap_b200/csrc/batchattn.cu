@@ -16,8 +16,6 @@
 // p's fp16 terms stay in range whatever the scales are.
 #include <algorithm>
 #include <mutex>
-#include <set>
-#include <utility>
 
 #include "batchattn.cuh"
 #include "batchattn_tc.cuh"
@@ -682,16 +680,17 @@ bool ba_ok(const char *who, const kllm_batch_attn *a) {
 }
 
 // A kernel's shared-memory limit, raised once per device.
-bool ba_prepare(const void *kernel, size_t smem) {
+template <auto KERNEL>
+bool ba_prepare(size_t smem) {
     static std::mutex mu;
-    static std::set<std::pair<int, const void *>> done;
+    static bool ready[64] = {};
     int dev = 0;
     if (!KLLM_CUDA(cudaGetDevice(&dev))) return false;
     std::lock_guard<std::mutex> lk(mu);
-    if (done.count({dev, kernel})) return true;
-    if (!KLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
+    if (dev < 64 && ready[dev]) return true;
+    if (!KLLM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
         return false;
-    done.insert({dev, kernel});
+    if (dev < 64) ready[dev] = true;
     return true;
 }
 
@@ -756,19 +755,21 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
         return KLLM_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     };
     if (x.wide) {
-        auto kernel = k_ba_prefix<HD, FMT>;
         constexpr size_t smem = bt_smem<HD, FMT>();
-        if (!ba_prepare(reinterpret_cast<const void *>(kernel), smem) ||
-            !launch(kernel, (unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
+        if (!ba_prepare<k_ba_prefix<HD, FMT>>(smem) ||
+            !launch(k_ba_prefix<HD, FMT>, (unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
             return false;
     }
     auto part = [&](long long pre, long long own) {
-        const int nb = pre ? x.nb_pre : x.nb;
-        auto kernel = nb == 1 ? k_ba_part<HD, FMT, 1> : k_ba_part<HD, FMT, 2>;
         using G = BaRing<HD, FMT>;
+        if (pre + own == 0) return true;
         k.blocks_pre = (int)pre;
-        return pre + own == 0 || (ba_prepare(reinterpret_cast<const void *>(kernel), G::SMEM) &&
-                                  launch(kernel, (unsigned)(pre + own), 32 * G::WARPS, G::SMEM, k));
+        auto go = [&](auto nb) {
+            constexpr auto kernel = k_ba_part<HD, FMT, decltype(nb)::value>;
+            return ba_prepare<kernel>(G::SMEM) && launch(kernel, (unsigned)(pre + own), 32 * G::WARPS, G::SMEM, k);
+        };
+        return (pre ? x.nb_pre : x.nb) == 1 ? go(std::integral_constant<int, 1>())
+                                            : go(std::integral_constant<int, 2>());
     };
     const long long narrow = x.wide ? 0 : pre_blocks;
     if (x.join || x.nb != x.nb_pre ? !part(narrow, 0) || !part(0, own_blocks) : !part(narrow, own_blocks)) return false;

@@ -227,9 +227,10 @@ def test_128_row_tiles_magnitudes(gpu, fmt, kscale):
 
 @pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
 @pytest.mark.parametrize("n,P", [(50, 2700), (5, 300)])
-def test_rows_spoil_only_what_sees_them(gpu, fmt, n, P):
-    """Queries of NaN and infinities, one position of a kv head with NaN: the
-    other rows and heads keep their bits."""
+@pytest.mark.parametrize("what,bad", [("v", "nan"), ("k", "nan"), ("v", "inf"), ("k", "-inf")])
+def test_rows_spoil_only_what_sees_them(gpu, fmt, n, P, what, bad):
+    """Queries of NaN and infinities, one position of a kv head that is not
+    finite: the other rows and heads keep their bits."""
     import torch
 
     import servecases as S
@@ -247,9 +248,9 @@ def test_rows_spoil_only_what_sees_them(gpu, fmt, n, P):
     S.run_attention(S.dev(q), b, nh, 0.125, pre, P, own, lens, 16)
     at = P - 2                                          # of kv head 0
     if fmt == "f32":
-        pre.v.view(-1)[at * hd:(at + 1) * hd] = float("nan")
+        getattr(pre, what).view(-1)[at * hd:(at + 1) * hd] = float(bad)
     else:
-        pre.vs.view(-1)[at] = float("nan")
+        getattr(pre, what + "s").view(-1)[at] = float("nan")
     S.run_attention(S.dev(q), d, nh, 0.125, pre, P, own, lens, 16)
     a, b, d = (t.cpu().numpy().reshape(n, nh, hd) for t in (a, b, d))
     spoilt = np.zeros((n, nh), bool)
