@@ -895,8 +895,15 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
 }  // namespace
 
 bool sample_rows(cudaStream_t s, const kllm_sample_rows &r, int nz, long long plane) {
+    // A row's blocks: at least 2048 tokens each (1 row of 1000 tokens: 13.2 us with one, 16.1 with eight;
+    // of 16000: 19.5, 16.6 with two, 15.7 with four, 16.5 with eight), and fewer where all rows' are more
+    // than one an SM, a block's fixed work being that of some 2000 tokens (128 rows of 32000: 81 us with
+    // one, 38 with two, 47 with four, 68 with eight; 32 rows: 64, 35, 26, 29), but slices of 64 KB at
+    // most, three an SM (128 rows of 128256: 128 us with eight, 172 with four).
     int C = SA_CL;
     while (C > 1 && r.vocab <= C * 2048) C /= 2;
+    auto cost = [&](int c) { return std::max(148ll, (long long)r.rows * c) * (2000 + r.vocab / c); };
+    while (C > 1 && r.vocab / (C / 2) <= 16384 && cost(C / 2) < cost(C)) C /= 2;
     const int per = ((r.vocab + C - 1) / C + 3) / 4 * 4;
     const int wper = ((per + SA_WARPS - 1) / SA_WARPS + 127) / 128 * 128;
     const size_t slice = (size_t)wper * SA_WARPS * 4;

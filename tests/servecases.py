@@ -164,15 +164,20 @@ def sample_plain(x, T, k, p, mp, u):
     return int(kept[min(int((c <= u * c[-1]).sum()), n - 1)])
 
 
-def run_sample(x, T=None, k=None, p=None, mp=None, u=None, vocab=None, stream=None):
-    """kllm_sample on rows x (device tensor [rows][stride])."""
+def sample_args(x, T=None, k=None, p=None, mp=None, u=None, vocab=None):
+    """kllm_sample's arguments for rows x (device tensor [rows][stride]), the
+    tokens (one more than there are) and what they point to."""
     rows = x.shape[0]
     t = [None if a is None else dev(np.asarray(a, d)) for a, d in
          ((T, np.float32), (k, np.int32), (p, np.float32), (mp, np.float32), (u, np.float32))]
     out = torch.full((rows + 1,), -7, dtype=torch.int32, device=DEV)
     ptr = [None if a is None else a.data_ptr() for a in t]
-    a = K.SampleRows(rows, vocab or x.shape[1], x.data_ptr(), x.stride(0), *ptr, out.data_ptr())
+    return K.SampleRows(rows, vocab or x.shape[1], x.data_ptr(), x.stride(0), *ptr, out.data_ptr()), out, t
+
+
+def run_sample(x, *settings, vocab=None, stream=None, **named):
+    a, out, _keep = sample_args(x, *settings, vocab=vocab, **named)
     K.check(K.lib().kllm_sample(C.byref(a), stream), "kllm_sample")
     torch.cuda.synchronize()
-    assert int(out[rows]) == -7
-    return out[:rows].cpu().numpy()
+    assert int(out[-1]) == -7
+    return out[:-1].cpu().numpy()

@@ -298,3 +298,30 @@ def test_two_calls_at_once(gpu, fmt):
     torch.cuda.synchronize()
     for a, stream, o, want, _ in calls:
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_prefix_past_32_bits(gpu, n):
+    """2^31 codes of keys and of values: every weight is one, the last
+    position alone has a value.  Its share is exact but for the tolerance
+    above (S = 0)."""
+    import torch
+
+    import kmap_b200 as K
+    import servecases as S
+    nkv, hd, mp = 8, 128, (1 << 21) + 77
+    codes = torch.zeros(2, nkv, mp, hd, dtype=torch.uint8, device="cuda")
+    codes[1, :, mp - 1] = torch.arange(1, 1 + hd, device="cuda", dtype=torch.uint8).clamp(max=127)
+    scales = torch.ones(nkv, mp, device="cuda")
+    c = K.KvCache(S.FORMATS["i8"], 1, nkv, hd, mp, codes[0].data_ptr(), codes[1].data_ptr(), scales.data_ptr(),
+                  scales.data_ptr(), nkv * mp * hd, nkv * mp)
+
+    class Prefix:
+        pass
+    pre = Prefix()
+    pre.c = c
+    q, out = torch.ones(n, nkv * hd, device="cuda"), torch.zeros(n, nkv * hd, device="cuda")
+    S.run_attention(q, out, nkv, 1.0, pre, mp)
+    want = np.minimum(np.arange(1, 1 + hd), 127) / mp
+    got = out.cpu().numpy().astype(np.float64).reshape(n, nkv, hd)
+    assert (np.abs(got - want) <= 4 * 2.0 ** -18 * want).all()

@@ -151,3 +151,68 @@ def test_nothing_to_do(gpu):
     K.check(K.lib().kllm_kv_append(cache.by(), C.byref(r), None))
     K.check(K.lib().kllm_kv_read(cache.by(), 0, None, None, 0, 16, 16, 32, 32, None))
     assert K.lib().kllm_launch_count() == n
+
+
+@pytest.mark.parametrize("fmt", ["i8", "f32"])
+def test_in_a_graph(gpu, fmt):
+    """A captured append, replayed with new rows and positions, on another stream."""
+    import torch
+
+    import kmap_b200 as K
+    import servecases as S
+    rng = np.random.default_rng(3)
+    n, nkv, hd, mp = 5, 2, 64, 40
+    x = [rng.standard_normal((n, 2 * nkv, hd)).astype(np.float32) for _ in range(3)]
+    at = [rng.permutation(mp)[:n].astype(np.int32) for _ in range(3)]
+    a, b = S.Cache(fmt, n, nkv, mp, hd), S.Cache(fmt, n, nkv, mp, hd)
+    dx, dp = S.dev(x[0]), S.dev(at[0])
+
+    def call(cache, stream):
+        r = K.KvRows(n, 0, 0, 0, 0, None, dp.data_ptr(), None, dx.data_ptr(), dx.data_ptr() + 4 * nkv * hd,
+                     2 * nkv * hd, hd)
+        K.check(K.lib().kllm_kv_append(cache.by(), C.byref(r), stream))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        call(a, torch.cuda.current_stream().cuda_stream)
+    for xi, pi in zip(x, at):
+        dx.copy_(S.dev(xi))
+        dp.copy_(S.dev(pi))
+        graph.replay()
+        call(b, None)
+        torch.cuda.synchronize()
+    for t in ("k", "v", "ks", "vs"):
+        assert torch.equal(getattr(a, t).nan_to_num(), getattr(b, t).nan_to_num())
+        assert fmt == "f32" and t[1:] or bool((getattr(a, t).nan_to_num() != 0).any())
+
+
+def test_sequences_more_than_32_bits_apart(gpu):
+    """Sequences 2^31 codes apart: written, read and attended as those of a small cache."""
+    import torch
+
+    import kmap_b200 as K
+    import servecases as S
+    rng = np.random.default_rng(9)
+    nkv, hd, mp, n = 2, 128, 16, 2
+    x = S.dev(rng.standard_normal((n, 2 * nkv, hd)).astype(np.float32))
+    q = S.dev(rng.standard_normal((n, 2 * nkv * hd)).astype(np.float32))
+    seq, lens = S.dev(np.array([1, 0], np.int32)), S.dev(np.array([3, 3], np.int32))
+    pos = S.dev(np.array([2, 2], np.int32))
+    got = []
+    for pad in (0, 2 ** 31 + 64):
+        c = S.Cache("i8", n, nkv, mp, hd)
+        c.stride += pad
+        c.k, c.v = (torch.zeros(c.stride + nkv * mp * hd, dtype=torch.uint8, device="cuda") for _ in "kv")
+        c.ks.zero_(), c.vs.zero_()
+        c.c.k, c.c.v, c.c.seq_stride = c.k.data_ptr(), c.v.data_ptr(), c.stride
+        r = K.KvRows(n, 0, 0, 0, 0, seq.data_ptr(), pos.data_ptr(), None, x.data_ptr(),
+                     x.data_ptr() + 4 * nkv * hd, 2 * nkv * hd, hd)
+        K.check(K.lib().kllm_kv_append(c.by(), C.byref(r), None))
+        back = torch.zeros(2, n, nkv, hd, device="cuda")
+        K.check(K.lib().kllm_kv_read(c.by(), n, seq.data_ptr(), pos.data_ptr(), 0, back[0].data_ptr(),
+                                     back[1].data_ptr(), nkv * hd, hd, None))
+        out = torch.zeros(n, 2 * nkv * hd, device="cuda")
+        S.run_attention(q, out, 2 * nkv, 0.1, own=c, lens=lens, max_len=mp)
+        got.append((back, out))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert bool((got[0][0] != 0).any(-1).all()) and bool((got[0][1] != 0).any(-1).all())

@@ -172,3 +172,40 @@ def test_in_a_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert out.tolist() == _want(x, None, None, np.full(16, np.float32(0.9)), None, u)
+
+
+@pytest.mark.parametrize("V", [7000, 16000, 33000])
+@pytest.mark.parametrize("rows", [40, 160])
+def test_many_rows_and_their_split(gpu, V, rows):
+    """Rows take fewer blocks each where there are many: the tokens are those
+    of a row alone, and of the definition."""
+    import servecases as S
+    rng = np.random.default_rng(V + rows)
+    x = _logits(rng, rows, V, "ties" if rows == 40 else "bulk")
+    T, k, p, mp, u = _settings(rng, rows)
+    k[::2] = 0
+    got = S.run_sample(S.dev(x), T, k, p, mp, u).tolist()
+    assert got[:12] == _want(x[:12], T[:12], k[:12], p[:12], mp[:12], u[:12])
+    for i in range(0, rows, 7):
+        s = slice(i, i + 1)
+        assert S.run_sample(S.dev(x[s]), T[s], k[s], p[s], mp[s], u[s]).tolist() == got[s], i
+
+
+def test_two_calls_at_once(gpu):
+    import torch
+
+    import servecases as S
+    rng = np.random.default_rng(77)
+    x = [S.dev(_logits(rng, 16, 128256, "bulk")) for _ in "ab"]
+    T, k, p, mp, u = _settings(rng, 16)
+    k[:] = 0
+    want = [S.run_sample(t, T, k, p, mp, u).tolist() for t in x]
+    streams = [torch.cuda.Stream() for _ in "ab"]
+    a = [S.sample_args(t, T, k, p, mp, u) for t in x]
+    torch.cuda.synchronize()
+    import kmap_b200 as K
+    for _ in range(5):
+        for args, s in zip(a, streams):
+            K.check(K.lib().kllm_sample(C.byref(args[0]), s.cuda_stream))
+    torch.cuda.synchronize()
+    assert [args[1][:-1].cpu().tolist() for args in a] == want
