@@ -4,8 +4,10 @@
 //
 // Both are cut into ranges of positions ("parts"); a part's block leaves its
 // running maximum m, its sum l and its unnormalised sum of p v per query
-// row, and k_ba_merge joins a row's parts:
+// row, and a row's parts are joined by the block of its own positions (where
+// they are one part) or by k_ba_merge:
 //     M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
+// k_ba_part takes four or eight query rows; batchattn_tc.cuh 128, of a prefix.
 //
 // Products of fp32 queries and weights run on the tensor cores without
 // losing them to 16 bits: a row of q (and of p) is split into two terms,
@@ -630,8 +632,14 @@ BaCut ba_cut(const kllm_batch_attn &a) {
     if (x.own_cap > 0) {
         x.tiles_own = (groups + tile - 1) / tile;
         const long long items = (long long)a.n_seq * c->n_kv * x.tiles_own;
-        if (x.own_cap <= 256 || (x.own_cap <= 1024 && items >= 296)) {
-            // short, or as many items as blocks at a time: one part, and no launch for the join
+        // One part, joined where it is computed (no launch for the join), where a block's keys are few, or
+        // the blocks as many as they are KB: measured, more parts and one, in us, after 64 positions of a
+        // prefix: head dim 128, 8 kv heads of 8 bits, 512 positions: 1 sequence 7.8 8.7, 8 sequences 10.1
+        // 9.3, 48 20 17; 1000: 8 sequences 11.8 12.4, 16 15.0 12.2; 128: 1 sequence 6.5 6.2; 32 kv heads of
+        // fp32, 64: 6.9 6.3; 256: 1 sequence 9.0 11.4, 8 19.6 13.7; 1000: 4 20 34, 16 55 55.  Above 1024
+        // positions lengths differ enough for parts to even them out.
+        const long long kb = (long long)x.own_cap * c->head_dim * (c->format == KLLM_KV_F32 ? 4 : 1) / 1024;
+        if (kb <= 32 || (x.own_cap <= 1024 && items >= kb)) {
             x.parts_own = 1;
             x.chunk_own = x.own_cap;
             x.join = true;

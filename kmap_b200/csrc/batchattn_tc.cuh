@@ -14,20 +14,29 @@
 // tile's value scale come in.
 //
 // Warps: two groups of four that take the tiles' softmax in turn (a row per
-// thread) and each keep half of O's columns; four (fp32: eight) that bring
-// keys and values from global memory to fp16 operands in shared memory (the
-// next tile's loads in flight in registers); one that issues the products.
+// thread) and each keep half of O's columns; four that bring keys and values
+// from global memory to fp16 operands in shared memory, the next tile's loads
+// in flight in registers (fp32: four for keys and four for values, the next
+// tile's copies in flight in shared memory, since two terms to make of each
+// number leave no time to wait); one that issues the products.  Warps whose
+// rows lie behind the last leave their part of a tile alone.
 // A tile's weights are relative to the tile's own maximum, so that the two
 // groups need nothing of one another; the running maximum is applied where O
-// is added up.  Keys and values (8 bits), S/P and O have two buffers each; S of the next
-// tile is issued before P.V of this one, so that the tensor cores work while
-// the softmax does.  Every wait is bounded; one that gives up leaves NaN in
-// the part's sums.
+// is added up.  S/P and O have two buffers each, keys and values two (8 bits)
+// or one; S of the next tile is issued before P.V of this one, so that the
+// tensor cores work while the softmax does.  Every wait is bounded; one that
+// gives up leaves NaN in the part's sums.
 //
-// Bound: products.  With two terms a tile of 128 positions of 8 bits takes
-// 16.8 MFLOP, 1.5 us at the tensor cores' rate, where its bytes take 0.8 us
-// of an SM's share of the memory's; fp32 tiles take three products (25
-// MFLOP, 2.3 us per 128 positions) against 2.9 us of bytes.
+// Bound: of a tile of 128 positions of 8 bits (16.8 MFLOP with two terms) the
+// products take some 2900 cycles, the bytes 1600 of an SM's share of the
+// memory's; a tile takes 5700, in the softmax's shared-memory reads (scales,
+// the same for all lanes) and tensor-memory loads and stores.  256 rows x
+// 16384 positions of 8 kv heads of 128, e4m3, two tiles of rows: 77 us in all
+// (17.2 GFLOP: 0.22 PFLOP/s, 0.45 as issued in two terms).  An fp32 tile of
+// 64 positions takes 5700 cycles too: its keys' conversion and the three
+// products of its scores follow one another (one buffer of keys: two, with the
+// queries in tensor memory, measured the same).  24 rows x 4000 positions of
+// 32 kv heads of 128, fp32: 55 us (131 MB, 2.4 TB/s).
 #pragma once
 
 #include "batchattn.cuh"

