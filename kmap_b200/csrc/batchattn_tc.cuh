@@ -29,8 +29,12 @@
 //
 // Bound: of a tile of 128 positions of 8 bits (16.8 MFLOP with two terms) the
 // products take some 2900 cycles, the bytes 1600 of an SM's share of the
-// memory's; a tile takes 5700, in the softmax's shared-memory reads (scales,
-// the same for all lanes) and tensor-memory loads and stores.  256 rows x
+// memory's; a tile takes 5700: of the two groups' 11400 each, 1400 are the
+// maxima's, 4800 the weights', 1200 O's, the rest waiting for products that
+// wait for weights.  Taking the weights four rows a lane (a quarter of the
+// scales' reads), their first terms without a conversion back, or their loads
+// a step ahead measured the same 79 us as below; 16 softmax warps 109 (80
+// registers).  256 rows x
 // 16384 positions of 8 kv heads of 128, e4m3, two tiles of rows: 77 us in all
 // (17.2 GFLOP: 0.22 PFLOP/s, 0.45 as issued in two terms).  An fp32 tile of
 // 64 positions takes 5700 cycles too: its keys' conversion and the three
