@@ -159,8 +159,16 @@ struct SaKept {
 struct SaScale {
     float m, unit;
     int q_bits;
-    double md, lt;
+    double md, mw, lt;      // the maximum, wide(it), log2(e) / T in wide's units
     const uint32_t *tab;    // sa_tab in shared memory
+
+    // A float times 2^-896, exactly: its exponent and fraction bits in a double's place, where zero and
+    // the subnormals are what they were too (a double's conversion from a float is slow).  -infinity
+    // becomes -2^128 times that.
+    static __device__ __forceinline__ double wide(float x) {
+        const uint32_t b = __float_as_uint(x);
+        return __hiloint2double((int)(((b & 0x7fffffffu) >> 3) | (b & 0x80000000u)), (int)(b << 29));
+    }
 
     // Distance to the maximum in units.
     __device__ __forceinline__ float dist(float x) const { return (m - x) * unit; }
@@ -174,12 +182,7 @@ struct SaScale {
     // (relative error below 2^-29); the shift by n and the rounding are one addition of 2^52.
     // No branch: several tokens' chains overlap.
     __device__ __forceinline__ u64 weight(float x) const {
-        // the float's bits as a double's (what is below 2^-126 becomes some number below it,
-        // -infinity becomes -2^128)
-        const uint32_t b = __float_as_uint(x);
-        const double xd = __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)),
-                                           (int)(b << 29));
-        const double y = fma(md - xd, lt, 0x1.8p20);
+        const double y = fma(mw - wide(x), lt, 0x1.8p20);
         const uint32_t n = min((uint32_t)__double2hiint(y) - 0x41380000u, 63u);
         const uint32_t lo = (uint32_t)__double2loint(y), z = lo & 0x07ffffffu, t = tab[lo >> 27];
         uint32_t q = 0x3d7f23e8u - __umulhi(z, 0x0e181d25u);
@@ -596,9 +599,11 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
         return;     // the last barrier is behind every remote access
     }
     sc.md = (double)sc.m;
-    sc.lt = 1.4426950408889634 / (double)(T == T ? fminf(fmaxf(T, 1e-30f), 1e30f) : 1.f);
+    sc.mw = SaScale::wide(sc.m);
+    const double lt = 1.4426950408889634 / (double)(T == T ? fminf(fmaxf(T, 1e-30f), 1e30f) : 1.f);
+    sc.lt = lt * 0x1p896;
     sc.q_bits = q_bits;
-    sc.unit = (float)(sc.lt * (double)(SA_BINS << q_bits) / (double)SA_OCTAVES);
+    sc.unit = (float)(lt * (double)(SA_BINS << q_bits) / (double)SA_OCTAVES);
     const float f_all = sc.units(SA_BINS);      // weights are zero from here on
     // min-p: a bound on the weight, which the largest always meets
     u64 wmin = 1;

@@ -1,0 +1,47 @@
+"""Ends of kllm_sample's range: rows whose largest logit is a zero or a
+subnormal number, at the lowest temperatures.  Tokens are compared for equality
+with the definition in 64 bits, temperatures taken into [1e-30, 1e30] as the
+header has it; no number lies within 2^-24 of a border."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+SUB = np.float32(1e-40)     # a subnormal number
+
+
+def _tops(V, rng):
+    """Rows by their largest logit: zeros of either sign, subnormals, alone and many."""
+    below = -np.abs(rng.standard_normal((8, V))).astype(np.float32) - np.float32(0.5)
+    x = below.copy()
+    at = rng.integers(0, V, 8)
+    x[0, at[0]] = 0.0                              # shifted by its maximum
+    x[1, at[1]] = -0.0
+    x[2, at[2]] = SUB
+    x[3] = 0.0                                     # equal ones
+    x[4] = -0.0
+    x[5] = SUB
+    x[6] = np.where(rng.random(V) < 0.5, np.float32(0.0), np.float32(-0.0))
+    x[7] = np.where(rng.random(V) < 0.5, SUB, np.float32(0.0))
+    return x
+
+
+def _check(x, T, k, p, mp, u):
+    import servecases as S
+    n = len(x)
+    full = lambda a, d, t: None if a is None else np.full(n, a, t)
+    Tc = min(max(float(np.float32(T)), float(np.float32(1e-30))), float(np.float32(1e30)))
+    got = S.run_sample(S.dev(x), np.full(n, T, np.float32), full(k, 0, np.int32), full(p, 1, np.float32),
+                       full(mp, 0, np.float32), u)
+    want = [S.sample_plain(r, Tc, k or 0, 1.0 if p is None else float(np.float32(p)),
+                           0.0 if mp is None else float(np.float32(mp)), float(u[i])) for i, r in enumerate(x)]
+    assert got.tolist() == want, (T, k, p, mp)
+
+
+@pytest.mark.parametrize("V", [3, 700, 5000, 40001])
+@pytest.mark.parametrize("T", [1e-38, 1e-30, 5e-29, 7.2e-29, 1e-28, 1e-10, 1.0])
+@pytest.mark.parametrize("k,p,mp", [(None, None, None), (2, None, None), (600, None, None), (None, 0.7, None),
+                                    (650, 0.9, None), (None, None, 0.5), (20, 0.5, 0.1)])
+def test_largest_logit_of_zero_or_subnormal(gpu, V, T, k, p, mp):
+    rng = np.random.default_rng(V)
+    _check(_tops(V, rng), T, k, p, mp, rng.random(8).astype(np.float32))
