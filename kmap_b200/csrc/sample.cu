@@ -330,7 +330,7 @@ __device__ SaKept sa_narrow(cg::cluster_group &cl, SaShared &sh, const SaScale &
                 near[e] = in[e] && t >= flo && t < fhi;
                 if (MASS) {
                     u64 w = sc.weight(x[e]);
-                    if (limited && !in[e]) w = 0;
+                    if (!in[e]) w = 0;      // (-infinity's is not zero at every temperature)
                     all_mass += w;
                     if (t < flo) a += w;
                 }
@@ -723,7 +723,7 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
 #pragma unroll
                          for (int e = 0; e < 4; e++) {
                              near[e] = in[e] && sc.dist(x[e]) < fhi;
-                             if (mass) sum += sc.weight(x[e]);
+                             if (mass && in[e]) sum += sc.weight(x[e]);
                          }
                          if (!__any_sync(0xffffffffu, near[0] || near[1] || near[2] || near[3])) return;
                          sa_append(&sh.n_list, near, at);
@@ -767,7 +767,8 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
         }
     }
     // where the kept ties end: the index of the last of them
-    int icut = 0x7fffffff;
+    // (where nothing cuts, tau is -infinity and none of those is kept)
+    int icut = kept.tau == -INFINITY ? -1 : 0x7fffffff;
     if (kept.cut) {
         int n = 0;
         sl.each4([&](float x, int) { return x == kept.tau; },

@@ -1,7 +1,7 @@
-"""Ends of kllm_sample's range: rows whose largest logit is a zero or a
-subnormal number, at the lowest temperatures.  Tokens are compared for equality
-with the definition in 64 bits, temperatures taken into [1e-30, 1e30] as the
-header has it; no number lies within 2^-24 of a border."""
+"""Ends of kllm_sample's range: rows whose largest logit is a zero, a
+subnormal or the lowest number, at the ends of the temperatures.  Tokens are
+compared for equality with the definition in 64 bits, temperatures taken into
+[1e-30, 1e30] as the header has it; no number lies within 2^-24 of a border."""
 import numpy as np
 import pytest
 
@@ -45,3 +45,23 @@ def _check(x, T, k, p, mp, u):
 def test_largest_logit_of_zero_or_subnormal(gpu, V, T, k, p, mp):
     rng = np.random.default_rng(V)
     _check(_tops(V, rng), T, k, p, mp, rng.random(8).astype(np.float32))
+
+
+@pytest.mark.parametrize("V", [600, 5000, 40001])
+@pytest.mark.parametrize("T", [1e28, 1e30])
+@pytest.mark.parametrize("k,p,mp", [(None, None, None), (3, None, None), (None, 0.6, None), (900, 0.9, None),
+                                    (None, None, 0.5)])
+def test_masked_tokens_beside_the_lowest_number(gpu, V, T, k, p, mp):
+    """-infinity weighs nothing, even where the largest logit is the type's lowest
+    number and the temperature so high that the distance to 2^128 is small."""
+    rng = np.random.default_rng(V)
+    low = np.finfo(np.float32).min
+    x = np.full((6, V), -np.inf, np.float32)
+    x[0, V // 2] = low
+    x[1, 1:] = low
+    x[2, 5::2] = low
+    x[3] = np.where(rng.random(V) < 0.2, low, -np.inf)
+    x[4, V - 3:] = low * np.float32(0.75)
+    x[5] = np.where(rng.random(V) < 0.2, low * rng.random(V).astype(np.float32), -np.inf)
+    for u in (0.0, 0.5, 0.999):
+        _check(x, T, k, p, mp, np.full(6, u, np.float32))
