@@ -518,6 +518,9 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
     extern __shared__ __align__(16) float cache[];
     __shared__ SaShared sh;
     cg::cluster_group cl = cg::this_cluster();
+    // (a block's shared memory is there for the others once it has started: waited for ahead of step 1's
+    // first access)
+    cl.barrier_arrive();
     const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
     const int r = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     SaSlice<CACHED> sl;
@@ -561,6 +564,7 @@ k_sample(const kllm_sample_rows a, int nz, long long plane, int per, int wper, i
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) sh.wlo[warp] = (double)top;
     __syncthreads();
+    cl.barrier_wait();
     if (tid < C) {
         double b = sh.wlo[0];
 #pragma unroll

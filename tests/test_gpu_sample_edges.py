@@ -65,3 +65,25 @@ def test_masked_tokens_beside_the_lowest_number(gpu, V, T, k, p, mp):
     x[5] = np.where(rng.random(V) < 0.2, low * rng.random(V).astype(np.float32), -np.inf)
     for u in (0.0, 0.5, 0.999):
         _check(x, T, k, p, mp, np.full(6, u, np.float32))
+
+
+def test_clusters_on_a_busy_gpu(gpu):
+    """A row's blocks start whenever the work beside them leaves room: the tokens stay."""
+    import ctypes as C
+
+    import kmap_b200 as K
+    import torch
+
+    import servecases as S
+    rng = np.random.default_rng(21)
+    x = S.dev(rng.standard_normal((96, 128256)).astype(np.float32))
+    p, u = np.full(96, 0.9, np.float32), rng.random(96).astype(np.float32)
+    want = S.run_sample(x, None, None, p, None, u).tolist()
+    outs = [S.sample_args(x, None, None, p, None, u) for _ in range(20)]
+    work, side = torch.randn(4096, 4096, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for a, _, _ in outs:
+        work @ work
+        K.check(K.lib().kllm_sample(C.byref(a), side.cuda_stream))
+    torch.cuda.synchronize()
+    assert [o[:-1].cpu().tolist() for _, o, _ in outs] == [want] * len(outs)
