@@ -25,7 +25,8 @@
 // is added up.  S/P and O have two buffers each, keys and values two (8 bits)
 // or one; S of the next tile is issued before P.V of this one, so that the
 // tensor cores work while the softmax does.  Every wait is bounded; one that
-// gives up leaves NaN in the part's sums.
+// gives up leaves NaN in the part's sums.  The issuing warp sees all of its
+// products end before the block gives its memory back, on that path too.
 //
 // Bound: of a tile of 128 positions of 8 bits (16.8 MFLOP with two terms) the
 // products take some 2900 cycles, the bytes 1600 of an SM's share of the
@@ -719,11 +720,12 @@ k_ba_prefix(const BaArgs a) {
         };
         // S of the next tile ahead of O of this one: the tensor cores work while the softmax does.
         bool ok = true;
+        int n_s = 0, n_o = 0;      // tiles whose scores, outputs were issued
         for (int t = 0; t <= nt && ok; t++) {
             if (t < nt) {
                 ok = bt_wait(&sh.k_full[t % G::ST], (t / G::ST) & 1, &sh.dead);
                 tc_fence_after();
-                if (ok) scores(t);
+                if (ok) scores(t), n_s++;
             }
             const int u = t - 1;
             if (u < 0 || !ok) continue;
@@ -731,8 +733,18 @@ k_ba_prefix(const BaArgs a) {
                  bt_wait(&sh.v_full[u % G::ST], (u / G::ST) & 1, &sh.dead) &&
                  (u < 2 || bt_wait(&sh.o_empty[u & 1], ((u / 2) & 1) ^ 1, &sh.dead));
             tc_fence_after();
-            if (ok) output(u);
+            if (ok) output(u), n_o++;
         }
+        // Products and their arrivals are over before the memory that they write is given back (they wait
+        // for nothing themselves, so this ends, given up or not).
+        auto drain = [](uint64_t *bar, int buffers, int n) {
+            for (int b = 0; b < buffers; b++)
+                if (n > b) mbar_wait(&bar[b], (n - b - 1) / buffers & 1, nullptr);
+        };
+        drain(sh.s_full, 2, n_s);
+        drain(sh.k_empty, G::ST, n_s);
+        drain(sh.o_full, 2, n_o);
+        drain(sh.v_empty, G::ST, n_o);
     }
     __syncwarp();
     tc_fence_before();
