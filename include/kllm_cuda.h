@@ -291,7 +291,8 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  * max_len is an upper bound of the own lengths (it sizes the launch, so a
  * captured graph serves every length up to it).  Positions past the lengths
  * are not read.  workspace: kllm_batch_attention_workspace(a) bytes on 16
- * bytes; calls that overlap on the GPU need one each. */
+ * bytes; calls that overlap on the GPU need one each.  Waits inside the call
+ * are bounded (2 s); should one give up, its rows are NaN. */
 typedef struct {
     int n_seq, n_heads;
     int prefix_len, max_len;

@@ -703,7 +703,8 @@ bool ba_prepare(size_t smem) {
 }
 
 template <int HD, int FMT>
-bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int terms, void *terms_out) {
+bool ba_launch(cudaStream_t s, const BatchAttention &call, const BaCut &x) {
+    const kllm_batch_attn &a = call.a;
     const kllm_kv_cache *c = a.prefix ? a.prefix : a.own;
     BaArgs k = {};
     auto side = [](const kllm_kv_cache *c, int parts, int chunk) {
@@ -735,8 +736,10 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
     k.join = x.join;
     k.out = a.out;
     k.out_stride = a.out_stride;
-    k.terms = terms;
-    k.terms_out = terms_out;
+    k.terms = call.terms;
+    k.terms_out = call.terms_out;
+    k.status = call.status;
+    k.wait_ns = call.wait_ns;
     const long long pre_blocks = (long long)k.nkv * x.tiles_pre * x.parts_pre;
     const long long own_blocks = (long long)a.n_seq * k.nkv * x.tiles_own * x.parts_own;
     if (pre_blocks + own_blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
@@ -787,15 +790,16 @@ bool ba_launch(cudaStream_t s, const kllm_batch_attn &a, const BaCut &x, int ter
 
 }  // namespace
 
-bool batch_attention(cudaStream_t s, const kllm_batch_attn &a, int terms, void *terms_out) {
+bool batch_attention(cudaStream_t s, const BatchAttention &b) {
     const char *who = "kllm_batch_attention";
+    const kllm_batch_attn &a = b.a;
     if (!ba_ok(who, &a)) return false;
-    if (!a.out && !terms_out) {
+    if (!a.out && !b.terms_out) {
         set_error("%s: invalid arguments", who);
         return false;
     }
     const kllm_kv_cache *c = a.prefix ? a.prefix : a.own;
-    if (!terms_out && a.n_seq > 1 && a.out_stride < (long long)a.n_heads * c->head_dim) {
+    if (!b.terms_out && a.n_seq > 1 && a.out_stride < (long long)a.n_heads * c->head_dim) {
         set_error("%s: out_stride %lld for %d heads of %d", who, a.out_stride, a.n_heads, c->head_dim);
         return false;
     }
@@ -807,9 +811,9 @@ bool batch_attention(cudaStream_t s, const kllm_batch_attn &a, int terms, void *
     }
     auto go = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        return c->format == KLLM_KV_F32 ? ba_launch<HD, KLLM_KV_F32>(s, a, x, terms, terms_out)
-             : c->format == KLLM_KV_I8  ? ba_launch<HD, KLLM_KV_I8>(s, a, x, terms, terms_out)
-                                        : ba_launch<HD, KLLM_KV_E4M3>(s, a, x, terms, terms_out);
+        return c->format == KLLM_KV_F32 ? ba_launch<HD, KLLM_KV_F32>(s, b, x)
+             : c->format == KLLM_KV_I8  ? ba_launch<HD, KLLM_KV_I8>(s, b, x)
+                                        : ba_launch<HD, KLLM_KV_E4M3>(s, b, x);
     };
     return c->head_dim == 32 ? go(std::integral_constant<int, 32>())
          : c->head_dim == 64 ? go(std::integral_constant<int, 64>())
@@ -829,5 +833,7 @@ extern "C" int kllm_batch_attention(const kllm_batch_attn *a, void *stream) {
         set_error("kllm_batch_attention: invalid arguments");
         return -1;
     }
-    return batch_attention((cudaStream_t)stream, *a, 0, nullptr) ? 0 : -1;
+    BatchAttention b;
+    b.a = *a;
+    return batch_attention((cudaStream_t)stream, b) ? 0 : -1;
 }

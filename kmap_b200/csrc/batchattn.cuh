@@ -35,6 +35,8 @@ struct BaArgs {
     long long out_stride;
     int terms;                  // as bd_emit
     void *terms_out;
+    int *status;                // gets ST_WAIT_TIMEOUT when a wait gives up (may be null)
+    unsigned long long wait_ns; // bound of each wait
 };
 
 __device__ __forceinline__ uint32_t ba_prmt(uint32_t a, uint32_t b, uint32_t sel) {

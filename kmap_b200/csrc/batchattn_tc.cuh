@@ -25,8 +25,9 @@
 // is added up.  S/P and O have two buffers each, keys and values two (8 bits)
 // or one; S of the next tile is issued before P.V of this one, so that the
 // tensor cores work while the softmax does.  Every wait is bounded; one that
-// gives up leaves NaN in the part's sums.  The issuing warp sees all of its
-// products end before the block gives its memory back, on that path too.
+// gives up leaves NaN in the part's sums and ST_WAIT_TIMEOUT in the status word
+// (where there is one).  The issuing warp sees all of its products end before
+// the block gives its memory back, on that path too.
 //
 // Bound: of a tile of 128 positions of 8 bits (16.8 MFLOP with two terms) the
 // products take some 2900 cycles, the bytes 1600 of an SM's share of the
@@ -90,17 +91,18 @@ constexpr size_t bt_smem() {
     return 1024 + BtGeom<HD, FMT>::END + sizeof(BtShared);
 }
 
-// Wait for phase `parity`; false when it, or another warp's wait, gave up.
-__device__ __forceinline__ bool bt_wait(uint64_t *bar, uint32_t parity, int *dead) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Wait for phase `parity`; false when it, or another warp's wait, gave up (with
+// a limit of 0, as soon as it would have to wait).
+__device__ __forceinline__ bool bt_wait(uint64_t *bar, uint32_t parity, int *dead, unsigned long long limit) {
+    if (limit ? mbar_try_wait(bar, parity) : mbar_test_wait(bar, parity)) return true;
     const unsigned long long t0 = globaltimer();
-    while (!mbar_try_wait(bar, parity)) {
+    do {
         if (*(volatile int *)dead) return false;
-        if (globaltimer() - t0 > kWaitLimitNs) {
+        if (globaltimer() - t0 >= limit) {
             *(volatile int *)dead = 1;
             return false;
         }
-    }
+    } while (!mbar_try_wait(bar, parity));
     return true;
 }
 
@@ -533,8 +535,8 @@ k_ba_prefix(const BaArgs a) {
         // the weights of tile t
         auto soft = [&](int t) {
             const int ring = t & (BT_RING - 1), n = min(G::BN, p1 - p0 - t * G::BN);
-            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.sc_full[ring], (t / BT_RING) & 1, &sh.dead) &&
-                                             bt_wait(&sh.s_full[t & 1], (t / 2) & 1, &sh.dead));
+            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.sc_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns) &&
+                                             bt_wait(&sh.s_full[t & 1], (t / 2) & 1, &sh.dead, a.wait_ns));
             if (!ok) return;
             tc_fence_after();
             const float4 *ks = reinterpret_cast<const float4 *>(sh.ks[ring]);
@@ -554,9 +556,9 @@ k_ba_prefix(const BaArgs a) {
         // tile t's output to the registers
         auto add = [&](int t) {
             const int ring = t & (BT_RING - 1);
-            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead) &&
-                                             (!F32 || bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead)) &&
-                                             bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead));
+            ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns) &&
+                                             (!F32 || bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns)) &&
+                                             bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead, a.wait_ns));
             if (!ok) return;
             tc_fence_after();
             if (rows_here) {
@@ -588,6 +590,7 @@ k_ba_prefix(const BaArgs a) {
         static_assert(BT_ROWS * PITCH * 4 <= G::V_AT, "rows of fp32 in the place of Q and K");
         float *rows = reinterpret_cast<float *>(smem);
         ok = bt_all<32 * BT_SOFT>(ok);
+        if (!ok && a.status && tid == 0) atomicOr(a.status, ST_WAIT_TIMEOUT);
 #pragma unroll
         for (int e = 0; e < NC / 4; e++)
             if (rows_here) *reinterpret_cast<float4 *>(rows + r * PITCH + c0 + 4 * e) =
@@ -627,7 +630,7 @@ k_ba_prefix(const BaArgs a) {
                     if (t + 1 < nt) x.prefetch(kb, p0 + (t + 1) * G::BN, left(t + 1));
                     x.wait();
                     const float km = ba_pow2(bt_feed_max<1>(x.max_k(), sh.wmax[0]));
-                    if (t) ok = bt_wait(&sh.k_empty[0], (t & 1) ^ 1, &sh.dead);
+                    if (t) ok = bt_wait(&sh.k_empty[0], (t & 1) ^ 1, &sh.dead, a.wait_ns);
                     if (!bt_all<128, 2>(ok)) break;
                     x.store_k(kt, G::K_TERM, 0x1p14f / km);
                     if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
@@ -643,7 +646,7 @@ k_ba_prefix(const BaArgs a) {
                     if (t + 1 < nt) x.prefetch(vb, p0 + (t + 1) * G::BN, left(t + 1));
                     x.wait();
                     const float vm = ba_pow2(bt_feed_max<4>(x.max_v(), sh.wmax[1]));
-                    if (t) ok = bt_wait(&sh.v_empty[0], (t & 1) ^ 1, &sh.dead);
+                    if (t) ok = bt_wait(&sh.v_empty[0], (t & 1) ^ 1, &sh.dead, a.wait_ns);
                     if (!bt_all<128, 5>(ok)) break;
                     x.store_v(vt, G::V_TERM, 0x1p14f / vm);
                     if (f == 0) sh.vscale[ring] = vm * 0x1p-14f * 0x1p-14f;
@@ -662,7 +665,7 @@ k_ba_prefix(const BaArgs a) {
             for (int t = 0; t < nt; t++) {
                 const int st = t & 1, ring = t & (BT_RING - 1);
                 const uint32_t free_parity = ((t / 2) & 1) ^ 1;
-                if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead);
+                if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead, a.wait_ns);
                 if (!bt_all<128, 2>(ok)) break;
                 x.template store_k<FMT>(smem + G::K_AT + st * G::K_STAGE);
                 const float vscale = ba_pow2(bt_feed_max<1>(fabsf(x.vs), sh.wmax[st]));
@@ -672,7 +675,7 @@ k_ba_prefix(const BaArgs a) {
                 mbar_arrive(&sh.k_full[st]);
                 mbar_arrive(&sh.sc_full[ring]);
                 if (t + 1 < nt) x.load_k(kb, ksc, vsc, p0 + (t + 1) * G::BN, left(t + 1));
-                if (t >= 2) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead);
+                if (t >= 2) ok = bt_wait(&sh.v_empty[st], free_parity, &sh.dead, a.wait_ns);
                 if (ok) {
                     x.template store_v<FMT>(smem + G::V_AT + st * G::V_STAGE);
                     fence_async_shared();
@@ -723,15 +726,15 @@ k_ba_prefix(const BaArgs a) {
         int n_s = 0, n_o = 0;      // tiles whose scores, outputs were issued
         for (int t = 0; t <= nt && ok; t++) {
             if (t < nt) {
-                ok = bt_wait(&sh.k_full[t % G::ST], (t / G::ST) & 1, &sh.dead);
+                ok = bt_wait(&sh.k_full[t % G::ST], (t / G::ST) & 1, &sh.dead, a.wait_ns);
                 tc_fence_after();
                 if (ok) scores(t), n_s++;
             }
             const int u = t - 1;
             if (u < 0 || !ok) continue;
-            ok = bt_wait(&sh.p_full[u & 1], (u / 2) & 1, &sh.dead) &&
-                 bt_wait(&sh.v_full[u % G::ST], (u / G::ST) & 1, &sh.dead) &&
-                 (u < 2 || bt_wait(&sh.o_empty[u & 1], ((u / 2) & 1) ^ 1, &sh.dead));
+            ok = bt_wait(&sh.p_full[u & 1], (u / 2) & 1, &sh.dead, a.wait_ns) &&
+                 bt_wait(&sh.v_full[u % G::ST], (u / G::ST) & 1, &sh.dead, a.wait_ns) &&
+                 (u < 2 || bt_wait(&sh.o_empty[u & 1], ((u / 2) & 1) ^ 1, &sh.dead, a.wait_ns));
             tc_fence_after();
             if (ok) output(u), n_o++;
         }

@@ -458,6 +458,17 @@ k_attention(const StepState *st, const float *__restrict__ qkv_part, int T, int 
     }
 }
 
+// Every device wait gives up after this long (default 2 s); KLLM_WAIT_LIMIT_MS
+// sets it, e.g. for a test that makes one run out (values below `least`: the
+// default).
+static unsigned long long wait_limit_ns(long long least) {
+    if (const char *e = getenv("KLLM_WAIT_LIMIT_MS")) {
+        const long long ms = *e >= '0' && *e <= '9' ? atoll(e) : -1;
+        if (ms >= least && ms <= 60000) return (unsigned long long)ms * 1000000ull;
+    }
+    return kWaitLimitNs;
+}
+
 // ================================================================ plan ===
 
 struct DecodePlan {
@@ -876,13 +887,7 @@ static bool persist_prepare(CtxImpl *c, DecodePlan *p, const std::vector<int> &t
         a.prof_pos = e ? atoi(e) : 100;
     }
 #endif
-    // every device wait of the step gives up after this long (default 2 s);
-    // KLLM_WAIT_LIMIT_MS shortens it, e.g. for a test that makes one run out
-    a.wait_ns = kWaitLimitNs;
-    if (const char *e = getenv("KLLM_WAIT_LIMIT_MS")) {
-        const long long ms = atoll(e);
-        if (ms > 0 && ms <= 60000) a.wait_ns = (unsigned long long)ms * 1000000ull;
-    }
+    a.wait_ns = wait_limit_ns(1);
     a.task_warps = p->task_warps;
     a.kv_prefetch = env_on("KLLM_KV_PREFETCH", true) ? 1 : 0;
     a.gpu_scope = env_on("KLLM_GPU_SCOPE", true) ? 1 : 0;
@@ -1563,7 +1568,9 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     kllm_kv_cache pfx = own;
     pfx.n_seq = 1;
     pfx.max_pos = std::max(P, 1);
-    kllm_batch_attn at = {};
+    BatchAttention att_call;
+    kllm_batch_attn &at = att_call.a;
+    at = {};
     at.n_seq = nseq;
     at.n_heads = nh;
     at.prefix_len = P;
@@ -1736,6 +1743,7 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
     // terms of each GEMM's input: 3 for the tensor cores, 0 (fp32) for the
     // exact TT-GEMM
     const int lt = layer_tc ? 3 : 0, lmt = lm_tc ? 3 : 0;
+    const unsigned long long wait_ns = wait_limit_ns(0);
     if (tc && !bd_gemm_prepare()) return false;
     const int ew_blocks = 148 * 8;
     auto att_for = [](auto hdc, int groups) {
@@ -1781,7 +1789,11 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
                 at.own_len = d_pos;
                 at.workspace = d_ws;
                 at.workspace_bytes = rws * 4;
-                if (!kv_append(s, a) || !batch_attention(s, at, lt, xs)) return false;
+                att_call.terms = lt;
+                att_call.terms_out = xs;
+                att_call.status = p->status;
+                att_call.wait_ns = wait_ns;
+                if (!kv_append(s, a) || !batch_attention(s, att_call)) return false;
             } else {
                 k_bd_rope_kv<<<dim3(nseq, 8), PF_THREADS, 0, s>>>(y, nz, d_pos, nq, nh, nkv, hd,
                                                                   p->rcos, p->rsin, mp, seq_stride,
@@ -1850,7 +1862,8 @@ bool plan_infer_batch(CtxImpl *c, const int *prompts, const int *lens, int nseq,
         !KLLM_CUDA(cudaStreamSynchronize(s)))
         return false;
     if (status) {
-        set_error("batched decode kernels reported status 0x%x", status);
+        set_error("batched decode kernels reported status 0x%x%s", status,
+                  (status & ST_WAIT_TIMEOUT) ? " (a wait timed out)" : "");
         return false;
     }
     for (int i = 0; i < nseq; i++) {

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace kllm {
 
@@ -25,10 +26,20 @@ bool kv_read(cudaStream_t s, const kllm_kv_cache &c, int rows, const int *seq, c
 
 // ------------------------------------------- batchattn.cu: attention -------
 
-// kllm_batch_attention, its output written as the next GEMM's input: fp32
-// rows (terms 0, `out` as the struct has it), or `terms` bf16 terms of the
-// exact split in planes of n_seq * n_heads * head_dim (batch.cuh, bd_emit).
-bool batch_attention(cudaStream_t s, const kllm_batch_attn &a, int terms, void *terms_out);
+// What kllm_batch_attention runs.  The output may be written as the next
+// GEMM's input: fp32 rows (terms 0, `out` as the struct has it), or `terms`
+// bf16 terms of the exact split in planes of n_seq * n_heads * head_dim
+// (rows.cuh, bd_emit).  A wait that takes longer than wait_ns gives up, leaves
+// NaN in the rows it was for and ST_WAIT_TIMEOUT in *status (may be null).
+struct BatchAttention {
+    kllm_batch_attn a;
+    int terms = 0;
+    void *terms_out = nullptr;
+    int *status = nullptr;
+    unsigned long long wait_ns = kWaitLimitNs;
+};
+
+bool batch_attention(cudaStream_t s, const BatchAttention &b);
 
 // ------------------------------------------------- sample.cu: the draw -----
 
