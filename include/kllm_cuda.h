@@ -288,6 +288,8 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  * that sees a position whose fp32 key or value is not finite, or whose scale
  * is NaN; no other row changes by it.  fp32 keys and values are taken to 22 bits, q and
  * p to 22.
+ * n_seq * n_heads and the positions (prefix_len, the smaller of max_len and
+ * own->max_pos) are at most 2^31 - 1024.
  * max_len is an upper bound of the own lengths (it sizes the launch, so a
  * captured graph serves every length up to it).  Positions past the lengths
  * are not read.  workspace: kllm_batch_attention_workspace(a) bytes on 16
@@ -307,8 +309,9 @@ typedef struct {
     size_t workspace_bytes;
 } kllm_batch_attn;
 
-/* Bytes of workspace the call needs (workspace and its size unread), or 0
- * for a call that kllm_batch_attention would refuse. */
+/* Bytes of workspace the call needs, or 0 with kllm_last_error() set for a
+ * call that kllm_batch_attention would refuse.  The workspace, its size, out
+ * and out_stride are not looked at. */
 size_t kllm_batch_attention_workspace(const kllm_batch_attn *a);
 int kllm_batch_attention(const kllm_batch_attn *a, void *stream);
 

@@ -173,7 +173,7 @@ k_ba_part(const BaArgs a) {
     }
     const int own = pre ? 0 : a.own_len[seq], len = pre ? a.prefix_len : min(own, a.own_cap);
     const BaSide &S = pre ? a.pre : a.own;
-    const int p0 = part * S.chunk, p1 = max(min(len, p0 + S.chunk), p0);
+    const int p0 = part * S.chunk, p1 = p0 + max(min(len - p0, S.chunk), 0);
     const bool join = a.join && !pre;
     if ((p0 >= p1 && !join) || own < 0) {
         pdl_wait();
@@ -578,7 +578,17 @@ struct BaCut {
     int nb = 1, nb_pre = 1; // a tile's query rows over four
     bool join = false;      // own positions in one part, joined where they are computed
     size_t rows = 0, bytes = 0;
+    long long pre_blocks = 0, own_blocks = 0;
 };
+
+// Most positions of a range: what the kernels and the cut count in 32 bits, with room for a piece's rounding.
+constexpr int BA_POSITIONS = 0x7ffffc00;
+
+// len positions (at most BA_POSITIONS) in n pieces of a multiple of 128, or fewer.
+void ba_pieces(int len, int n, int *parts, int *chunk) {
+    *chunk = ((len - 1) / n + 128) / 128 * 128;
+    *parts = (len - 1) / *chunk + 1;
+}
 
 // `items` ranges of up to len positions into parts of at least 128 positions
 // (a turn of each warp), as many as give every SM its two blocks twice over,
@@ -587,9 +597,7 @@ struct BaCut {
 void ba_split_range(long long items, int len, bool bound, int *parts, int *chunk) {
     const long long want = std::max<long long>(1, (148 * 4 + items - 1) / items);
     const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : 1;
-    const int n = (int)std::min(std::max(want, least), most);
-    *chunk = ((len + n - 1) / n + 127) / 128 * 128;
-    *parts = (len + *chunk - 1) / *chunk;
+    ba_pieces(len, (int)std::min(std::max(want, least), most), parts, chunk);
 }
 
 BaCut ba_cut(const kllm_batch_attn &a) {
@@ -622,9 +630,8 @@ BaCut ba_cut(const kllm_batch_attn &a) {
         const long long items = (long long)c->n_kv * x.tiles_pre;
         if (x.wide) {
             // one block an SM: as many parts as fill them once
-            const int n = (int)std::min<long long>(std::max<long long>(148 / items, 1), (pre + 127) / 128);
-            x.chunk_pre = ((pre + n - 1) / n + 127) / 128 * 128;
-            x.parts_pre = (pre + x.chunk_pre - 1) / x.chunk_pre;
+            ba_pieces(pre, (int)std::min<long long>(std::max<long long>(148 / items, 1), (pre + 127) / 128),
+                      &x.parts_pre, &x.chunk_pre);
         } else {
             ba_split_range(items, pre, false, &x.parts_pre, &x.chunk_pre);
         }
@@ -647,13 +654,16 @@ BaCut ba_cut(const kllm_batch_attn &a) {
             ba_split_range(items, x.own_cap, true, &x.parts_own, &x.chunk_own);
         }
     }
+    x.pre_blocks = (long long)c->n_kv * x.tiles_pre * x.parts_pre;
+    x.own_blocks = (long long)a.n_seq * c->n_kv * x.tiles_own * x.parts_own;
     x.rows = (size_t)a.n_seq * a.n_heads;
     const size_t parts = x.parts_pre + x.parts_own;
     x.bytes = ((x.rows * parts * 2 * 4 + 15) / 16 * 16) + x.rows * parts * c->head_dim * 4 + 16;
     return x;
 }
 
-bool ba_ok(const char *who, const kllm_batch_attn *a) {
+// Whether the call can be run, and its cut.
+bool ba_ok(const char *who, const kllm_batch_attn *a, BaCut *x) {
     if (!a || a->n_seq < 1 || a->n_heads < 1 || !a->q || (!a->prefix && !a->own)) {
         set_error("%s: invalid arguments", who);
         return false;
@@ -682,6 +692,17 @@ bool ba_ok(const char *who, const kllm_batch_attn *a) {
     }
     if (a->n_seq > 1 && a->q_stride < (long long)a->n_heads * c->head_dim) {
         set_error("%s: q_stride %lld for %d heads of %d", who, a->q_stride, a->n_heads, c->head_dim);
+        return false;
+    }
+    const int own = a->own ? std::min(a->max_len, a->own->max_pos) : 0;
+    if ((long long)a->n_seq * a->n_heads > 0x7fffffffll || std::max(a->prefix_len, own) > BA_POSITIONS) {
+        set_error("%s: %d sequences of %d heads, %d positions of a prefix and %d of their own are more than "
+                  "32 bits count", who, a->n_seq, a->n_heads, a->prefix_len, own);
+        return false;
+    }
+    *x = ba_cut(*a);
+    if (x->pre_blocks + x->own_blocks > 0x7fffffffll) {
+        set_error("%s: %lld blocks", who, x->pre_blocks + x->own_blocks);
         return false;
     }
     return true;
@@ -740,12 +761,6 @@ bool ba_launch(cudaStream_t s, const BatchAttention &call, const BaCut &x) {
     k.terms_out = call.terms_out;
     k.status = call.status;
     k.wait_ns = call.wait_ns;
-    const long long pre_blocks = (long long)k.nkv * x.tiles_pre * x.parts_pre;
-    const long long own_blocks = (long long)a.n_seq * k.nkv * x.tiles_own * x.parts_own;
-    if (pre_blocks + own_blocks > 0x7fffffffll || x.rows > 0x7fffffffull) {
-        set_error("kllm_batch_attention: %lld blocks", pre_blocks + own_blocks);
-        return false;
-    }
     // Each launch but the first may start beside the one before, and waits
     // for it where it needs it: the sequences' blocks before they join or end,
     // k_ba_merge at once.
@@ -768,7 +783,7 @@ bool ba_launch(cudaStream_t s, const BatchAttention &call, const BaCut &x) {
     if (x.wide) {
         constexpr size_t smem = bt_smem<HD, FMT>();
         if (!ba_prepare<k_ba_prefix<HD, FMT>>(smem) ||
-            !launch(k_ba_prefix<HD, FMT>, (unsigned)pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
+            !launch(k_ba_prefix<HD, FMT>, (unsigned)x.pre_blocks, BtGeom<HD, FMT>::THREADS, smem, k))
             return false;
     }
     auto part = [&](long long pre, long long own) {
@@ -782,8 +797,9 @@ bool ba_launch(cudaStream_t s, const BatchAttention &call, const BaCut &x) {
         return (pre ? x.nb_pre : x.nb) == 1 ? go(std::integral_constant<int, 1>())
                                             : go(std::integral_constant<int, 2>());
     };
-    const long long narrow = x.wide ? 0 : pre_blocks;
-    if (x.join || x.nb != x.nb_pre ? !part(narrow, 0) || !part(0, own_blocks) : !part(narrow, own_blocks)) return false;
+    const long long narrow = x.wide ? 0 : x.pre_blocks;
+    if (x.join || x.nb != x.nb_pre ? !part(narrow, 0) || !part(0, x.own_blocks) : !part(narrow, x.own_blocks))
+        return false;
     if (!x.join && !launch(k_ba_merge<HD>, (unsigned)((x.rows + 3) / 4), 128, 0, k)) return false;
     return KLLM_CUDA(cudaGetLastError());
 }
@@ -793,7 +809,8 @@ bool ba_launch(cudaStream_t s, const BatchAttention &call, const BaCut &x) {
 bool batch_attention(cudaStream_t s, const BatchAttention &b) {
     const char *who = "kllm_batch_attention";
     const kllm_batch_attn &a = b.a;
-    if (!ba_ok(who, &a)) return false;
+    BaCut x;
+    if (!ba_ok(who, &a, &x)) return false;
     if (!a.out && !b.terms_out) {
         set_error("%s: invalid arguments", who);
         return false;
@@ -803,7 +820,6 @@ bool batch_attention(cudaStream_t s, const BatchAttention &b) {
         set_error("%s: out_stride %lld for %d heads of %d", who, a.out_stride, a.n_heads, c->head_dim);
         return false;
     }
-    const BaCut x = ba_cut(a);
     if (!a.workspace || a.workspace_bytes < x.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 15)) {
         set_error("%s: %zu bytes of workspace on 16 bytes needed, %zu given", who, x.bytes,
                   a.workspace ? a.workspace_bytes : (size_t)0);
@@ -825,7 +841,8 @@ bool batch_attention(cudaStream_t s, const BatchAttention &b) {
 using namespace kllm;
 
 extern "C" size_t kllm_batch_attention_workspace(const kllm_batch_attn *a) {
-    return ba_ok("kllm_batch_attention_workspace", a) ? ba_cut(*a).bytes : 0;
+    BaCut x;
+    return ba_ok("kllm_batch_attention_workspace", a, &x) ? x.bytes : 0;
 }
 
 extern "C" int kllm_batch_attention(const kllm_batch_attn *a, void *stream) {

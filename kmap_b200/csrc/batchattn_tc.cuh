@@ -419,7 +419,7 @@ k_ba_prefix(const BaArgs a) {
     const int part = b % a.pre.parts;
     b /= a.pre.parts;
     const int tile = b % a.tiles_pre, kvh = b / a.tiles_pre;
-    const int p0 = part * a.pre.chunk, p1 = min(a.prefix_len, p0 + a.pre.chunk);
+    const int p0 = part * a.pre.chunk, p1 = p0 + min(a.prefix_len - p0, a.pre.chunk);
     const int nt = (p1 - p0 + G::BN - 1) / G::BN;
     const int n_rows = a.n_seq * a.groups;
 
