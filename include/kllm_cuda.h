@@ -284,6 +284,8 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  *   own_len[i] < 0      a padding row: out[i] is left as it was
  *   own_len[i] > own->max_pos or max_len: the smaller of those is taken
  *   no position at all  out[i] is zeros
+ * Scores are fp32 numbers (one past their range is an infinity); a row none of
+ * whose scores is above -infinity is NaN.
  * A row of q that holds an infinity or a NaN gets NaN, and so does every row
  * that sees a position whose fp32 key or value is not finite, or whose scale
  * is NaN; no other row changes by it.  fp32 keys and values are taken to 22 bits, q and

@@ -72,9 +72,10 @@ __device__ __forceinline__ uint32_t ba_transpose(uint32_t x) {
 }
 
 // The output of row (seq, h), by one warp, VEC = HD / 32 dims a lane: the join
-// of n parts from `at` on and one more (its maximum m, sum l and o).
+// of n parts from `at` on and, where `one`, one more (its maximum m, sum l and
+// o).
 template <int HD>
-__device__ __forceinline__ void ba_join(const BaArgs &a, long long at, int n, float m, float l,
+__device__ __forceinline__ void ba_join(const BaArgs &a, long long at, int n, bool one, float m, float l,
                                         float (&o)[HD / 32], int seq, int h, int lane) {
     constexpr int VEC = HD / 32;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
@@ -110,7 +111,7 @@ __device__ __forceinline__ void ba_join(const BaArgs &a, long long at, int n, fl
             for (int e = 0; e < VEC; e++) o[e] = fmaf(wp, v[e], o[e]);
         }
     }
-    const bool empty = n == 0 && none;
+    const bool empty = n == 0 && !one;
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         const float v = empty ? 0.f : o[e] / L;
@@ -544,7 +545,7 @@ k_ba_part(const BaArgs a) {
         const long long at = ((long long)rs * a.nh + rh) * parts;
         if (join) {
             pdl_wait();
-            ba_join<HD>(a, at, a.pre.parts, m, l, v, rs, rh, lane);
+            ba_join<HD>(a, at, a.pre.parts, p1 > p0, m, l, v, rs, rh, lane);
         } else {
             float *o = a.part_o + (at + pi) * HD + VEC * lane;
 #pragma unroll
@@ -567,7 +568,8 @@ k_ba_merge(const BaArgs a) {
     if (own < 0) return;
     const int n = a.pre.parts + (len > 0 ? (len + a.own.chunk - 1) / a.own.chunk : 0);
     float v[HD / 32] = {};
-    ba_join<HD>(a, (long long)R * (a.pre.parts + a.own.parts), n, -INFINITY, 0.f, v, seq, h, lane);
+    ba_join<HD>(a, (long long)R * (a.pre.parts + a.own.parts), n, false, -INFINITY, 0.f, v,
+                seq, h, lane);
 }
 
 // How a call is cut.
