@@ -1,0 +1,116 @@
+"""How many bits kllm_batch_attention keeps of queries, keys, weights and values,
+on inputs that leave its other roundings little to do.
+
+A query row has one element that is not zero, so a score is one product; each
+output dim has one position with a value (every position has one in the last dim
+besides, so that none is a row of zeros).  |s| <= 1.5.  Then out_d = p_j v_jd / L,
+relative to which, in units of 2^-24:
+  queries (2^-22 of the element) and keys (2^-21, cut to two terms) change a
+  score by 12 |s|, a weight and the sum L by that at most      2 x 18
+  three roundings of a score in log2 (|s| log2 e < 2.2), exp2    2 x 15
+  weight and value to two terms, their product without the
+  smallest (4 + 8 + 4), cut off while it is added (2 a term)         24
+  corrections by exp2 where the maximum moves, some 10               40
+  L: at most 64 additions a thread, 40 tiles, 74 parts              180
+in all 310 < 2^-24 x 2^8.3: the bound is 2^-15.5.  A form that leaves out the
+second term of any operand is off by up to 2^-11, which the last test shows on
+the host for these inputs."""
+import numpy as np
+import pytest
+
+TOL = 2.0 ** -15.5
+# (hd, nh, nkv, n, P): the few-row kernel, the 128-row tiles
+NARROW = [(128, 8, 2, 5, 300), (64, 8, 1, 3, 517), (32, 4, 4, 9, 1000)]
+WIDE = [(128, 8, 2, 64, 3001), (128, 4, 4, 129, 3000), (64, 8, 1, 41, 2500), (64, 8, 8, 33, 4100),
+        (32, 8, 2, 35, 3700)]
+
+
+def sparse(seed, hd, nh, nkv, n, P):
+    """q [n][nh][hd], k and v [nkv][P][hd] as above; dims 0..3 carry scores."""
+    rng = np.random.default_rng(seed)
+    q = np.zeros((n, nh, hd), np.float32)
+    at = rng.integers(0, 4, (n, nh))
+    i, h = np.mgrid[:n, :nh]
+    q[i, h, at] = rng.uniform(1, 1.5, (n, nh)) * rng.choice([-1, 1], (n, nh))
+    k = np.zeros((nkv, P, hd), np.float32)
+    k[..., :4] = rng.uniform(-1, 1, (nkv, P, 4))
+    v = np.zeros((nkv, P, hd), np.float32)
+    v[..., hd - 1] = rng.uniform(1, 2, (nkv, P))
+    for g in range(nkv):
+        v[g, rng.permutation(P)[:hd - 1], np.arange(hd - 1)] = rng.uniform(1, 2, hd - 1)
+    return q, k, v
+
+
+def exact(q, k, v):
+    """Output [n][nh][hd] and the mean of the rows' largest |v|, weighted as the output is, in 64 bits."""
+    n, nh, hd = q.shape
+    nkv = k.shape[0]
+    x = q.astype(np.float64).reshape(n, nkv, nh // nkv, hd)
+    out, norm = np.empty(x.shape), np.empty(x.shape[:3])
+    for g in range(nkv):
+        s = x[:, g] @ k[g].astype(np.float64).T
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[:, g], norm[:, g] = p @ v[g].astype(np.float64), p @ np.abs(v[g]).max(-1)
+    return out.reshape(n, nh, hd), norm.reshape(n, nh)
+
+
+def run(fmt, q, k, v, own=0):
+    """kllm_batch_attention of q on a prefix k, v but its last `own` positions, which every
+    sequence has in a cache of its own.  The output and the keys and values that the caches hold."""
+    import torch
+
+    import servecases as S
+    n, nh, hd = q.shape
+    nkv, P = k.shape[:2]
+    pre = S.Cache(fmt, 1, nkv, P - own, hd)
+    held = [pre.put(name, x[None, :, :P - own])[0] for name, x in (("k", k), ("v", v))]
+    mine = lens = None
+    if own:
+        mine = S.Cache(fmt, n, nkv, own, hd)
+        lens = S.dev(np.full(n, own, np.int32))
+        for j, (name, x) in enumerate((("k", k), ("v", v))):
+            y = mine.put(name, np.broadcast_to(x[None, :, P - own:], (n, nkv, own, hd)).copy())
+            held[j] = np.concatenate([held[j], y[0]], 1)
+    out = torch.zeros(n, nh * hd, device="cuda")
+    S.run_attention(S.dev(q.reshape(n, -1)), out, nh, 1.0, pre, P - own, mine, lens, own)
+    return out.cpu().numpy().astype(np.float64).reshape(q.shape), *held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", NARROW + WIDE)
+@pytest.mark.parametrize("own", [0, 3])
+def test_every_operand_keeps_its_second_term(gpu, fmt, hd, nh, nkv, n, P, own):
+    q, k, v = sparse(hd + n, hd, nh, nkv, n, P)
+    got, k, v = run(fmt, q, k, v, own)
+    want, _ = exact(q, k, v)
+    assert (np.abs(got - want) <= TOL * np.abs(want)).all()
+
+
+def _two(x, drop=False):
+    """Two terms of 11 bits, or one."""
+    hi = np.float16(x).astype(np.float64)
+    return hi if drop else hi + np.float16(x - hi).astype(np.float64)
+
+
+@pytest.mark.parametrize("hd,nh,nkv,n,P", NARROW + WIDE)
+def test_one_term_would_show(hd, nh, nkv, n, P):
+    """The bound on these inputs, on the host: met with two terms of everything, not with one term
+    of the queries, the keys, the weights or the values."""
+    q, k, v = sparse(hd + n, hd, nh, nkv, n, P)
+    want, _ = exact(q, k, v)
+    at = {}
+    for drop in (None, "q", "k", "p", "v"):
+        qq, kk, vv = (_two(x.astype(np.float64) * 2.0 ** 13, drop == name) * 2.0 ** -13
+                      for name, x in (("q", q), ("k", k), ("v", v)))
+        x = qq.reshape(n, nkv, nh // nkv, hd)
+        out = np.empty(x.shape)
+        for g in range(nkv):
+            s = x[:, g] @ kk[g].T
+            p = np.exp(s - s.max(-1, keepdims=True))
+            out[:, g] = _two(p * 2.0 ** 13, drop == "p") * 2.0 ** -13 @ vv[g] / p.sum(-1, keepdims=True)
+        err = np.abs(out.reshape(want.shape) - want)
+        at[drop] = (err[want != 0] / np.abs(want[want != 0])).max()
+    assert at.pop(None) < TOL / 8
+    assert min(at.values()) > 4 * TOL, at
