@@ -6,9 +6,9 @@
 //   scores  S[128][BN] = Q . K^T     two fp16 terms of q, keys as fp16
 //   weights P = 2^(S - m)            back into S's columns, two fp16 terms
 //   output  O[128][HD] = P . V       values as fp16, transposed
-// tile by tile of BN positions.  Codes of 8 bits are exact in fp16; an fp32
-// tile is brought to [2^13, 2^14) by a power of two and taken as two fp16
-// terms (22 bits).  O does not stay in tensor memory: the tensor core cuts
+// tile by tile of BN positions.  Codes of 8 bits are exact in fp16; fp32 keys
+// are brought to [2^13, 2^14) by a power of two of their own, fp32 values by
+// one of their tile's, and taken as two fp16 terms (22 bits).  O does not stay in tensor memory: the tensor core cuts
 // its sums off instead of rounding them, so each tile's O is added to fp32
 // registers, which is also where the running maximum's corrections and the
 // tile's value scale come in.
@@ -350,11 +350,24 @@ struct BtFeed32 {
     static __device__ __forceinline__ void prefetch(const uint8_t *b, int j0, int n) {
         for (int o = thread() * 128; o < n * HD * 4; o += 128 * 128) prefetch_l2_line(b + (long long)j0 * HD * 4 + o);
     }
-    __device__ __forceinline__ float max_k() const {
-        float m = 0.f;
+    // The power of two that brings a key to [2^13, 2^14) is its own; the inverse takes part in the scores
+    // as an 8-bit key's scale does.  A key's pieces are in PIECES lanes of a warp, of which lane e works
+    // it out for the warp's e-th keys and returns it.
+    __device__ __forceinline__ float scale_k(float *scale) const {
+        float mine = 0.f;
 #pragma unroll 8
-        for (int e = 0; e < NK; e++) m = fmaxf(m, most(reinterpret_cast<const float4 *>(raw_k)[e * 128 + thread()]));
-        return m;
+        for (int e = 0; e < NK; e++) {
+            float m = most(reinterpret_cast<const float4 *>(raw_k)[e * 128 + thread()]);
+            if constexpr (PIECES == 32) m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            else
+#pragma unroll
+                for (int o = PIECES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (thread() % PIECES == e) mine = m;
+        }
+        mine = ba_pow2(mine);
+        const int e = thread() % PIECES;
+        if (e < NK) scale[e * (128 / PIECES) + thread() / PIECES] = mine * 0x1p-14f;
+        return 0x1p14f / mine;
     }
     __device__ __forceinline__ float max_v() const {
         float m = 0.f;
@@ -367,11 +380,12 @@ struct BtFeed32 {
         }
         return m;
     }
-    __device__ __forceinline__ void store_k(uint8_t *tile, int term, float f) const {
+    __device__ __forceinline__ void store_k(uint8_t *tile, int term, float mine) const {
 #pragma unroll 8
         for (int e = 0; e < NK; e++) {
             const int q = e * 128 + thread(), r = q / PIECES, i = q % PIECES, blk = i >> 4;
             const float4 x = reinterpret_cast<const float4 *>(raw_k)[q];
+            const float f = __shfl_sync(0xffffffffu, mine, e, PIECES);
             uint2 h, l;
             ba_split(x.x * f, x.y * f, &h.x, &l.x);
             ba_split(x.z * f, x.w * f, &h.y, &l.y);
@@ -613,7 +627,8 @@ k_ba_prefix(const BaArgs a) {
         // --------------------------------------------------------- feeding --
         // Before the scales of a tile are written: the scores of tile t - ST are done.  They were issued
         // behind the output of tile t - 4 or a later one, which waited for all to be done with that of
-        // tile t - 6; so the ring's slot, tile t - 8's, is free.
+        // tile t - 6; so the ring's slot, tile t - 8's, is free.  (fp32 keys' are written before that wait:
+        // then the scores of tile t - 2 are done, issued behind the output of tile t - 4, as above.)
         const int f = tid & 127;
         const uint8_t *kb = static_cast<const uint8_t *>(a.pre.k) + row0 * HD * (F32 ? 4 : 1);
         const uint8_t *vb = static_cast<const uint8_t *>(a.pre.v) + row0 * HD * (F32 ? 4 : 1);
@@ -629,11 +644,11 @@ k_ba_prefix(const BaArgs a) {
                     const int ring = t & (BT_RING - 1);
                     if (t + 1 < nt) x.prefetch(kb, p0 + (t + 1) * G::BN, left(t + 1));
                     x.wait();
-                    const float km = ba_pow2(bt_feed_max<1>(x.max_k(), sh.wmax[0]));
+                    const float up = x.scale_k(sh.ks[ring]);      // (a free slot: above)
                     if (t) ok = bt_wait(&sh.k_empty[0], (t & 1) ^ 1, &sh.dead, a.wait_ns);
                     if (!bt_all<128, 2>(ok)) break;
-                    x.store_k(kt, G::K_TERM, 0x1p14f / km);
-                    if (f < G::BN) sh.ks[ring][f] = km * 0x1p-14f, sh.pv[ring][f] = 0x1p14f;
+                    x.store_k(kt, G::K_TERM, up);
+                    if (f < G::BN) sh.pv[ring][f] = 0x1p14f;
                     fence_async_shared();
                     mbar_arrive(&sh.k_full[0]);
                     mbar_arrive(&sh.sc_full[ring]);

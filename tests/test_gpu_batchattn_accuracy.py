@@ -114,3 +114,40 @@ def test_one_term_would_show(hd, nh, nkv, n, P):
         at[drop] = (err[want != 0] / np.abs(want[want != 0])).max()
     assert at.pop(None) < TOL / 8
     assert min(at.values()) > 4 * TOL, at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", NARROW + WIDE)
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 30, 2.0 ** 100])
+def test_a_key_beside_much_larger_ones(gpu, fmt, hd, nh, nkv, n, P, size):
+    """Every 16th key has a very large element where the queries have none: it changes
+    no score, and no other key's.
+
+    The 128-row tiles bring an fp32 key's largest element to [2^13, 2^14) and round its second
+    terms to multiples of 2^-24 there: the key's smaller elements are off by up to 2^-38 of the
+    largest, or are lost (a change by their score).  Such a position's weight is off by
+    e^d - 1, d = min(2^-38 size |q|, |s|) at most, and with L, of which it is 1 / 16, every
+    output by that times its share."""
+    q, k, v = sparse(hd + n, hd, nh, nkv, n, P)
+    k[:, 3::16, 5] = size
+    got, k, v = run(fmt, q, k, v)
+    want, _ = exact(q, k, v)
+    tol = np.full(want.shape, TOL)
+    if fmt == "f32" and (hd, nh, nkv, n, P) in WIDE:
+        x = q.astype(np.float64).reshape(n, nkv, nh // nkv, hd)
+        tol = tol.reshape(x.shape)
+        for g in range(nkv):
+            s = x[:, g] @ k[g].T
+            p = np.exp(s)
+            d = np.minimum(2.0 ** -38 * size * np.abs(x[:, g]).sum(-1), 1.5)[..., None] * (np.arange(P) % 16 == 3)
+            d = np.expm1(np.minimum(d, np.abs(s)))
+            share = (p * d).sum(-1, keepdims=True) / p.sum(-1, keepdims=True)
+            # the position that dim e's value comes from: its own weight is off too
+            own = np.zeros(x[:, g].shape)
+            for e in range(hd - 1):
+                own[..., e] = d[..., np.nonzero(v[g, :, e])[0][0]]
+            own[..., hd - 1] = 2 * share[..., 0]        # (values of 1 to 2 at every position)
+            tol[:, g] += own + share + own * share
+        tol = tol.reshape(want.shape)
+    assert (np.abs(got - want) <= tol * np.abs(want)).all()
