@@ -289,9 +289,9 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  * A row of q that holds an infinity or a NaN gets NaN, and so does every row
  * that sees a position whose fp32 key or value is not finite, or whose scale
  * is NaN; no other row changes by it.  q, p and fp32 keys and values are taken
- * to 22 bits; numbers of q and of a key that lie far below the largest of the
- * same head's row keep 2^-38 of that one at least, values 2^-38 of the largest
- * of 64 neighbouring positions.
+ * to 22 bits; numbers of a row of q, of a key or of a value that lie far below
+ * the largest of the same head_dim numbers keep 2^-38 of that one at least.
+ * Other positions and rows do not matter for that.
  * n_seq * n_heads and the positions (prefix_len, the smaller of max_len and
  * own->max_pos) are at most 2^31 - 1024.
  * max_len is an upper bound of the own lengths (it sizes the launch, so a

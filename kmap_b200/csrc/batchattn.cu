@@ -14,8 +14,10 @@
 // hi = rn(x), lo = rn(x - hi), and both go through one product as two columns
 // of the same operand.  Codes of 8 bits are exact in fp16; fp32 rows run as two tf32 terms each.
 // Scores carry scale * log2(e) * (the key row's scale); a weight carries the
-// value row's scale over the largest scale met so far (a power of two), so
-// p's fp16 terms stay in range whatever the scales are.
+// value row's scale, times a power of two that brings a query row's largest
+// p times scale so far to 2^14: p's fp16 terms, which end at 2^-24, stay in
+// range and lose nothing that counts beside it, whatever the scales of values
+// without weight are.
 #include <algorithm>
 #include <mutex>
 
@@ -256,11 +258,13 @@ k_ba_part(const BaArgs a) {
                 }
         }
     }
-    // of row 4 nb + i: maximum and sum; of the warp: the value scale in use (8-bit)
-    float m_run[NB], l_run[NB], sv = 0x1p-110f, o[NB][DT][4];
+    // of row 4 nb + i: maximum and sum; 8-bit: the largest log2 of a weight times its value's scale (to
+    // within a few 2^-20), and o in units of 2^-up
+    float m_run[NB], l_run[NB], w_run[NB], o[NB][DT][4];
+    int up[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        m_run[nb] = -INFINITY, l_run[nb] = 0.f;
+        m_run[nb] = w_run[nb] = -INFINITY, l_run[nb] = 0.f, up[nb] = 14;
 #pragma unroll
         for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -354,43 +358,44 @@ k_ba_part(const BaArgs a) {
                         if (r + 8 * e >= left) s[nb][t][e] = -INFINITY;
             }
         }
-        // the value rows' scales, relative to the largest met
-        float vs[NT][2], down = 1.f;
+        float vs[NT][2], lv[NT][2];      // the values' scales and their log2
         if constexpr (!F32) {
-            float most = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     vs[t][e] = vsc[16 * t + g + 8 * e];
-                    most = fmaxf(most, fabsf(vs[t][e]));
+                    lv[t][e] = ba_lg2(fabsf(vs[t][e]));
                 }
-            if (__any_sync(0xffffffffu, most >= sv)) {      // (of the warp: rare)
-#pragma unroll
-                for (int x = 16; x; x >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
-                const float up = fmaxf(sv, ba_pow2(most));
-                down = sv / up;
-                sv = up;
-            }
-            const float isv = 0x1p14f / sv;
-#pragma unroll
-            for (int t = 0; t < NT; t++) vs[t][0] *= isv, vs[t][1] *= isv;
         }
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
-            float mx = m_run[nb];
+            float mx = m_run[nb], wx = w_run[nb];
 #pragma unroll
-            for (int t = 0; t < NT; t++) mx = fmaxf(mx, fmaxf(s[nb][t][0], s[nb][t][1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            for (int t = 0; t < NT; t++) {
+                mx = fmaxf(mx, fmaxf(s[nb][t][0], s[nb][t][1]));
+                if constexpr (!F32) wx = fmaxf(wx, fmaxf(s[nb][t][0] + lv[t][0], s[nb][t][1] + lv[t][1]));
+            }
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                if constexpr (!F32) wx = fmaxf(wx, __shfl_xor_sync(0xffffffffu, wx, x));
+            }
             const float ref = mx == -INFINITY ? 0.f : mx, corr = ba_ex2(m_run[nb] - ref);
-            if (__any_sync(0xffffffffu, corr * down != 1.f)) {
+            float corr_o = corr;
+            if constexpr (!F32) {
+                // (scales between 2^-112 and 2^112: beyond, weights keep fewer bits)
+                const int to = wx == -INFINITY ? up[nb] : 14 + min(max(__float2int_rn(ref - wx), -112), 112);
+                corr_o *= ba_exp2i(min(max(to - up[nb], -126), 126));
+                up[nb] = to;
+                w_run[nb] = wx;
+            }
+            if (__any_sync(0xffffffffu, corr != 1.f || corr_o != 1.f)) {
                 l_run[nb] *= corr;
 #pragma unroll
                 for (int t = 0; t < DT; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[nb][t][e] *= corr * down;
+                    for (int e = 0; e < 4; e++) o[nb][t][e] *= corr_o;
             }
             m_run[nb] = mx;
 #pragma unroll
@@ -446,7 +451,7 @@ k_ba_part(const BaArgs a) {
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float p = s[nb][t][e] * vs[t][e];
+                        const float p = s[nb][t][e] * vs[t][e] * ba_exp2i(up[nb]);
                         const float h = __half2float(__float2half_rn(p));
                         pb[nb][e] = ba_transpose(ba_h2(h, p - h));
                     }
@@ -510,7 +515,7 @@ k_ba_part(const BaArgs a) {
 #pragma unroll
         for (int w = 1; w < W; w++) M = fmaxf(M, sm_ml[w][rr][0]);
         float f = m_run[nb] == -INFINITY ? 0.f : exp2f(m_run[nb] - M);
-        if constexpr (!F32) f *= sv * 0x1p-14f;
+        if constexpr (!F32) f *= ba_exp2i(-up[nb]);
 #pragma unroll
         for (int t = 0; t < DT; t++) {
             // dims of rows g and g + 8 of tile t

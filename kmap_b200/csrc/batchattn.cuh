@@ -54,6 +54,15 @@ __device__ __forceinline__ float ba_ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float ba_lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 2^n, n from -126 to 127
+__device__ __forceinline__ float ba_exp2i(int n) { return __int_as_float((n + 127) << 23); }
+
 // hi and lo fp16 terms of a pair
 __device__ __forceinline__ void ba_split(float a, float b, uint32_t *hi, uint32_t *lo) {
     const __half2 h = __floats2half2_rn(a, b);

@@ -6,12 +6,13 @@
 //   scores  S[128][BN] = Q . K^T     two fp16 terms of q, keys as fp16
 //   weights P = 2^(S - m)            back into S's columns, two fp16 terms
 //   output  O[128][HD] = P . V       values as fp16, transposed
-// tile by tile of BN positions.  Codes of 8 bits are exact in fp16; fp32 keys
-// are brought to [2^13, 2^14) by a power of two of their own, fp32 values by
-// one of their tile's, and taken as two fp16 terms (22 bits).  O does not stay in tensor memory: the tensor core cuts
-// its sums off instead of rounding them, so each tile's O is added to fp32
-// registers, which is also where the running maximum's corrections and the
-// tile's value scale come in.
+// tile by tile of BN positions.  Codes of 8 bits are exact in fp16; an fp32 key
+// or value is brought to [2^13, 2^14) by a power of two of its own and taken as
+// two fp16 terms (22 bits).  Keys' scales go to the scores, values' to the
+// weights.  O does not stay in tensor memory: the tensor core cuts its sums off
+// instead of rounding them, so each tile's O is added to fp32 registers, which
+// is also where the running maximum's corrections and the unit of the tile's
+// weights come in.
 //
 // Warps: two groups of four that take the tiles' softmax in turn (a row per
 // thread) and each keep half of O's columns; four that bring keys and values
@@ -79,11 +80,14 @@ struct BtShared {
     uint64_t sc_full[BT_RING], m_full[BT_RING], vs_full[BT_RING];
     uint32_t tmem;
     int dead;
-    float wmax[2][4];
-    float vscale[BT_RING];               // what O of the tile is in units of
+    uint2 range[2][4];
+    float vscale[BT_RING];               // what the tile's pv are in units of
+    int spread[BT_RING];                 // whether its value scales lie far apart
     float rowfac[BT_ROWS];
-    float mt[BT_RING][BT_ROWS], lt[BT_RING][BT_ROWS];     // a tile's maximum and sum of weights, per row
+    // a tile's maximum and sum of weights per row, and what O of the tile is in units of
+    float mt[BT_RING][BT_ROWS], lt[BT_RING][BT_ROWS], ot[BT_RING][BT_ROWS];
     alignas(16) float ks[BT_RING][128], pv[BT_RING][128];
+    alignas(16) float vu[64];            // fp32: the scales of the tile's values
 };
 
 template <int HD, int FMT>
@@ -127,11 +131,23 @@ __device__ __forceinline__ float bt_max16(const uint32_t (&x)[16], const float4 
     return mx;
 }
 
+// The largest p times its value's scale of 16 columns, and `most`.
+__device__ __forceinline__ float bt_most16(const uint32_t (&x)[16], const float *ks, const float *pv,
+                                           float fac, float ref, float most, int n) {
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        if (e < n) most = fmaxf(most, ba_ex2(__fmaf_rn(__uint_as_float(x[e]) * ks[e], fac, -ref)) * fabsf(pv[e]));
+    return most;
+}
+
 // 16 columns' weights p = 2^(score - ref) to the tensor memory: the fp16 terms
-// of p times their values' scales, the first in columns at.., the second 8
-// columns behind.  Returns the weights' sum with them.
+// of p times their values' scales (SPREAD: and times `up`), the first in
+// columns at.., the second 8 columns behind.  Returns the weights' sum with
+// them.
+template <bool SPREAD>
 __device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4 *ks, const float4 *pv,
-                                           float fac, float ref, float2 sum, bool cut, int n, uint32_t at) {
+                                           float fac, float ref, float up, float2 sum, bool cut, int n,
+                                           uint32_t at) {
     const float2 f = make_float2(fac, fac), r = make_float2(-ref, -ref), minus = make_float2(-1.f, -1.f);
 #pragma unroll
     for (int q = 0; q < 2; q++) {
@@ -154,6 +170,7 @@ __device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4
             sum = __fadd2_rn(sum, __fadd2_rn(p, w));
             p = __fmul2_rn(p, make_float2(v.x, v.y));
             w = __fmul2_rn(w, make_float2(v.z, v.w));
+            if (SPREAD) p.x *= up, p.y *= up, w.x *= up, w.y *= up;
             const __half2 ph = __float22half2_rn(p), wh = __float22half2_rn(w);
             const __half2 pl = __float22half2_rn(__ffma2_rn(__half22float2(ph), minus, p));
             const __half2 wl = __float22half2_rn(__ffma2_rn(__half22float2(wh), minus, w));
@@ -168,30 +185,55 @@ __device__ __forceinline__ float2 bt_exp16(const uint32_t (&x)[16], const float4
     return sum;
 }
 
-// The softmax of one row of a tile: scores in columns at.., their maximum (in
-// log2, *m) and the weights' sum relative to it; the weights' two terms take
-// the columns of their scores, 8 columns each for 16 positions.
+// The softmax of one row of a tile, its scores in columns at..: first their
+// maximum (before fac); the first 16 columns are on their way to `first` then.
 template <int BN, bool CUT>
-__device__ __forceinline__ void bt_soft(uint32_t at, const float4 *ks, const float4 *pv, float fac, int n,
-                                        float *m, float *sum) {
-    uint32_t s0[16], s1[16];
+__device__ __forceinline__ float bt_top(uint32_t at, const float4 *ks, int n, uint32_t (&first)[16]) {
+    uint32_t s1[16];
     float mx = -INFINITY;
-    tmem_ld16(at, s0);
+    tmem_ld16(at, first);
 #pragma unroll 1
     for (int c = 0; c < BN; c += 32) {
-        tmem_wait_ld16(s0);
+        tmem_wait_ld16(first);
         tmem_ld16(at + c + 16, s1);
-        mx = bt_max16(s0, ks + c / 4, mx, CUT, n - c);
+        mx = bt_max16(first, ks + c / 4, mx, CUT, n - c);
         tmem_wait_ld16(s1);
-        tmem_ld16(at + (c + 32) % BN, s0);       // behind the last, the first again
+        tmem_ld16(at + (c + 32) % BN, first);       // behind the last, the first again
         mx = bt_max16(s1, ks + c / 4 + 4, mx, CUT, n - c - 16);
     }
+    return mx;
+}
+
+// Then the weights relative to the maximum, in log2 *m, and their sum; their two
+// terms take the columns of their scores, 8 columns each for 16 positions.  pv
+// is in units of *unit.  The weights times pv have to be fp16 numbers, whose
+// terms end at 2^-24: with pv all near 2^13 that is far below the row's largest.
+// Where they lie apart (SPREAD), a row whose large values have no weight would
+// be left with nothing, so its own largest p pv is found first and brought to
+// [2^13, 2^14) (a third pass; *unit changes with it).
+template <int BN, bool CUT, bool SPREAD>
+__device__ __forceinline__ void bt_weights(uint32_t at, const float4 *ks, const float4 *pv, float fac, int n,
+                                           float mx, uint32_t (&s0)[16], float *m, float *sum, float *unit) {
     const float top = mx * fac, ref = top == -INFINITY ? 0.f : top;
+    float up = 1.f;
+    if constexpr (SPREAD) {
+        float most = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 16) {
+            tmem_wait_ld16(s0);
+            most = bt_most16(s0, reinterpret_cast<const float *>(ks) + c, reinterpret_cast<const float *>(pv) + c,
+                             fac, ref, most, n - c);
+            tmem_ld16(at + (c + 16) % BN, s0);
+        }
+        most = ba_pow2(most);
+        up = 0x1p14f / most;
+        *unit *= most * 0x1p-14f;
+    }
     float2 t = make_float2(0.f, 0.f);
 #pragma unroll 1
     for (int c = 0; c < BN; c += 16) {
         tmem_wait_ld16(s0);
-        t = bt_exp16(s0, ks + c / 4, pv + c / 4, fac, ref, t, CUT, n - c, at + c);
+        t = bt_exp16<SPREAD>(s0, ks + c / 4, pv + c / 4, fac, ref, up, t, CUT, n - c, at + c);
         if (c + 16 < BN) tmem_ld16(at + c + 16, s0);
     }
     *m = top;
@@ -203,16 +245,34 @@ __device__ __forceinline__ uint8_t *bt_at(uint8_t *tile, int r, int c) {
     return tile + r * 128 + ((c ^ (r & 7)) << 4);
 }
 
-// the largest |x| of the feeding warps' threads (all call it)
 template <int BAR>
-__device__ __forceinline__ float bt_feed_max(float m, float *wmax) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5 & 3] = m;
+__device__ __forceinline__ void bt_feed_bar() {
     asm volatile("bar.sync %0, 128;" ::"n"(BAR) : "memory");
+}
+
+// How a tile's value scales (four feeding warps, one or none, that is 0, a
+// thread; all call it) go to pv: times `by`, in units of `unit`.  Near one
+// another, the largest to [2^13, 2^14); with one 2^10 times another, as they are.
+struct BtScales {
+    float by, unit;
+    bool spread;
+};
+template <int BAR>
+__device__ __forceinline__ BtScales bt_feed_scales(float s, uint2 *range) {
+    const uint32_t b = __float_as_uint(s) & 0x7fffffffu;
+    // (zeros, one below which is the largest number, do not count for the smallest)
+    uint2 r = make_uint2(__reduce_max_sync(0xffffffffu, b), __reduce_min_sync(0xffffffffu, b - 1u));
+    if ((threadIdx.x & 31) == 0) range[threadIdx.x >> 5 & 3] = r;
+    bt_feed_bar<BAR>();
 #pragma unroll
-    for (int i = 0; i < 4; i++) m = fmaxf(m, wmax[i]);
-    return m;
+    for (int i = 0; i < 4; i++) r.x = max(r.x, range[i].x), r.y = min(r.y, range[i].y);
+    BtScales o = {1.f, 1.f, (int)(r.x >> 23) - (int)((r.y + 1u) >> 23) > 10};
+    if (!o.spread) {
+        const float most = ba_pow2(__uint_as_float(r.x));
+        o.by = 0x1p14f / most;
+        o.unit = most * 0x1p-14f;
+    }
+    return o;
 }
 
 // Whether all of a role's THREADS threads say yes (so that they leave their
@@ -369,16 +429,30 @@ struct BtFeed32 {
         if (e < NK) scale[e * (128 / PIECES) + thread() / PIECES] = mine * 0x1p-14f;
         return 0x1p14f / mine;
     }
-    __device__ __forceinline__ float max_v() const {
-        float m = 0.f;
+    // The same of the values: their scales to `scale` (0 for a row of zeros, NaN for one that is not
+    // finite); returns this thread's, or 0.  (All four warps' copies are there: this reads whole rows.)
+    __device__ __forceinline__ float scale_v(float *scale) const {
+        float mine = 0.f;
+#pragma unroll 8
+        for (int e = 0; e < NK; e++) {
+            const float4 x = reinterpret_cast<const float4 *>(raw_v)[e * 128 + thread()];
+            float m = max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(x.z), fabsf(x.w)));
+            if constexpr (PIECES == 32) m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            else
 #pragma unroll
-        for (int e = 0; e < NV; e++) {
-            const int t = e * 128 + thread();
-            if (t < ITEMS)
-#pragma unroll 4
-                for (int j = 0; j < 8; j++) m = fmaxf(m, most(*v_at((t & 7) * 8 + j, t >> 3)));
+                for (int o = PIECES / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (thread() % PIECES == e) mine = m;
         }
-        return m;
+        const int e = thread() % PIECES;
+        if (e >= NK) return 0.f;
+        mine = mine < INFINITY ? mine > 0.f ? ba_pow2(mine) * 0x1p-14f : 0.f : __uint_as_float(0x7fffffffu);
+        scale[e * (128 / PIECES) + thread() / PIECES] = mine;
+        return mine;
+    }
+    static __device__ __forceinline__ float max_nan(float a, float b) {
+        float c;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+        return c;
     }
     __device__ __forceinline__ void store_k(uint8_t *tile, int term, float mine) const {
 #pragma unroll 8
@@ -394,7 +468,7 @@ struct BtFeed32 {
             *reinterpret_cast<uint2 *>(a + term) = l;
         }
     }
-    __device__ __forceinline__ void store_v(uint8_t *tile, int term, float f) const {
+    __device__ __forceinline__ void store_v(uint8_t *tile, int term, const float *scale) const {
 #pragma unroll 1
         for (int e = 0; e < NV; e++) {
             const int t = e * 128 + thread(), pg = t & 7, dg = t >> 3;
@@ -403,10 +477,14 @@ struct BtFeed32 {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float4 x = *v_at(pg * 8 + 2 * i, dg), y = *v_at(pg * 8 + 2 * i + 1, dg);
-                ba_split(x.x * f, y.x * f, &h[0][i], &l[0][i]);
-                ba_split(x.y * f, y.y * f, &h[1][i], &l[1][i]);
-                ba_split(x.z * f, y.z * f, &h[2][i], &l[2][i]);
-                ba_split(x.w * f, y.w * f, &h[3][i], &l[3][i]);
+                // (the inverse of a power of two; of 0 it is 2^127, of NaN some number: p is NaN then)
+                const float2 s = *reinterpret_cast<const float2 *>(scale + pg * 8 + 2 * i);
+                const float f = __uint_as_float(0x7f000000u - __float_as_uint(s.x));
+                const float g = __uint_as_float(0x7f000000u - __float_as_uint(s.y));
+                ba_split(x.x * f, y.x * g, &h[0][i], &l[0][i]);
+                ba_split(x.y * f, y.y * g, &h[1][i], &l[1][i]);
+                ba_split(x.z * f, y.z * g, &h[2][i], &l[2][i]);
+                ba_split(x.w * f, y.w * g, &h[3][i], &l[3][i]);
             }
 #pragma unroll
             for (int d = 0; d < 4; d++) {
@@ -550,17 +628,24 @@ k_ba_prefix(const BaArgs a) {
         auto soft = [&](int t) {
             const int ring = t & (BT_RING - 1), n = min(G::BN, p1 - p0 - t * G::BN);
             ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.sc_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns) &&
+                                             (!F32 || bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns)) &&
                                              bt_wait(&sh.s_full[t & 1], (t / 2) & 1, &sh.dead, a.wait_ns));
             if (!ok) return;
             tc_fence_after();
             const float4 *ks = reinterpret_cast<const float4 *>(sh.ks[ring]);
             const float4 *pv = reinterpret_cast<const float4 *>(sh.pv[ring]);
+            const uint32_t at = s_cols(t) + lanes;
+            uint32_t first[16];
+            float mx = 0.f;
+            if (rows_here) mx = n == G::BN ? bt_top<G::BN, false>(at, ks, n, first) : bt_top<G::BN, true>(at, ks, n, first);
             if (rows_here) {
-                float m, sum;
-                if (n == G::BN) bt_soft<G::BN, false>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
-                else bt_soft<G::BN, true>(s_cols(t) + lanes, ks, pv, fac, n, &m, &sum);
+                float m, sum, unit = sh.vscale[ring];
+                if (sh.spread[ring]) bt_weights<G::BN, true, true>(at, ks, pv, fac, n, mx, first, &m, &sum, &unit);
+                else if (n == G::BN) bt_weights<G::BN, false, false>(at, ks, pv, fac, n, mx, first, &m, &sum, &unit);
+                else bt_weights<G::BN, true, false>(at, ks, pv, fac, n, mx, first, &m, &sum, &unit);
                 sh.mt[ring][r] = m;
                 sh.lt[ring][r] = sum;
+                sh.ot[ring][r] = unit;
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -571,13 +656,12 @@ k_ba_prefix(const BaArgs a) {
         auto add = [&](int t) {
             const int ring = t & (BT_RING - 1);
             ok = __all_sync(0xffffffffu, ok && bt_wait(&sh.m_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns) &&
-                                             (!F32 || bt_wait(&sh.vs_full[ring], (t / BT_RING) & 1, &sh.dead, a.wait_ns)) &&
                                              bt_wait(&sh.o_full[t & 1], (t / 2) & 1, &sh.dead, a.wait_ns));
             if (!ok) return;
             tc_fence_after();
             if (rows_here) {
                 const float m = sh.mt[ring][r], m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
-                const float corr = ba_ex2(m_run - ref), w = ba_ex2(m - ref), f = w * sh.vscale[ring];
+                const float corr = ba_ex2(m_run - ref), w = ba_ex2(m - ref), f = w * sh.ot[ring][r];
                 l_run = l_run * corr + sh.lt[ring][r] * w;
                 m_run = m_new;
 #pragma unroll
@@ -648,7 +732,6 @@ k_ba_prefix(const BaArgs a) {
                     if (t) ok = bt_wait(&sh.k_empty[0], (t & 1) ^ 1, &sh.dead, a.wait_ns);
                     if (!bt_all<128, 2>(ok)) break;
                     x.store_k(kt, G::K_TERM, up);
-                    if (f < G::BN) sh.pv[ring][f] = 0x1p14f;
                     fence_async_shared();
                     mbar_arrive(&sh.k_full[0]);
                     mbar_arrive(&sh.sc_full[ring]);
@@ -660,14 +743,18 @@ k_ba_prefix(const BaArgs a) {
                     const int ring = t & (BT_RING - 1);
                     if (t + 1 < nt) x.prefetch(vb, p0 + (t + 1) * G::BN, left(t + 1));
                     x.wait();
-                    const float vm = ba_pow2(bt_feed_max<4>(x.max_v(), sh.wmax[1]));
+                    bt_feed_bar<4>();
+                    // (the ring's slot is free: the output of tile t - 2 is done, issued when all were done
+                    // with that of tile t - 4)
+                    const BtScales vs = bt_feed_scales<4>(x.scale_v(sh.vu), sh.range[1]);
+                    if (f < G::BN) sh.pv[ring][f] = sh.vu[f] * vs.by;
+                    if (f == 0) sh.vscale[ring] = vs.unit, sh.spread[ring] = vs.spread;
+                    mbar_arrive(&sh.vs_full[ring]);
                     if (t) ok = bt_wait(&sh.v_empty[0], (t & 1) ^ 1, &sh.dead, a.wait_ns);
                     if (!bt_all<128, 5>(ok)) break;
-                    x.store_v(vt, G::V_TERM, 0x1p14f / vm);
-                    if (f == 0) sh.vscale[ring] = vm * 0x1p-14f * 0x1p-14f;
+                    x.store_v(vt, G::V_TERM, sh.vu);
                     fence_async_shared();
                     mbar_arrive(&sh.v_full[0]);
-                    mbar_arrive(&sh.vs_full[ring]);
                     if (t + 1 < nt) x.load_v(vb, p0 + (t + 1) * G::BN, left(t + 1));
                 }
             }
@@ -683,9 +770,9 @@ k_ba_prefix(const BaArgs a) {
                 if (t >= 2) ok = ok && bt_wait(&sh.k_empty[st], free_parity, &sh.dead, a.wait_ns);
                 if (!bt_all<128, 2>(ok)) break;
                 x.template store_k<FMT>(smem + G::K_AT + st * G::K_STAGE);
-                const float vscale = ba_pow2(bt_feed_max<1>(fabsf(x.vs), sh.wmax[st]));
-                sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * (0x1p14f / vscale);
-                if (f == 0) sh.vscale[ring] = vscale * 0x1p-14f;
+                const BtScales vs = bt_feed_scales<1>(x.vs, sh.range[st]);
+                sh.ks[ring][f] = x.ks, sh.pv[ring][f] = x.vs * vs.by;
+                if (f == 0) sh.vscale[ring] = vs.unit, sh.spread[ring] = vs.spread;
                 fence_async_shared();
                 mbar_arrive(&sh.k_full[st]);
                 mbar_arrive(&sh.sc_full[ring]);

@@ -151,3 +151,60 @@ def test_a_key_beside_much_larger_ones(gpu, fmt, hd, nh, nkv, n, P, size):
             tol[:, g] += own + share + own * share
         tol = tol.reshape(want.shape)
     assert (np.abs(got - want) <= tol * np.abs(want)).all()
+
+
+def _spread(seed, hd, nh, nkv, n, P):
+    """As sparse(), with dim 4 for scores that all query rows share."""
+    q, k, v = sparse(seed, hd, nh, nkv, n, P)
+    q[..., 4] = 1
+    return q, k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", NARROW + WIDE)
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 30, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("step", [16, 601])
+def test_values_beside_much_larger_ones_without_weight(gpu, fmt, hd, nh, nkv, n, P, size, step):
+    """Every 16th (or 601st) position has a very large value and a weight of e^-300: nothing
+    of it shows, and nothing of the others is lost."""
+    q, k, v = _spread(hd + n, hd, nh, nkv, n, P)
+    k[:, 3::step, 4] = -300
+    v[:, 3::step] = 0
+    v[:, 3::step, hd - 1] = size
+    got, k, v = run(fmt, q, k, v, 2)
+    want, _ = exact(q, k, v)
+    assert (np.abs(got - want) <= TOL * np.abs(want)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", NARROW + WIDE)
+def test_values_of_every_size(gpu, fmt, hd, nh, nkv, n, P):
+    """Value rows of 2^-30 to 2^30 whose weights nearly make up for it: every position counts.
+    Scores reach |s| = 21, where a score's roundings come to 2 (12 |s|) + 2 (3 |s| log2 e / 2) of the
+    units above, 595: with the 310 there less than 2^10, 2^-14 of the mean largest value."""
+    rng = np.random.default_rng(hd)
+    q, k, _ = _spread(hd + n, hd, nh, nkv, n, P)
+    e = rng.uniform(-30, 30, (nkv, P))
+    v = (rng.uniform(-1, 1, (nkv, P, hd)) * 2.0 ** e[..., None]).astype(np.float32)
+    k[..., :4] *= np.float32(0.2)
+    k[..., 4] = -0.9 * np.log(2) * e + rng.uniform(-1, 1, (nkv, P))
+    got, k, v = run(fmt, q, k, v, 3)
+    want, norm = exact(q, k, v)
+    assert (np.abs(got - want) <= 2.0 ** -14 * norm[..., None]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", [NARROW[0], WIDE[0]])
+def test_values_without_any(gpu, fmt, hd, nh, nkv, n, P):
+    """Rows of zeros among the values, a tile of them, and all of them."""
+    q, k, v = sparse(hd + n, hd, nh, nkv, n, P)
+    v[:, 5::7] = 0
+    v[:, :140] = 0
+    got, kk, vv = run(fmt, q, k, v, 3)
+    want, _ = exact(q, kk, vv)
+    assert (np.abs(got - want) <= TOL * np.abs(want)).all()
+    got, _, _ = run(fmt, q, k, 0 * v, 3)
+    assert (got == 0).all()
