@@ -291,7 +291,9 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  * is NaN; no other row changes by it.  q, p and fp32 keys and values are taken
  * to 22 bits; numbers of a row of q, of a key or of a value that lie far below
  * the largest of the same head_dim numbers keep 2^-38 of that one at least.
- * Other positions and rows do not matter for that.
+ * Other positions and rows do not matter for that.  Keys of 2^100 and more, and
+ * scores and |v| times the positions past fp32's range, may become infinities
+ * or NaN.
  * n_seq * n_heads and the positions (prefix_len, the smaller of max_len and
  * own->max_pos) are at most 2^31 - 1024.
  * max_len is an upper bound of the own lengths (it sizes the launch, so a

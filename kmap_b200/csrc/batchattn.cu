@@ -246,8 +246,8 @@ k_ba_part(const BaArgs a) {
             for (int d = 0; d < HD / 4; d++) m = fmaxf(m, fabsf(qx[nb][d]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float up = ba_pow2(m), f = 0x1p14f / up;
-            fac[nb] = __shfl_sync(0xffffffffu, a.qk * up * 0x1p-14f, 8 * i);
+            const float up = ba_pow2(m), f = 0x1p13f / up;
+            fac[nb] = __shfl_sync(0xffffffffu, a.qk * up * 0x1p-13f, 8 * i);
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ks++)
 #pragma unroll
@@ -384,8 +384,8 @@ k_ba_part(const BaArgs a) {
             const float ref = mx == -INFINITY ? 0.f : mx, corr = ba_ex2(m_run[nb] - ref);
             float corr_o = corr;
             if constexpr (!F32) {
-                // (scales between 2^-112 and 2^112: beyond, weights keep fewer bits)
-                const int to = wx == -INFINITY ? up[nb] : 14 + min(max(__float2int_rn(ref - wx), -112), 112);
+                // (an append's scales lie between 2^-109 and 2^120)
+                const int to = wx == -INFINITY ? up[nb] : 14 + min(max(__float2int_rn(ref - wx), -126), 112);
                 corr_o *= ba_exp2i(min(max(to - up[nb], -126), 126));
                 up[nb] = to;
                 w_run[nb] = wx;

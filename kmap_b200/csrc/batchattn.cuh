@@ -104,10 +104,11 @@ __device__ __forceinline__ void ba_mma_tf32(float (&d)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// the power of two above |x|'s, within the range whose inverse stays normal
+// The power of two that |x| lies above (to 2^126, which goes for all larger
+// numbers too): x times its inverse and 2^13 is below 2^15.
 __device__ __forceinline__ float ba_pow2(float x) {
-    const float c = fminf(fmaxf(x, 0x1p-110f), 0x1p110f);
-    return __uint_as_float((__float_as_uint(c) & 0x7f800000u) + 0x00800000u);
+    const float c = fminf(fmaxf(x, 0x1p-110f), 0x1p126f);
+    return __uint_as_float(__float_as_uint(c) & 0x7f800000u);
 }
 
 // Loads that stay where they are written (ahead of their use, which the

@@ -226,8 +226,8 @@ __device__ __forceinline__ void bt_weights(uint32_t at, const float4 *ks, const 
             tmem_ld16(at + (c + 16) % BN, s0);
         }
         most = ba_pow2(most);
-        up = 0x1p14f / most;
-        *unit *= most * 0x1p-14f;
+        up = 0x1p13f / most;
+        *unit *= most * 0x1p-13f;
     }
     float2 t = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -269,8 +269,8 @@ __device__ __forceinline__ BtScales bt_feed_scales(float s, uint2 *range) {
     BtScales o = {1.f, 1.f, (int)(r.x >> 23) - (int)((r.y + 1u) >> 23) > 10};
     if (!o.spread) {
         const float most = ba_pow2(__uint_as_float(r.x));
-        o.by = 0x1p14f / most;
-        o.unit = most * 0x1p-14f;
+        o.by = 0x1p13f / most;
+        o.unit = most * 0x1p-13f;
     }
     return o;
 }
@@ -426,8 +426,8 @@ struct BtFeed32 {
         }
         mine = ba_pow2(mine);
         const int e = thread() % PIECES;
-        if (e < NK) scale[e * (128 / PIECES) + thread() / PIECES] = mine * 0x1p-14f;
-        return 0x1p14f / mine;
+        if (e < NK) scale[e * (128 / PIECES) + thread() / PIECES] = mine * 0x1p-13f;
+        return 0x1p13f / mine;
     }
     // The same of the values: their scales to `scale` (0 for a row of zeros, NaN for one that is not
     // finite); returns this thread's, or 0.  (All four warps' copies are there: this reads whole rows.)
@@ -445,7 +445,7 @@ struct BtFeed32 {
         }
         const int e = thread() % PIECES;
         if (e >= NK) return 0.f;
-        mine = mine < INFINITY ? mine > 0.f ? ba_pow2(mine) * 0x1p-14f : 0.f : __uint_as_float(0x7fffffffu);
+        mine = mine < INFINITY ? mine > 0.f ? ba_pow2(mine) * 0x1p-13f : 0.f : __uint_as_float(0x7fffffffu);
         scale[e * (128 / PIECES) + thread() / PIECES] = mine;
         return mine;
     }
@@ -578,8 +578,8 @@ k_ba_prefix(const BaArgs a) {
             float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
 #pragma unroll
             for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float up = ba_pow2(m), f = 0x1p14f / up;
-            if (i == 0) sh.rowfac[r] = up * 0x1p-14f;
+            const float up = ba_pow2(m), f = 0x1p13f / up;
+            if (i == 0) sh.rowfac[r] = up * 0x1p-13f;
             uint2 h, l;
             ba_split(y.x * f, y.y * f, &h.x, &l.x);
             ba_split(y.z * f, y.w * f, &h.y, &l.y);

@@ -36,3 +36,32 @@ def test_no_score_above_minus_infinity_is_nan(gpu, fmt, P, m):
     out = torch.zeros(n, nh * hd, device="cuda")
     S.run_attention(S.dev(q.reshape(n, -1)), out, nh, 1.0, pre, P, own, lens, max(m, 1))
     assert np.isnan(out.cpu().numpy()).all()
+
+
+def _few(hd, nh, nkv, n, P, seed, qsize, ksize, vsize):
+    """Inputs of test_gpu_batchattn_accuracy's sparse() brought to other sizes, with one position of
+    30 above the others' scores for each query row's dims: sums of p |v| stay near the largest |v|."""
+    import test_gpu_batchattn_accuracy as A
+    q, k, v = A.sparse(seed, hd, nh, nkv, n, P)
+    q[..., 4] = 1
+    k[..., 4] = -30
+    k[:, P // 2, 4] = 0
+    q, k, v = (np.float32(x * s) for x, s in ((q, qsize), (k, ksize), (v, vsize)))
+    return q, k, v
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "f32"])
+@pytest.mark.parametrize("hd,nh,nkv,n,P", [(128, 8, 2, 5, 300), (128, 8, 2, 64, 3001), (64, 8, 8, 33, 4100)])
+@pytest.mark.parametrize("qsize,ksize,vsize", [
+    (1.0, 1.0, 2.0 ** 112), (1.0, 1.0, 2.0 ** 116), (1.0, 1.0, 2.0 ** -90),
+    (2.0 ** 95, 2.0 ** -95, 1.0), (2.0 ** 120, 2.0 ** -120, 1.0), (2.0 ** -90, 2.0 ** 90, 2.0 ** 116)])
+def test_large_finite_numbers(gpu, fmt, hd, nh, nkv, n, P, qsize, ksize, vsize):
+    """Queries up to 2^121, values up to 2^117: as near as of moderate size.  (Larger values are
+    documented to overflow: a part's sum of p |v|, p relative to the part's own largest score, is
+    up to its positions times |v|, 128 x 2^126 at the least.)"""
+    import test_gpu_batchattn_accuracy as A
+    q, k, v = _few(hd, nh, nkv, n, P, hd + n, qsize, ksize, vsize)
+    got, k, v = A.run(fmt, q, k, v, 2)
+    want, norm = A.exact(q, k, v)
+    # (scores reach 33: the 595 units of scores up to 21 there become 935, with the 310 2^-13.7)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -13.7 * norm[..., None]).all()
