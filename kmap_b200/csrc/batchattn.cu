@@ -407,9 +407,10 @@ k_ba_part(const BaArgs a) {
         }
         // P.V
         if constexpr (F32) {
+            constexpr int T8 = G::PT / 8;      // by 8 positions: rows i and i + 4 of them
+            uint32_t pb[T8][NB][2];
 #pragma unroll
-            for (int t = 0; t < G::PT / 8; t++) {      // 8 positions: rows i and i + 4 of them
-                uint32_t pb[NB][2];
+            for (int t = 0; t < T8; t++)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -417,11 +418,16 @@ k_ba_part(const BaArgs a) {
                         const float p = __shfl_sync(0xffffffffu, s[nb][t >> 1][t & 1], 4 * (i + 4 * e) + (g >> 1));
                         uint32_t h, l;
                         ba_split32(p, &h, &l);
-                        pb[nb][e] = g & 1 ? l : h;
+                        pb[t][nb][e] = g & 1 ? l : h;
                     }
-                const int r = 8 * t + i, tn = ba_turn<HD, FMT>(r);      // (the same of r + 4)
+            // (the turn's sum by itself: the tensor core cuts its sums off, always towards zero, and o would
+            // lose some 2^-25 of itself with each product)
 #pragma unroll
-                for (int u = 0; u < HD / 32; u++) {
+            for (int u = 0; u < HD / 32; u++) {
+                float d[NB][2][4] = {};
+#pragma unroll
+                for (int t = 0; t < T8; t++) {
+                    const int r = 8 * t + i, tn = ba_turn<HD, FMT>(r);      // (the same of r + 4)
                     const uint8_t *p = vt + r * G::ROW + (((8 * u + g) ^ tn) << 4);
                     const float4 x = *reinterpret_cast<const float4 *>(p);
                     const float4 y = *reinterpret_cast<const float4 *>(p + 4 * G::ROW);
@@ -438,10 +444,16 @@ k_ba_part(const BaArgs a) {
                     for (int e = 0; e < 2; e++)
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            ba_mma_tf32(o[nb][2 * u + e], l[e], pb[nb][0], pb[nb][1]);
-                            ba_mma_tf32(o[nb][2 * u + e], h[e], pb[nb][0], pb[nb][1]);
+                            ba_mma_tf32(d[nb][e], l[e], pb[t][nb][0], pb[t][nb][1]);
+                            ba_mma_tf32(d[nb][e], h[e], pb[t][nb][0], pb[t][nb][1]);
                         }
                 }
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[nb][2 * u + e][c] += d[nb][e][c];
             }
         } else {
 #pragma unroll
@@ -600,10 +612,12 @@ void ba_pieces(int len, int n, int *parts, int *chunk) {
 // `items` ranges of up to len positions into parts of at least 128 positions
 // (a turn of each warp), as many as give every SM its two blocks twice over,
 // and of at most 512 where the lengths are only bounds (blocks past a length
-// end at once, the others even out).
+// end at once, the others even out), else 2048: with 8 bits a warp's sums pass
+// through the tensor core with every 16 positions, which cuts off half a unit
+// of 2^-23 in the mean, always towards zero (over 14,500 positions a warp, 2^-16).
 void ba_split_range(long long items, int len, bool bound, int *parts, int *chunk) {
     const long long want = std::max<long long>(1, (148 * 4 + items - 1) / items);
-    const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : 1;
+    const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : (len + 2047) / 2048;
     ba_pieces(len, (int)std::min(std::max(want, least), most), parts, chunk);
 }
 

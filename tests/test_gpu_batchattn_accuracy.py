@@ -208,3 +208,46 @@ def test_values_without_any(gpu, fmt, hd, nh, nkv, n, P):
     assert (np.abs(got - want) <= TOL * np.abs(want)).all()
     got, _, _ = run(fmt, q, k, 0 * v, 3)
     assert (got == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,P", [("i8", 1000003), ("e4m3", 1000003), ("f32", 500003)])
+def test_sums_over_many_positions(gpu, fmt, P):
+    """The mean of a million values of one sign, all weights being one: additions that are cut
+    off instead of rounded lean one way and would add up.
+
+    A part's sum takes 32 cut additions (8 bits; fp32: four, its other sums are rounded), each
+    of at most 2^-23 of a partial sum that is half the whole in the mean: 2^-19.  Some 2^9 parts
+    and turns are added with roundings of either sign: six standard deviations of
+    2^-25 sqrt(2^9 / 3) are 2^-18.7.  Together less than 2^-17."""
+    import torch
+
+    import kmap_b200 as K
+    import servecases as S
+    nkv, hd = 32, 128
+    g = torch.Generator(device="cuda").manual_seed(3)
+    if fmt == "f32":
+        x = torch.rand(nkv, P, hd, generator=g, device="cuda") + 1
+        mean = torch.stack([x[h].sum(0, dtype=torch.float64) / P for h in range(nkv)])
+    else:
+        x = torch.randint(40, 120, (nkv, P, hd), generator=g, device="cuda", dtype=torch.uint8)
+        if fmt == "e4m3":      # codes of 0x40 to 0x50: 2 to 8
+            x = (x & 15) + 0x40
+        y = x.view(torch.int8 if fmt == "i8" else torch.float8_e4m3fn)
+        mean = torch.stack([y[h].float().sum(0, dtype=torch.float64) / P for h in range(nkv)])
+    scales = torch.full((nkv, P), 0.8, device="cuda")
+    c = K.KvCache(S.FORMATS[fmt], 1, nkv, hd, P, x.data_ptr(), x.data_ptr(), scales.data_ptr(), scales.data_ptr(),
+                  nkv * P * hd, nkv * P)
+
+    class Prefix:
+        pass
+    pre = Prefix()
+    pre.c = c
+    if fmt != "f32":
+        mean *= float(np.float32(0.8))
+    q, out = torch.zeros(1, nkv * hd, device="cuda"), torch.zeros(1, nkv * hd, device="cuda")
+    S.run_attention(q, out, nkv, 1.0, pre, P)
+    err = ((out.view(nkv, hd).double() - mean) / mean).abs().max().item()
+    del x, scales, pre, c
+    torch.cuda.empty_cache()
+    assert err <= 2.0 ** -17
