@@ -633,18 +633,18 @@ BaCut ba_cut(const kllm_batch_attn &a) {
         const long long rows = (long long)a.n_seq * groups;
         // The 128-row tiles have a start of some 12 us and little time per row, the narrow tiles 6 us and
         // theirs per row: which ends first goes with positions x rows x kv heads, and 24 rows leave the
-        // wide tiles too empty.  Measured, narrow and wide, in us:
-        //   8 bits  head dim 128, 32 kv heads: 32 rows x 2000  36.7 36.6, 48 x 1000  36.9 37.6, 64 x 1000
-        //           45 43, 64 x 4000  81 65, 24 x 4000  38 47; 8 kv heads: 32 x 4000  16.6 20.1, 48 x 4000
-        //           24 22; head dim 64, 4 kv heads: 256 x 500  15.1 15.7, 192 x 1000  14.1 14.4, 256 x 1000
-        //           17 14, 128 x 1000  13.7 14.3, 32 x 1000  8.2 12.5
-        //   fp32    head dim 128, 32 kv heads: 16 x 4000  56 66, 24 x 4000  88 67, 24 x 1000  31 33, 32 x
-        //           1000  42 37; head dim 64, 4 kv heads: 128 x 1000  16 19, 192 x 1000  23 19
+        // wide tiles too empty.  Measured, narrow and wide, in us (with one own position each):
+        //   e4m3    head dim 128, 32 kv heads: 32 rows x 2000  36.0 35.4, 48 x 1000  35.6 36.1, 64 x 1000
+        //           44 42, 64 x 4000  81 59, 24 x 4000  39 43; 8 kv heads: 32 x 4000  16.5 19.4, 48 x 4000
+        //           24 21; head dim 64, 4 kv heads: 256 x 500  14.1 15.5, 192 x 1000  12.8 14.1, 256 x 1000
+        //           15.9 14.1, 128 x 1000  12.6 14.1, 32 x 1000  7.9 12.4
+        //   fp32    head dim 128, 32 kv heads: 16 x 4000  60 76, 24 x 4000  92 76, 24 x 1000  31 32, 32 x
+        //           1000  43 35; head dim 64, 4 kv heads: 128 x 1000  16 19, 192 x 1000  23 19
         const long long work = c->n_kv * rows * pre;
         x.wide = c->format == KLLM_KV_F32 ? rows >= 24 && work >= 1000000
                                           : rows >= 32 && work >= 12000ll * c->head_dim;
         // fp32 tiles are read once per tile: eight rows as soon as there are more than four (24 rows x 4000
-        // as above: 89 us, 95 in tiles of four)
+        // as above: 91 us, 96 in tiles of four)
         x.nb_pre = c->format == KLLM_KV_F32 ? (rows > 4 ? 2 : 1) : x.nb;
         const int t = x.wide ? BT_ROWS : 4 * x.nb_pre;
         x.tiles_pre = (int)((rows + t - 1) / t);
@@ -662,9 +662,9 @@ BaCut ba_cut(const kllm_batch_attn &a) {
         const long long items = (long long)a.n_seq * c->n_kv * x.tiles_own;
         // One part, joined where it is computed (no launch for the join), where a block's keys are few, or
         // the blocks as many as they are KB: measured, more parts and one, in us, after 64 positions of a
-        // prefix: head dim 128, 8 kv heads of 8 bits, 512 positions: 1 sequence 7.8 8.7, 8 sequences 10.1
-        // 9.3, 48 20 17; 1000: 8 sequences 11.8 12.4, 16 15.0 12.2; 128: 1 sequence 6.5 6.2; 32 kv heads of
-        // fp32, 64: 6.9 6.3; 256: 1 sequence 9.0 11.4, 8 19.6 13.7; 1000: 4 20 34, 16 55 55.  Above 1024
+        // prefix: head dim 128, 8 kv heads of int8, 512 positions: 1 sequence 7.4 8.2, 8 sequences 9.8
+        // 8.8, 48 19 16; 1000: 8 sequences 11.5 11.7, 16 14.7 12.1; 128: 1 sequence 6.3 5.6; 32 kv heads of
+        // fp32, 64: 6.9 6.3; 256: 1 sequence 8.8 11.7, 8 19.8 12.2; 1000: 4 19 33, 16 54 57.  Above 1024
         // positions lengths differ enough for parts to even them out.
         const long long kb = (long long)x.own_cap * c->head_dim * (c->format == KLLM_KV_F32 ? 4 : 1) / 1024;
         if (kb <= 32 || (x.own_cap <= 1024 && items >= kb)) {

@@ -31,19 +31,20 @@
 // the block gives its memory back, on that path too.
 //
 // Bound: of a tile of 128 positions of 8 bits (16.8 MFLOP with two terms) the
-// products take some 2900 cycles, the bytes 1600 of an SM's share of the
-// memory's; a tile takes 5700: of the two groups' 11400 each, 1400 are the
-// maxima's, 4800 the weights', 1200 O's, the rest waiting for products that
-// wait for weights.  Taking the weights four rows a lane (a quarter of the
-// scales' reads), their first terms without a conversion back, or their loads
-// a step ahead measured the same 79 us as below; 16 softmax warps 109 (80
-// registers).  256 rows x
-// 16384 positions of 8 kv heads of 128, e4m3, two tiles of rows: 77 us in all
-// (17.2 GFLOP: 0.22 PFLOP/s, 0.45 as issued in two terms).  An fp32 tile of
-// 64 positions takes 5700 cycles too: its keys' conversion and the three
-// products of its scores follow one another (one buffer of keys: two, with the
-// queries in tensor memory, measured the same).  24 rows x 4000 positions of
-// 32 kv heads of 128, fp32: 55 us (131 MB, 2.4 TB/s).
+// products take some 1900 cycles (the tensor pipe is active 27 % of the
+// kernel's time), the bytes 1600 of an SM's share of the memory's; a tile takes
+// some 5700: of the two groups' 11400 each, 1400 are the maxima's, 4800 the
+// weights', 1200 O's, the rest waiting for products that wait for weights.
+// Taking the weights four rows a lane (a quarter of the scales' reads), their
+// first terms without a conversion back, or their loads a step ahead measured
+// the same; 16 softmax warps were a third slower (80 registers).  256 rows x
+// 16384 positions of 8 kv heads of 128, e4m3, two tiles of rows: 75 us in all
+// (17.2 GFLOP: 0.23 PFLOP/s, 0.46 as issued in two terms).  An fp32 tile's
+// keys' conversion and the three products of its scores follow one another (one
+// buffer of keys: two, with the queries in tensor memory, measured the same),
+// and its weights wait for the values' scales.  24 rows x 4000 positions of 32
+// kv heads of 128, fp32: 62 us (131 MB, 2.1 TB/s); 52 before keys and values
+// had scales of their own.
 #pragma once
 
 #include "batchattn.cuh"

@@ -10,15 +10,16 @@
 // turned first, with the tape's float arithmetic (rotate-half RoPE:
 // fl(fl(y cos) + fl(y' sin))).
 //
-// Bound by memory: each value is loaded once and leaves as one byte.  A row
+// Bound by memory, 8-bit appends by instructions: each value is loaded once and
+// leaves as one byte.  A row
 // lives in head_dim / 4 lanes, four values each, so its loads (16 bytes a
 // lane) and its code stores (4 bytes a lane) are whole 128-byte lines; the
 // rotation's partner values and the row's maximum come by shuffles.
-// Measured: 4095 positions of 32 heads of 128, 8 bits: appended in 72 us
-// (301 MB, 4.2 TB/s: between a row's loads and its stores lie the rotation,
-// the maximum over its lanes and the division, and registers keep the warps
-// that could cover that to 24 an SM), read back in 26 us (169 MB, 6.5 TB/s).
-// 32 rows of 48 heads: 4.0 us for both, two launches.
+// Measured: 4095 positions of 32 heads of 128, 8 bits: appended in 70 us
+// (307 MB, 4.4 TB/s: instructions, 76 % of the issue slots; the rotation, the
+// maximum over a row's lanes, the division and the codes), read back in 28 us
+// (169 MB, 6.0 TB/s); fp32 65 us (407 MB, 6.3 TB/s) and 43 us (268 MB, 6.2).
+// 32 rows of 48 heads: 3.9 us for both, two launches.
 #include <cuda_fp8.h>
 #include <float.h>
 

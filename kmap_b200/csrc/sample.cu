@@ -28,12 +28,14 @@
 // Histograms are summed over the cluster by every block for itself
 // (distributed shared memory): one cluster barrier a step.
 //
-// Bound: a row's 4 vocab bytes are read once; past that, instructions: some
-// 30 a weight, and a weight a token where all are needed (top-p alone, plain
-// temperature), another for the kept ones; few rows wait for the chain of
-// dependent steps.  Measured: 1 row of 32000 tokens 17 us, 32 rows of 128256
-// (a mix of settings) 45 us, 128 rows of 128256 with top-p and many equal
-// logits 209 us (0.3 TB/s: instructions, in step 4b).
+// Bound: a row's 4 vocab bytes are read once; past that, some 30 instructions
+// a weight, a weight a token where all are needed (top-p alone, plain
+// temperature) and another for the kept ones, between barriers that wait for a
+// row's slowest warp: two blocks an SM use 43 % of the issue slots, and the
+// barriers are the longest stall.  Few rows wait for the chain of dependent
+// steps.  Measured: 1 row of 32000 tokens 17 us, 32 rows of 128256 (a mix of
+// settings) 45 us, 128 rows of 128256 with top-p and many equal logits 192 to
+// 208 us (0.3 TB/s, in step 4b).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -911,7 +913,7 @@ bool sample_rows(cudaStream_t s, const kllm_sample_rows &r, int nz, long long pl
     // of 16000: 19.5, 16.6 with two, 15.7 with four, 16.5 with eight), and fewer where all rows' are more
     // than one an SM, a block's fixed work being that of some 2000 tokens (128 rows of 32000: 81 us with
     // one, 38 with two, 47 with four, 68 with eight; 32 rows: 64, 35, 26, 29), but slices of 64 KB at
-    // most, three an SM (128 rows of 128256: 128 us with eight, 172 with four).
+    // most, two blocks an SM (128 rows of 128256: 128 us with eight, 172 with four).
     int C = SA_CL;
     while (C > 1 && r.vocab <= C * 2048) C /= 2;
     auto cost = [&](int c) { return std::max(148ll, (long long)r.rows * c) * (2000 + r.vocab / c); };
