@@ -617,7 +617,7 @@ void ba_pieces(int len, int n, int *parts, int *chunk) {
 // of 2^-23 in the mean, always towards zero (over 14,500 positions a warp, 2^-16).
 void ba_split_range(long long items, int len, bool bound, int *parts, int *chunk) {
     const long long want = std::max<long long>(1, (148 * 4 + items - 1) / items);
-    const long long most = (len + 127) / 128, least = bound ? (len + 511) / 512 : (len + 2047) / 2048;
+    const long long most = (len + 127) / 128, least = (len - 1) / (bound ? 512 : 2048) + 1;
     ba_pieces(len, (int)std::min(std::max(want, least), most), parts, chunk);
 }
 

@@ -77,3 +77,10 @@ def test_nearly_2_to_31_positions(gpu, n):
     del codes, scales
     torch.cuda.empty_cache()
     assert (np.abs(got - want) <= 2.0 ** -14 * want).all()
+
+
+def test_parts_are_bounded_up_to_the_limit(built_lib):
+    """A prefix's parts hold at most 2048 positions (32 floats, a maximum and a sum each)."""
+    for P in (1 << 20, 1 << 30, 0x7ffffc00 - 1, 0x7ffffc00):
+        a, _kv = _call(1, 1, P, True)
+        assert built_lib.kllm_batch_attention_workspace(C.byref(a)) >= (P + 2047) // 2048 * 34 * 4
