@@ -211,7 +211,8 @@ __device__ __forceinline__ float bt_top(uint32_t at, const float4 *ks, int n, ui
 // terms end at 2^-24: with pv all near 2^13 that is far below the row's largest.
 // Where they lie apart (SPREAD), a row whose large values have no weight would
 // be left with nothing, so its own largest p pv is found first and brought to
-// [2^13, 2^14) (a third pass; *unit changes with it).
+// [2^13, 2^14) (a third pass; *unit changes with it).  With every tile's scales
+// apart: 64 sequences x 16384 e4m3 99 us for 74, 24 x 4000 fp32 105 for 92.
 template <int BN, bool CUT, bool SPREAD>
 __device__ __forceinline__ void bt_weights(uint32_t at, const float4 *ks, const float4 *pv, float fac, int n,
                                            float mx, uint32_t (&s0)[16], float *m, float *sum, float *unit) {
