@@ -287,8 +287,9 @@ int kllm_kv_read(const kllm_kv_cache *cache, int rows, const int *seq, const int
  * Scores are fp32 numbers (one past their range is an infinity); a row none of
  * whose scores is above -infinity is NaN.
  * A row of q that holds an infinity or a NaN gets NaN, and so does every row
- * that sees a position whose fp32 key or value is not finite, or whose scale
- * is NaN; no other row changes by it.  q, p and fp32 keys and values are taken
+ * that sees a position whose fp32 key or value is not finite (of a value, in
+ * its dim at least), or whose scale is NaN; no other row changes by it.
+ * q, p and fp32 keys and values are taken
  * to 22 bits; numbers of a row of q, of a key or of a value that lie far below
  * the largest of the same head_dim numbers keep 2^-38 of that one at least.
  * Other positions and rows do not matter for that.  Keys of 2^100 and more, and

@@ -65,3 +65,27 @@ def test_large_finite_numbers(gpu, fmt, hd, nh, nkv, n, P, qsize, ksize, vsize):
     want, norm = A.exact(q, k, v)
     # (scores reach 33: the 595 units of scores up to 21 there become 935, with the 310 2^-13.7)
     assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -13.7 * norm[..., None]).all()
+
+
+@pytest.mark.parametrize("n,P", [(5, 300), (50, 2700)])
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+def test_one_number_of_a_value_that_is_not_finite(gpu, n, P, bad):
+    """An fp32 value with one such number: NaN in that dim for every row of its kv head; the other dims
+    are NaN or what they were, and never something else."""
+    import torch
+
+    import servecases as S
+    rng = np.random.default_rng(3)
+    nh, nkv, hd = 8, 2, 64
+    pre = S.Cache("f32", 1, nkv, P, hd)
+    for name in "kv":
+        pre.put(name, rng.standard_normal((1, nkv, P, hd)).astype(np.float32))
+    q = S.dev(rng.standard_normal((n, nh * hd)).astype(np.float32))
+    a, b = (torch.zeros(n, nh * hd, device="cuda") for _ in "ab")
+    S.run_attention(q, a, nh, 0.125, pre, P)
+    pre.v.view(-1)[(P // 2) * hd + 7] = float(bad)
+    S.run_attention(q, b, nh, 0.125, pre, P)
+    a, b = (t.cpu().numpy().reshape(n, nh, hd) for t in (a, b))
+    head = np.arange(nh) < nh // nkv
+    assert np.isnan(b[:, head, 7]).all() and np.array_equal(a[:, ~head], b[:, ~head])
+    assert (np.isnan(b[:, head]) | (a[:, head] == b[:, head])).all()
